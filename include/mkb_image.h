@@ -187,6 +187,57 @@ mkb_status mkb_attention_kv_arriving(const void* q, int Lq, int Lq_rows, const v
                                      const unsigned long long* shard_ready, const unsigned long long* shard_expect,
                                      void* stream);
 
+/* ---- A quantised, prompt-conditioned block: residual norms, 8-bit integer projections and attention to another stream's
+ * keys. No counterpart in the reference. Forward only, like everything here. */
+
+/* Rows to 8-bit integers: scale[r] = max |x[r]| / 127 (fp32) and q[r][i] = x[r][i] / scale[r] rounded to the nearest whole
+ * number, ties to even (decided exactly). x is bf16 (x_f32 = 0) or fp32, rows ldx apart; q rows ldq apart. A row of zeros,
+ * or with no magnitude above 127 * 2^-126, has scale 0 and zeros; a row holding an infinity or a NaN has scale NaN and
+ * zeros, so that a projection of it is NaN. Any n up to 2^24. */
+mkb_status mkb_quantize_rows(const void* x, long ldx, int x_f32, int8_t* q, long ldq, float* scale, long rows, int n,
+                             void* stream);
+
+/* y[m][n] = act(x_scale[m] * w_scale[n] * sum_k x[m][k] w[n][k] + bias[n]): mkb_proj on 8-bit integers, with the scale of
+ * each token (mkb_quantize_rows of the activations) and of each output channel (mkb_quantize_rows of the weight's rows).
+ * The sums are exact 32-bit integers (K <= 131071). x and w are 16-byte aligned with ldx and ldw multiples of 16 (K itself
+ * may be any: what lies between K and the row's end is not read as data); y is bf16 (out_f32 = 0) or fp32, any ldy >= N. */
+mkb_status mkb_proj_i8(const int8_t* x, long ldx, const float* x_scale, const int8_t* w, long ldw, const float* w_scale,
+                       const float* bias, void* y, long ldy, int M, int N, int K, int act, int out_f32, void* stream);
+
+/* Norms of mkb_gate_add_norm: none, t / rms(t), (t - mean) / std(t) (both with eps inside the root). */
+enum { MKB_NORM_NONE = 0, MKB_NORM_RMS = 1, MKB_NORM_LAYER = 2 };
+/* What it leaves of the next branch's input: nothing, bf16, fp32, 8-bit integers as mkb_quantize_rows makes them. */
+enum { MKB_OUT_NONE = 0, MKB_OUT_BF16 = 1, MKB_OUT_F32 = 2, MKB_OUT_I8 = 3 };
+
+/* The end of one branch of a block and the start of the next, in one pass over the rows:
+ *   x_out = x + g(gate) * N_y(y) * y_weight         (g: identity, or tanh with tanh_gate)
+ *   out   = N_x(x_out) * x_weight * (1 + scale) + shift
+ * x, x_out: the fp32 residual stream [rows][n] (x_out may be x; NULL or x where y is NULL, which leaves the residual as it
+ * is and only norms it). y: the branch's output, bf16 or fp32 (y_f32). y_weight and x_weight [n], gate, scale and shift
+ * (those of sample row / rows_per_sample at gate + sample * gate_stride, scale + sample * mod_stride and shift + sample *
+ * mod_stride) are fp32 and may each be NULL. out is written as out_type says, with out_scale [rows] for MKB_OUT_I8 (else
+ * NULL). Statistics are fp32, a LayerNorm's squares are taken about its mean. n up to 12288, any alignment (16-byte aligned
+ * rows and vectors with n a multiple of 4 take wide accesses). */
+mkb_status mkb_gate_add_norm(const float* x, long ldx, float* x_out, long ldxo, const void* y, long ldy, int y_f32,
+                             int y_norm, const float* y_weight, const float* gate, long gate_stride, int tanh_gate,
+                             int x_norm, const float* x_weight, const float* scale, const float* shift, long mod_stride,
+                             long rows_per_sample, float eps, void* out, long ldo, int out_type, float* out_scale,
+                             long rows, int n, void* stream);
+
+/* Cross attention to the keys of another stream (an encoder's states), of another length in each sample:
+ * out = softmax(q k^T * scale) v per (sample, head), over the keys j < key_len[b] (device int32 [B], values outside 0..Lk
+ * are clamped; NULL: Lk) with key_mask[b * mask_stride + j] != 0 (device bytes; NULL: all). A row with no key is zeros, and
+ * no key, mask or value outside that set reaches the result, whatever it holds (NaN and infinities too). Head h reads
+ * key head h / (H / Hkv). bf16, head_dim 64 or 128; element (b, h, row, i) of q is at
+ * q + b * q_sample + h * q_head + row * q_row + i, k, v and out likewise (strides in elements, multiples of 8, 0 where a
+ * sample or head is shared; pointers 16-byte aligned): head-major and token-major rows alike. scale <= 0: 1 /
+ * sqrt(head_dim). Lk may be 0 (zeros). */
+mkb_status mkb_cross_attention(const void* q, long q_row, long q_head, long q_sample, const void* k, long k_row,
+                               long k_head, long k_sample, const void* v, long v_row, long v_head, long v_sample, void* out,
+                               long out_row, long out_head, long out_sample, int B, int H, int Hkv, int Lq, int Lk,
+                               int head_dim, const int32_t* key_len, const uint8_t* key_mask, long mask_stride,
+                               float scale, void* stream);
+
 /* ---------------------------------------------------------------------------------------------------------------
  * The denoiser (image::Engine's model interface, src/image/engine.hpp:158-166, on the Qwen-Image-style MMDiT).
  * ------------------------------------------------------------------------------------------------------------- */

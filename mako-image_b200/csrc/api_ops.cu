@@ -3,7 +3,10 @@
 #include "common.cuh"
 #include "launch.cuh"
 #include "attention.cuh"
+#include "cross_attention.cuh"
+#include "gate_norm.cuh"
 #include "gemm.cuh"
+#include "gemm_i8.cuh"
 #include "rowops.cuh"
 #include "sm100.cuh"
 
@@ -60,12 +63,26 @@ uint32_t* device_status_word()
     if (int(g_status_words.size()) <= dev)
         g_status_words.resize(dev + 1, nullptr);
     if (!g_status_words[dev]) {
+        // The first call may come while a stream of this thread is being captured: the allocation is kept out of the
+        // capture, and the clearing goes to a stream of its own, waited for, so no kernel can run before it.
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
         uint32_t* p = nullptr;
-        if (cudaMalloc(&p, sizeof(uint32_t)) != cudaSuccess) {
+        cudaStream_t st = nullptr;
+        bool ok = cudaMalloc(&p, sizeof(uint32_t)) == cudaSuccess;
+        if (ok) {
+            ok = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess &&
+                 cudaMemsetAsync(p, 0, sizeof(uint32_t), st) == cudaSuccess && cudaStreamSynchronize(st) == cudaSuccess;
+            if (st)
+                cudaStreamDestroy(st);
+            if (!ok)
+                cudaFree(p);
+        }
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (!ok) {
             cudaGetLastError();
             return nullptr;
         }
-        cudaMemset(p, 0, sizeof(uint32_t));
         g_status_words[dev] = p;
     }
     return g_status_words[dev];
@@ -399,6 +416,152 @@ mkb_status mkb_attention_kv_arriving(const void* q, int Lq, int Lq_rows, const v
     if (!attn_prepare(op, q, Lq_rows, k, v, Lk_rows, a, &err))
         return fail(MKB_ERR_INVALID, err ? err : "attention: unsupported arguments");
     return cuda_status(attn_launch(op, static_cast<cudaStream_t>(stream)), "attention launch");
+}
+
+mkb_status mkb_quantize_rows(const void* x, long ldx, int x_f32, int8_t* q, long ldq, float* scale, long rows, int n,
+                             void* stream)
+{
+    if (rows < 0 || rows > (1L << 30) || n <= 0 || n > (1 << 24) || ldx < n || ldq < n)
+        return fail(MKB_ERR_INVALID, "quantize_rows: need 0 <= rows <= 2^30, 0 < n <= 2^24, ldx >= n and ldq >= n");
+    if (rows == 0)
+        return MKB_OK;
+    if (!x || !q || !scale)
+        return fail(MKB_ERR_INVALID, "quantize_rows: null argument");
+    if ((reinterpret_cast<uintptr_t>(x) & (x_f32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(scale) & 3))
+        return fail(MKB_ERR_INVALID, "quantize_rows: misaligned x or scale");
+    QuantRowsArgs a{x, ldx, x_f32, q, ldq, scale, rows, n};
+    return cuda_status(quantize_rows(a, static_cast<cudaStream_t>(stream)), "quantize_rows launch");
+}
+
+mkb_status mkb_proj_i8(const int8_t* x, long ldx, const float* x_scale, const int8_t* w, long ldw, const float* w_scale,
+                       const float* bias, void* y, long ldy, int M, int N, int K, int act, int out_f32, void* stream)
+{
+    if (act < MKB_ACT_NONE || act > MKB_ACT_GELU_ERF)
+        return fail(MKB_ERR_INVALID, "proj_i8: unknown activation");
+    if (M < 0 || N <= 0 || K <= 0 || K > kI8MaxK)
+        return fail(MKB_ERR_INVALID, "proj_i8: need M >= 0, N > 0 and 0 < K <= 131071 (exact 32-bit sums)");
+    if (ldx < K || ldw < K || ldy < N || (ldx & 15) || (ldw & 15))
+        return fail(MKB_ERR_INVALID, "proj_i8: need ldx, ldw >= K and multiples of 16, ldy >= N");
+    if (M == 0)
+        return MKB_OK;
+    if (!x || !x_scale || !w || !w_scale || !y)
+        return fail(MKB_ERR_INVALID, "proj_i8: null argument");
+    if ((reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(w) & 15) ||
+        (reinterpret_cast<uintptr_t>(y) & (out_f32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(x_scale) & 3) ||
+        (reinterpret_cast<uintptr_t>(w_scale) & 3) || (reinterpret_cast<uintptr_t>(bias) & 3))
+        return fail(MKB_ERR_INVALID, "proj_i8: x and w need 16-byte alignment, the others their element's");
+    GemmI8Args a{x, ldx, x_scale, w, ldw, w_scale, bias, y, ldy, M, N, K, act, out_f32, device_status_word()};
+    const char* err = nullptr;
+    const cudaError_t e = gemm_i8(a, &err, static_cast<cudaStream_t>(stream));
+    return err ? fail(MKB_ERR_INVALID, err) : cuda_status(e, "proj_i8 launch");
+}
+
+mkb_status mkb_gate_add_norm(const float* x, long ldx, float* x_out, long ldxo, const void* y, long ldy, int y_f32,
+                             int y_norm, const float* y_weight, const float* gate, long gate_stride, int tanh_gate,
+                             int x_norm, const float* x_weight, const float* scale, const float* shift, long mod_stride,
+                             long rows_per_sample, float eps, void* out, long ldo, int out_type, float* out_scale,
+                             long rows, int n, void* stream)
+{
+    if (rows < 0 || rows > (1L << 30) || n <= 0 || n > kGateNormMaxWidth || rows_per_sample <= 0)
+        return fail(MKB_ERR_INVALID, "gate_add_norm: need 0 <= rows <= 2^30, 0 < n <= 12288, rows_per_sample > 0");
+    if (y_norm < MKB_NORM_NONE || y_norm > MKB_NORM_LAYER || x_norm < MKB_NORM_NONE || x_norm > MKB_NORM_LAYER ||
+        out_type < MKB_OUT_NONE || out_type > MKB_OUT_I8)
+        return fail(MKB_ERR_INVALID, "gate_add_norm: unknown norm or output type");
+    if (!(eps >= 0.0f))
+        return fail(MKB_ERR_INVALID, "gate_add_norm: eps must not be negative");
+    if (!y && (gate || y_weight || y_norm != MKB_NORM_NONE || (x_out && x_out != x)))
+        return fail(MKB_ERR_INVALID, "gate_add_norm: without y there is no gate, weight or norm of it, and x_out is x");
+    if (!y && out_type == MKB_OUT_NONE)
+        return fail(MKB_ERR_INVALID, "gate_add_norm: nothing to do (no y and no output)");
+    if (out_type == MKB_OUT_NONE && (x_weight || scale || shift || x_norm != MKB_NORM_NONE))
+        return fail(MKB_ERR_INVALID, "gate_add_norm: a norm, weight or modulation without an output");
+    if (ldx < n || (y && (ldy < n || ldxo < n)) || (out_type != MKB_OUT_NONE && ldo < n) || gate_stride < 0 ||
+        mod_stride < 0)
+        return fail(MKB_ERR_INVALID, "gate_add_norm: leading dimensions below n, or a negative stride");
+    if (y && x_out == x && ldxo != ldx)
+        return fail(MKB_ERR_INVALID, "gate_add_norm: in place, ldxo must be ldx");
+    if (rows == 0)
+        return MKB_OK;
+    if (!x || (y && !x_out) || (out_type != MKB_OUT_NONE && !out) || (out_type == MKB_OUT_I8) != (out_scale != nullptr))
+        return fail(MKB_ERR_INVALID, "gate_add_norm: null argument (out_scale goes with 8-bit outputs alone)");
+    const uintptr_t words = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(x_out) |
+                            reinterpret_cast<uintptr_t>(y_weight) | reinterpret_cast<uintptr_t>(gate) |
+                            reinterpret_cast<uintptr_t>(x_weight) | reinterpret_cast<uintptr_t>(scale) |
+                            reinterpret_cast<uintptr_t>(shift) | reinterpret_cast<uintptr_t>(out_scale);
+    if ((words & 3) || (reinterpret_cast<uintptr_t>(y) & (y_f32 ? 3 : 1)) ||
+        (reinterpret_cast<uintptr_t>(out) & (out_type == MKB_OUT_F32 ? 3 : out_type == MKB_OUT_BF16 ? 1 : 0)))
+        return fail(MKB_ERR_INVALID, "gate_add_norm: misaligned pointer");
+    GateNormArgs a{x,        ldx,      x_out, ldxo,  y,     ldy,        y_f32,           y_norm, x_norm,
+                   tanh_gate, y_weight, gate,  gate_stride, x_weight, scale, shift,       mod_stride, rows_per_sample,
+                   eps,      out,      ldo,   out_type, out_scale, rows, n};
+    return cuda_status(gate_norm(a, static_cast<cudaStream_t>(stream)), "gate_add_norm launch");
+}
+
+mkb_status mkb_cross_attention(const void* q, long q_row, long q_head, long q_sample, const void* k, long k_row,
+                               long k_head, long k_sample, const void* v, long v_row, long v_head, long v_sample, void* out,
+                               long out_row, long out_head, long out_sample, int B, int H, int Hkv, int Lq, int Lk,
+                               int head_dim, const int32_t* key_len, const uint8_t* key_mask, long mask_stride,
+                               float scale, void* stream)
+{
+    if (B < 0 || H <= 0 || Hkv <= 0 || H % Hkv || Lq < 0 || Lk < 0)
+        return fail(MKB_ERR_INVALID, "cross_attention: need B, Lq, Lk >= 0 and H a multiple of Hkv > 0");
+    if (head_dim != 64 && head_dim != 128)
+        return fail(MKB_ERR_INVALID, "cross_attention: head dim must be 64 or 128");
+    if (Lq > (1 << 30) || Lk > (1 << 30) || double(B) * H * ((Lq + 127) / 128) > double(1 << 30))
+        return fail(MKB_ERR_INVALID, "cross_attention: too many rows");
+    if (!(scale == scale) || scale > 3.0e38f)
+        return fail(MKB_ERR_INVALID, "cross_attention: the scale must be finite");
+    if (B == 0 || Lq == 0)
+        return MKB_OK;
+    if (!q || !out || (Lk > 0 && (!k || !v)))
+        return fail(MKB_ERR_INVALID, "cross_attention: null q, k, v or out");
+    // A dimension of one element may come with any stride.
+    HeadStrides s[4] = {{q_row, q_head, q_sample}, {k_row, k_head, k_sample}, {v_row, v_head, v_sample},
+                        {out_row, out_head, out_sample}};
+    for (int i = 0; i < 4; ++i) {
+        const int rows = i == 0 || i == 3 ? Lq : Lk, heads = i == 0 || i == 3 ? H : Hkv;
+        if (rows <= 1)
+            s[i].row = head_dim;
+        if (heads == 1)
+            s[i].head = 0;
+        if (B == 1)
+            s[i].sample = 0;
+        if (s[i].row < head_dim || s[i].head < 0 || s[i].sample < 0 ||
+            ((s[i].row | s[i].head | s[i].sample) & 7) || s[i].row >= (1L << 38) || s[i].head >= (1L << 38) ||
+            s[i].sample >= (1L << 38))
+            return fail(MKB_ERR_INVALID, "cross_attention: strides must be multiples of 8 elements and rows head_dim apart");
+    }
+    if ((H > 1 && s[3].head == 0) || (B > 1 && s[3].sample == 0))
+        return fail(MKB_ERR_INVALID, "cross_attention: the output's heads and samples need their own rows");
+    if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(k) & 15) ||
+        (reinterpret_cast<uintptr_t>(v) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) ||
+        (reinterpret_cast<uintptr_t>(key_len) & 3))
+        return fail(MKB_ERR_INVALID, "cross_attention: q, k, v and out need 16-byte alignment");
+    if (key_mask && (mask_stride < 0 || (B > 1 && mask_stride != 0 && mask_stride < Lk)))
+        return fail(MKB_ERR_INVALID, "cross_attention: mask rows must be Lk apart, or one row for all (stride 0)");
+    CrossArgs a;
+    a.q = static_cast<const __nv_bfloat16*>(q);
+    a.k = static_cast<const __nv_bfloat16*>(k);
+    a.v = static_cast<const __nv_bfloat16*>(v);
+    a.out = static_cast<__nv_bfloat16*>(out);
+    a.sq = s[0];
+    a.sk = s[1];
+    a.sv = s[2];
+    a.so = s[3];
+    a.B = B;
+    a.H = H;
+    a.Hkv = Hkv;
+    a.Lq = Lq;
+    a.Lk = Lk;
+    a.d = head_dim;
+    a.key_len = key_len;
+    a.key_mask = key_mask;
+    a.mask_stride = mask_stride;
+    a.scale_log2 = 1.4426950408889634f * (scale > 0.0f ? scale : 1.0f / sqrtf(float(head_dim)));
+    a.status = device_status_word();
+    const char* err = nullptr;
+    const cudaError_t e = cross_attention(a, &err, static_cast<cudaStream_t>(stream));
+    return err ? fail(MKB_ERR_INVALID, err) : cuda_status(e, "cross_attention launch");
 }
 
 mkb_status mkb_selftest_stalled_gemm(const void* x, long ldx, const void* w, long ldw, float* y, long ldy, int M,

@@ -32,6 +32,12 @@ _SIGS = {
     "mkb_proj_geglu": (_i, [_vp, _l, _vp, _l, _vp, _vp, _l, _i, _i, _i, _vp]),
     "mkb_conv2d": (_i, [_vp, _i, _i, _i, _i, _vp, _i, _i, _i, _vp, _vp, _l, _vp, _l, _vp, _l, _i, _vp]),
     "mkb_ln_modulate": (_i, [_vp, _vp, _vp, _vp, _l, _i, _f, _l, _l, _l, _vp]),
+    "mkb_quantize_rows": (_i, [_vp, _l, _i, _vp, _l, _vp, _l, _i, _vp]),
+    "mkb_proj_i8": (_i, [_vp, _l, _vp, _vp, _l, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _vp]),
+    "mkb_gate_add_norm": (_i, [_vp, _l, _vp, _l, _vp, _l, _i, _i, _vp, _vp, _l, _i, _i, _vp, _vp, _vp, _l, _l, _f, _vp,
+                               _l, _i, _vp, _l, _i, _vp]),
+    "mkb_cross_attention": (_i, [_vp, _l, _l, _l, _vp, _l, _l, _l, _vp, _l, _l, _l, _vp, _l, _l, _l, _i, _i, _i, _i, _i,
+                                 _i, _vp, _vp, _l, _f, _vp]),
     "mkb_group_norm_workspace_size": (ctypes.c_size_t, [_i, _i, _i, _i]),
     "mkb_group_norm": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _i, _vp, ctypes.c_size_t, _vp]),
     "mkb_group_norm_static_max_bytes": (ctypes.c_size_t, []),

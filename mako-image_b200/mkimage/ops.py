@@ -2,7 +2,7 @@
 
 import ctypes
 
-from ._lib import lib, check, stream_ptr
+from ._lib import lib, check, stream_ptr, MkbError
 
 ACT_NONE, ACT_GELU_TANH, ACT_SILU, ACT_QUICK_GELU, ACT_GELU_ERF = 0, 1, 2, 3, 4
 
@@ -205,4 +205,174 @@ def group_norm(x, gamma, beta, groups=32, eps=1e-5, silu=False, out=None):
         out = torch.empty(x.shape, device=x.device, dtype=torch.bfloat16)
     check(lib.mkb_group_norm(_p(x), _p(out), _p(gamma), _p(beta), B, HW, C, groups, eps, int(silu), _p(ws),
                              ws.numel() * 4, stream_ptr()))
+    return out
+
+
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+OUT_NONE, OUT_BF16, OUT_F32, OUT_I8 = 0, 1, 2, 3
+
+
+def _need(ok, what):
+    if not ok:
+        raise MkbError(1, what)
+
+
+def _on(name, device, **tensors):
+    """Every given tensor lives on the CUDA device `device`."""
+    for k, t in tensors.items():
+        _need(t is None or t.device == device, f"{name}: {k} is on {getattr(t, 'device', None)}, not on {device}")
+    _need(device.type == "cuda", f"{name}: tensors must be CUDA tensors")
+
+
+def _launch(fn, device, *args):
+    """fn(*args, stream) on the tensors' device and its current stream, whatever device is current."""
+    import torch
+
+    if torch.cuda.current_device() == device.index:
+        return check(fn(*args, stream_ptr()))
+    with torch.cuda.device(device):
+        return check(fn(*args, stream_ptr()))
+
+
+def _row_stride(t):
+    """Elements between rows of a 2-D tensor (a single row may come with any stride)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _rows_i8(rows, n, device):
+    import torch
+
+    return torch.empty(rows, -(-n // 16) * 16, device=device, dtype=torch.int8)[:, :n]
+
+
+def quantize_rows(x, q=None, scale=None):
+    """(q, scale): rows of x [rows][n] (bf16 or fp32) as int8 with an fp32 step max|row| / 127 each, so that q * scale
+    is x to half a step (see mkb_quantize_rows). q's rows are 16 bytes aligned, as proj_i8 wants them."""
+    import torch
+
+    _need(x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float32), "quantize_rows: x must be 2-D bf16 or fp32")
+    rows, n = x.shape
+    if q is None:
+        q = _rows_i8(rows, n, x.device)
+    if scale is None:
+        scale = torch.empty(rows, device=x.device, dtype=torch.float32)
+    _on("quantize_rows", x.device, x=x, q=q, scale=scale)
+    _need(n > 0 and x.stride(1) == 1 or n == 1, "quantize_rows: the values of a row must be contiguous")
+    _need(q.shape == x.shape and q.dtype == torch.int8 and (q.stride(1) == 1 or n == 1),
+          "quantize_rows: q must be int8 rows of x's shape")
+    _need(scale.shape == (rows,) and scale.dtype == torch.float32 and scale.is_contiguous(),
+          "quantize_rows: scale must be contiguous fp32 [rows]")
+    _launch(lib.mkb_quantize_rows, x.device, _p(x), _row_stride(x), int(x.dtype == torch.float32), _p(q),
+            _row_stride(q), _p(scale), rows, n)
+    return q, scale
+
+
+def proj_i8(x, x_scale, w, w_scale, bias=None, act=ACT_NONE, out=None, out_f32=False):
+    """y = act(x_scale[:, None] * w_scale * (x @ w.T) + bias): x [M][K] and w [N][K] int8 with rows 16 bytes aligned
+    (quantize_rows makes such rows), scales fp32, exact integer sums (see mkb_proj_i8)."""
+    import torch
+
+    _need(x.dim() == 2 and w.dim() == 2 and x.dtype == torch.int8 and w.dtype == torch.int8 and
+          x.shape[1] == w.shape[1], "proj_i8: x [M][K] and w [N][K] must be int8")
+    M, K = x.shape
+    N = w.shape[0]
+    if out is None:
+        out = torch.empty(M, N, device=x.device, dtype=torch.float32 if out_f32 else torch.bfloat16)
+    _on("proj_i8", x.device, x=x, x_scale=x_scale, w=w, w_scale=w_scale, bias=bias, out=out)
+    for t in (x, w, out):
+        _need(t.stride(1) == 1 or t.shape[1] == 1, "proj_i8: the values of a row must be contiguous")
+    _need(out.shape == (M, N) and out.dtype in (torch.float32, torch.bfloat16), "proj_i8: out must be [M][N] fp32 or bf16")
+    for t, n in ((x_scale, M), (w_scale, N), (bias, N)):
+        _need(t is None or (t.shape == (n,) and t.dtype == torch.float32 and t.is_contiguous()),
+              "proj_i8: scales and bias must be contiguous fp32 vectors, one value a row of x or w")
+    ldx, ldw = (t.stride(0) if t.shape[0] > 1 else -(-max(t.stride(0), K) // 16) * 16 for t in (x, w))
+    _launch(lib.mkb_proj_i8, x.device, _p(x), ldx, _p(x_scale), _p(w), ldw, _p(w_scale), _p(bias), _p(out),
+            _row_stride(out), M, N, K, act, int(out.dtype == torch.float32))
+    return out
+
+
+def gate_add_norm(x, y=None, y_norm=NORM_NONE, y_weight=None, gate=None, tanh_gate=False, x_norm=NORM_RMS, x_weight=None,
+                  scale=None, shift=None, rows_per_sample=None, eps=1e-6, x_out=None, out=None, out_scale=None,
+                  out_type=OUT_BF16):
+    """The end of a block's branch and the start of the next in one pass (see mkb_gate_add_norm):
+
+        x  += g(gate) * norm_y(y) * y_weight            (into x_out when it is given)
+        out = norm_x(x) * x_weight * (1 + scale) + shift
+
+    x [rows][n] fp32, y bf16 or fp32; gate, scale, shift [samples][n] (or [n]) of the sample row // rows_per_sample.
+    Returns out as out_type says: bf16, fp32, (int8 rows, steps) or None."""
+    import torch
+
+    f32 = torch.float32
+    _need(x.dim() == 2 and x.dtype == f32, "gate_add_norm: x must be 2-D fp32")
+    rows, n = x.shape
+    rps = rows_per_sample or max(rows, 1)
+    samples = -(-rows // rps)
+    if x_out is None:
+        x_out = x
+    if out_type == OUT_I8:
+        if out is None:
+            out = _rows_i8(rows, n, x.device)
+        if out_scale is None:
+            out_scale = torch.empty(rows, device=x.device, dtype=f32)
+    elif out_type != OUT_NONE and out is None:
+        out = torch.empty(rows, n, device=x.device, dtype=f32 if out_type == OUT_F32 else torch.bfloat16)
+    _on("gate_add_norm", x.device, x=x, y=y, y_weight=y_weight, gate=gate, x_weight=x_weight, scale=scale, shift=shift,
+        x_out=x_out, out=out, out_scale=out_scale)
+    want = {OUT_BF16: torch.bfloat16, OUT_F32: f32, OUT_I8: torch.int8}.get(out_type)
+    _need(x_out.dtype == f32 and (y is None or y.dtype in (f32, torch.bfloat16)) and
+          (out is None) == (want is None) and (out is None or out.dtype == want), "gate_add_norm: wrong type")
+    for t in (x, x_out, y, out):
+        _need(t is None or (t.shape == x.shape and (n == 1 or t.stride(1) == 1)),
+              "gate_add_norm: x, x_out, y and out must be [rows][n] with contiguous rows")
+    for t in (y_weight, x_weight):
+        _need(t is None or (t.shape == (n,) and t.dtype == f32 and t.is_contiguous()),
+              "gate_add_norm: weights must be contiguous fp32 [n]")
+    for t in (gate, scale, shift):
+        _need(t is None or (t.dtype == f32 and t.shape[-1] == n and t.stride(-1) == 1 and
+                            (t.dim() == 1 or (t.dim() == 2 and t.shape[0] in (1, samples) or rows == 0))),
+              "gate_add_norm: gate, scale and shift must be fp32 [n] or [samples][n]")
+    _need(out_scale is None or (out_type == OUT_I8 and out_scale.shape == (rows,) and out_scale.dtype == f32 and
+                                out_scale.is_contiguous()), "gate_add_norm: out_scale must be contiguous fp32 [rows]")
+
+    def per_sample(t):
+        return t.stride(0) if t is not None and t.dim() == 2 and t.shape[0] > 1 else 0
+
+    _need(scale is None or shift is None or samples <= 1 or per_sample(scale) == per_sample(shift),
+          "gate_add_norm: scale and shift must have the same strides")
+    _launch(lib.mkb_gate_add_norm, x.device, _p(x), _row_stride(x), _p(x_out), _row_stride(x_out), _p(y),
+            _row_stride(y) if y is not None else 0, int(y is not None and y.dtype == f32), y_norm, _p(y_weight),
+            _p(gate), per_sample(gate), int(tanh_gate), x_norm if out_type != OUT_NONE else NORM_NONE, _p(x_weight),
+            _p(scale), _p(shift), per_sample(scale if scale is not None else shift), rps, eps, _p(out),
+            _row_stride(out) if out is not None else 0, out_type, _p(out_scale), rows, n)
+    return (out, out_scale) if out_type == OUT_I8 else out
+
+
+def cross_attention(q, k, v, key_len=None, key_mask=None, scale=None, out=None):
+    """Attention of q [B][H][Lq][d] to another stream's k, v [B][Hkv][Lk][d] (bf16, d 64 or 128, any strides with
+    contiguous heads: permuted token-major projections as well as head-major ones), over each sample's first key_len[b]
+    keys that key_mask [B][Lk] (bool) leaves (see mkb_cross_attention). Returns out [B][Lq][H * d] (given: any
+    [B][Lq][H][d] or [B][Lq][H * d] bf16)."""
+    import torch
+
+    _need(q.dim() == 4 and k.dim() == 4 and v.shape == k.shape and q.shape[0] == k.shape[0] and q.shape[3] == k.shape[3],
+          "cross_attention: q must be [B][H][Lq][d], k and v [B][Hkv][Lk][d]")
+    B, H, Lq, d = q.shape
+    Hkv, Lk = k.shape[1], k.shape[2]
+    if out is None:
+        out = torch.empty(B, Lq, H * d, device=q.device, dtype=torch.bfloat16)
+    _need(tuple(out.shape) in ((B, Lq, H * d), (B, Lq, H, d)), "cross_attention: out must be [B][Lq][H * d]")
+    heads = (out.stride(0), out.stride(2) if out.dim() == 4 else d, out.stride(1))
+    _on("cross_attention", q.device, q=q, k=k, v=v, out=out, key_len=key_len, key_mask=key_mask)
+    for t in (q, k, v, out):
+        _need(t.dtype == torch.bfloat16 and t.stride(-1) == 1, "cross_attention: tensors must be bf16 with contiguous heads")
+    _need(key_len is None or (key_len.shape == (B,) and key_len.dtype == torch.int32 and key_len.is_contiguous()),
+          "cross_attention: key_len must be contiguous int32 [B]")
+    _need(key_mask is None or (key_mask.shape == (B, Lk) and key_mask.dtype in (torch.bool, torch.uint8) and
+                               (key_mask.stride(1) == 1 or Lk <= 1)), "cross_attention: key_mask must be bool [B][Lk]")
+    _need(scale is None or scale > 0, "cross_attention: the scale must be positive")
+    _launch(lib.mkb_cross_attention, q.device, _p(q), q.stride(2), q.stride(1), q.stride(0), _p(k), k.stride(2),
+            k.stride(1), k.stride(0), _p(v), v.stride(2), v.stride(1), v.stride(0), _p(out), heads[2], heads[1],
+            heads[0], B, H, Hkv, Lq, Lk, d, _p(key_len), _p(key_mask),
+            key_mask.stride(0) if key_mask is not None else 0, scale or 0.0)
     return out
