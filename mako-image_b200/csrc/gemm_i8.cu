@@ -1,81 +1,731 @@
-// The 8-bit integer projection (see gemm_i8.cuh).
+// The 8-bit integer projection (see gemm_i8.cuh): three kernels for three ranges of rows.
+//   k_i8_rows   up to 8 rows: the weights stream through the CUDA cores once (dp4a); HBM is the bound.
+//   k_i8_split  few output tiles: 128 x BN tiles on one SM each, the K axis cut over a cluster whose CTAs add their
+//               integer sums through distributed shared memory; latency is the bound.
+//   k_i8_pair   the rest: persistent 256 x BN tiles on CTA pairs (cta_group::2), the tensor pipe is the bound.
+// The sums are exact integers, so a row's result is the same bits whichever kernel and split computes it.
 #include "gemm_i8.cuh"
 #include "common.cuh"
 #include "gemm.cuh"
 #include "launch.cuh"
+#include "sm100.cuh"
 
+#include <cuda.h>
 #include <cuda_bf16.h>
+#include <cudaTypedefs.h>
+#include <algorithm>
+#include <mutex>
 
 namespace mkb {
 
 namespace {
 
-__device__ __forceinline__ float act_of(float v, int act)
+constexpr int kBK = 128;  // bytes of K a stage: one 128-byte swizzle row
+
+// ------------------------------------------------------------------------------------------------ epilogue arithmetic
+
+// Activations. TANH_SFU: the GELU's tanh from the SFU (absolute error 2^-10.9, below the rounding of bf16 outputs);
+// otherwise (1 + tanh(u)) / 2 = 1 / (1 + e^-2u) to a few fp32 roundings.
+template <bool TANH_SFU>
+__device__ __forceinline__ float act1(float v, int act)
 {
-    switch (act) {
-    case kActGeluTanh:
-        return 0.5f * v * (1.0f + tanhf(0.7978845608028654f * (v + 0.044715f * v * v * v)));
-    case kActSilu:
-        return v / (1.0f + __expf(-v));
-    case kActQuickGelu:
-        return v / (1.0f + __expf(-1.702f * v));
-    case kActGeluErf:
-        return 0.5f * v * (1.0f + erff(v * 0.7071067811865476f));
+    if (act == kActGeluTanh) {
+        const float u = 0.7978845608028654f * fmaf(0.044715f * v, v * v, v);
+        if constexpr (TANH_SFU) {
+            float t;
+            asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(u));
+            return 0.5f * v * (1.0f + t);
+        }
+        return v / (1.0f + __expf(-2.0f * u));
     }
+    if (act == kActSilu)
+        return v / (1.0f + __expf(-v));
+    if (act == kActQuickGelu)
+        return v / (1.0f + __expf(-1.702f * v));
+    if (act == kActGeluErf)
+        return 0.5f * v * (1.0f + erff(v * 0.7071067811865476f));
     return v;
 }
 
-// 64 x 64 outputs a block, 4 x 4 a thread, 64 bytes of K at a time in shared memory.
-__global__ void __launch_bounds__(256) k_gemm_i8_simple(const GemmI8Args a)
+// The switch outside the loop, so that the columns' chains interleave.
+template <bool TANH_SFU, int N>
+__device__ __forceinline__ void act_all(float (&v)[N], int act)
 {
-    __shared__ int sx[64][17], sw[64][17];
+    switch (act) {
+    case kActGeluTanh:
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            v[j] = act1<TANH_SFU>(v[j], kActGeluTanh);
+        break;
+    case kActSilu:
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            v[j] = act1<TANH_SFU>(v[j], kActSilu);
+        break;
+    case kActQuickGelu:
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            v[j] = act1<TANH_SFU>(v[j], kActQuickGelu);
+        break;
+    case kActGeluErf:
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            v[j] = act1<TANH_SFU>(v[j], kActGeluErf);
+        break;
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void act_out(float (&v)[N], int act, bool f32)
+{
+    if (act == kActNone)
+        return;
+    if (f32)
+        act_all<false>(v, act);
+    else
+        act_all<true>(v, act);
+}
+
+// N consecutive columns of a row, as far as they exist, in the widest stores the address allows.
+template <int N>
+__device__ __forceinline__ void store_row(const GemmI8Args& a, long row, int col, const float (&v)[N])
+{
+    const int n = min(N, a.N - col);
+    if (a.out_f32) {
+        float* p = static_cast<float*>(a.y) + row * a.ldy + col;
+        if (n == N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < N; j += 4)
+                *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < n)
+                    p[j] = v[j];
+        }
+    } else {
+        __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.y) + row * a.ldy + col;
+        if (n == N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < N; j += 8)
+                *reinterpret_cast<uint4*>(p + j) =
+                    make_uint4(pack_bf16x2(v[j], v[j + 1]), pack_bf16x2(v[j + 2], v[j + 3]),
+                               pack_bf16x2(v[j + 4], v[j + 5]), pack_bf16x2(v[j + 6], v[j + 7]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (j < n)
+                    p[j] = __float2bfloat16(v[j]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+
+constexpr int kRowsMax = 8;
+
+// MR rows of x against R rows of W a warp (WK = 1), or against R rows of W a block whose 8 warps share the K axis (WK =
+// 8, for matrices with too few rows of W to fill the GPU otherwise). Lanes take 16 bytes of K each.
+template <int MR, int R, int WK>
+__global__ void __launch_bounds__(256) k_i8_rows(const GemmI8Args a)
+{
+    __shared__ int part[WK > 1 ? 8 * MR * R : 1];
     grid_dep_wait();
     grid_dep_launch();
-    const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < a.K; k0 += 64) {
-        for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-            const int r = i / 16, c = i % 16;
-            uint32_t xv = 0, wv = 0;
-            for (int b = 0; b < 4; ++b) {
-                const int k = k0 + 4 * c + b;
-                if (k < a.K) {
-                    if (m0 + r < a.M)
-                        xv |= uint32_t(uint8_t(a.x[(m0 + r) * a.ldx + k])) << (8 * b);
-                    if (n0 + r < a.N)
-                        wv |= uint32_t(uint8_t(a.w[(n0 + r) * a.ldw + k])) << (8 * b);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n0 = WK == 1 ? (blockIdx.x * 8 + warp) * R : blockIdx.x * R;
+    int acc[MR][R] = {};
+    if (WK > 1 || n0 < a.N) {
+        const int8_t* w[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            w[r] = a.w + long(min(n0 + r, a.N - 1)) * a.ldw;
+        const int whole = a.K >> 4;
+#pragma unroll 2
+        for (int c = (WK == 1 ? 0 : warp * 32) + lane; c < whole; c += 32 * WK) {
+            int4 wv[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                wv[r] = __ldg(reinterpret_cast<const int4*>(w[r]) + c);
+#pragma unroll
+            for (int m = 0; m < MR; ++m) {
+                if (m < a.M) {
+                    const int4 xv = __ldg(reinterpret_cast<const int4*>(a.x + m * a.ldx) + c);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        int s = __dp4a(xv.x, wv[r].x, acc[m][r]);
+                        s = __dp4a(xv.y, wv[r].y, s);
+                        s = __dp4a(xv.z, wv[r].z, s);
+                        acc[m][r] = __dp4a(xv.w, wv[r].w, s);
+                    }
                 }
             }
-            sx[r][c] = int(xv);
-            sw[r][c] = int(wv);
         }
-        __syncthreads();
-        for (int c = 0; c < 16; ++c)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j)
-                    acc[i][j] = __dp4a(sx[ty * 4 + i][c], sw[tx + 16 * j][c], acc[i][j]);
-        __syncthreads();
+        // The last K % 16 values one by one: a row's memory may end with them.
+        const int k = (whole << 4) + lane;
+        if (k < a.K && (WK == 1 || warp == 0))
+#pragma unroll
+            for (int m = 0; m < MR; ++m)
+                if (m < a.M)
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+                        acc[m][r] += int(a.x[m * a.ldx + k]) * int(w[r][k]);
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const long m = m0 + ty * 4 + i;
-            const int n = n0 + tx + 16 * j;
-            if (m >= a.M || n >= a.N)
-                continue;
-            const float v = act_of(float(acc[i][j]) * a.x_scale[m] * a.w_scale[n] + (a.bias ? a.bias[n] : 0.0f), a.act);
-            if (a.out_f32)
-                static_cast<float*>(a.y)[m * a.ldy + n] = v;
-            else
-                static_cast<__nv_bfloat16*>(a.y)[m * a.ldy + n] = __float2bfloat16(v);
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            acc[m][r] = __reduce_add_sync(0xffffffffu, acc[m][r]);
+    if constexpr (WK > 1) {
+        if (lane == 0)
+#pragma unroll
+            for (int m = 0; m < MR; ++m)
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    part[(warp * MR + m) * R + r] = acc[m][r];
+        __syncthreads();
+        if (warp)
+            return;
+    }
+    // Lane m * R + r finishes output (m, r).
+    const int m = lane / R, r = lane % R, n = n0 + r;
+    int s = 0;
+    if constexpr (WK > 1) {
+        if (m < MR)
+            for (int i = 0; i < 8; ++i)
+                s += part[(i * MR + m) * R + r];
+    } else {
+#pragma unroll
+        for (int i = 0; i < MR; ++i)
+#pragma unroll
+            for (int j = 0; j < R; ++j)
+                if (m == i && r == j)
+                    s = acc[i][j];
+    }
+    if (m >= a.M || m >= MR || n >= a.N)
+        return;
+    float v[1] = {fmaf(float(s) * a.x_scale[m], a.w_scale[n], a.bias ? a.bias[n] : 0.0f)};
+    act_out(v, a.act, a.out_f32);
+    if (a.out_f32)
+        static_cast<float*>(a.y)[m * a.ldy + n] = v[0];
+    else
+        static_cast<__nv_bfloat16*>(a.y)[m * a.ldy + n] = __float2bfloat16(v[0]);
+}
+
+// ------------------------------------------------------------------------------------------------ tensor-core kernels
+
+struct I8Params {
+    CUtensorMap tx, tw, ty;
+    GemmI8Args a;
+    int splits;   // k_i8_split: CTAs of a cluster, each a part of K
+    int boxes;    // k_i8_pair: outputs leave as TMA boxes
+};
+
+template <int BN>
+struct SplitCfg {
+    static constexpr int kABytes = 128 * kBK, kBBytes = BN * kBK, kStageBytes = kABytes + kBBytes;
+    static constexpr int kStages = BN == 64 ? 8 : 6;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + 256;
+    static_assert(kSmem <= 227 * 1024);
+    static_assert(kStages * kStageBytes >= 128 * BN * 4, "the partial sums reuse the stages");
+};
+
+// Columns [c0, c0 + 8) of this warp's rows.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v)
+{
+    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// One 128 x BN tile a cluster (blockIdx.x = tile * splits + part), K cut into `splits` runs of whole stages. After the
+// main loop CTA p holds the sums of its run; it hands columns [o * BN / splits, ...) to CTA o's shared memory for every
+// other o, and finishes its own columns with what the others brought.
+template <int BN>
+__global__ void __launch_bounds__(192, 1) k_i8_split(const __grid_constant__ I8Params P)
+{
+    using C = SplitCfg<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStageBytes);
+    uint64_t* empty = full + C::kStages;
+    uint64_t* acc_full = empty + C::kStages;
+    uint64_t* drain = acc_full + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const GemmI8Args& a = P.a;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int S = P.splits, part = S > 1 ? int(cluster_ctarank()) : 0, tile = blockIdx.x / S;
+    const int num_n = (a.N + BN - 1) / BN, mb = tile / num_n, nb = tile % num_n;
+    const int num_k = (a.K + kBK - 1) / kBK, k_lo = int(long(num_k) * part / S), k_hi = int(long(num_k) * (part + 1) / S);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
         }
+        mbar_init(acc_full, 1);
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&P.tx);
+        prefetch_tmap(&P.tw);
+    }
+    grid_dep_wait();  // before TMEM allocation and the first global access
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, BN);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    grid_dep_launch();
+    const uint32_t tmem = *tmem_slot;
+    bool ok = true;
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
+                const int s = it % C::kStages;
+                if (!mbar_wait(&empty[s], ((it / C::kStages) & 1) ^ 1, a.status, kErrWaitEmpty, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                uint8_t* sa = smem + s * C::kStageBytes;
+                mbar_arrive_expect_tx(&full[s], C::kStageBytes);
+                tma_load_2d(sa, &P.tx, &full[s], kb * kBK, mb * 128);
+                tma_load_2d(sa + C::kABytes, &P.tw, &full[s], kb * kBK, nb * BN);
+            }
+            if (!ok)  // let the loads already issued land before the CTA can exit
+                for (int j = std::max(0, it - C::kStages); j < it; ++j)
+                    mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1, a.status, kErrWaitDrain, nullptr);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_i8_s32(128, BN);
+            int it = 0;
+            for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
+                const int s = it % C::kStages;
+                if (!mbar_wait(&full[s], (it / C::kStages) & 1, a.status, kErrWaitFull, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t aa = smem_u32(smem + s * C::kStageBytes), bb = aa + C::kABytes;
+#pragma unroll
+                for (int k = 0; k < kBK / 32; ++k)
+                    mma_i8_ss(tmem, desc_kmajor_sw128(aa + k * 32), desc_kmajor_sw128(bb + k * 32), idesc,
+                              (it | k) != 0);
+                mma_commit(&empty[s]);
+            }
+            if (ok)
+                mma_commit(acc_full);
+            mma_commit(drain);
+            mbar_wait(drain, 0, a.status, kErrWaitDrain, nullptr);
+        }
+    } else {
+        ok = mbar_wait(acc_full, 0, a.status, kErrWaitAccFull, abort_flag);
+        tc_fence_after();
+    }
+    __syncwarp();
+    const int q = warp & 3, r = q * 32 + lane;
+    const uint32_t t_row = tmem + (uint32_t(q * 32) << 16);
+    const int cols = BN / S;  // of this CTA, a multiple of 8
+    int* sums = reinterpret_cast<int*>(smem);  // [splits - 1][cols][128]
+    if (S > 1) {
+        __syncthreads();  // the producer and the MMA warp are past their last use of the stages
+        cluster_sync_all();
+        if (warp >= 2 && ok)
+            for (int o = 0; o < S; ++o) {
+                if (o == part)
+                    continue;
+                const uint32_t slot = uint32_t(part < o ? part : part - 1);
+                const uint32_t dst = map_to_cta(smem_u32(sums) + (slot * cols * 128 + r) * 4, o);
+                for (int c = 0; c < cols; c += 8) {
+                    uint32_t v[8];
+                    tmem_ld8(t_row + o * cols + c, v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        st_cluster(dst + (c + j) * 512, v[j]);
+                }
+            }
+        cluster_sync_all();
+    }
+    if (warp >= 2 && ok) {
+        const long row = long(mb) * 128 + r;
+        const float sx = row < a.M ? __ldg(a.x_scale + row) : 0.0f;
+        for (int c = 0; c < cols; c += 8) {
+            const int col = nb * BN + part * cols + c;
+            if (col >= a.N)
+                break;
+            uint32_t t[8];
+            tmem_ld8(t_row + part * cols + c, t);
+            tmem_wait_ld();
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                int s = int(t[j]);
+                for (int o = 0; o < S - 1; ++o)
+                    s += sums[(o * cols + c + j) * 128 + r];
+                const bool in = col + j < a.N;
+                v[j] = fmaf(float(s) * sx, in ? __ldg(a.w_scale + col + j) : 0.0f,
+                            in && a.bias ? __ldg(a.bias + col + j) : 0.0f);
+            }
+            act_out(v, a.act, a.out_f32);
+            if (row < a.M)
+                store_row(a, row, col, v);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, BN);
+    }
+}
+
+template <int BN>
+struct PairCfg {
+    static constexpr int kABytes = 128 * kBK, kBBytes = BN / 2 * kBK, kStageBytes = kABytes + kBBytes;
+    static constexpr int kBox = 32 * 128;  // a warp's box: 32 rows of 128 bytes
+    static constexpr int kStages = BN == 256 ? 5 : 7;
+    static constexpr int kVec = 2 * 2 * BN * 4;  // w_scale and bias of two tiles
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + 8 * kBox + kVec + 256;
+    static constexpr int kTmemCols = 2 * BN;
+    static_assert(kSmem <= 227 * 1024);
+};
+
+// Tiles in groups of 8 along M, so that concurrent tiles share panels of x and W in L2.
+__device__ __forceinline__ void tile_of(int tile, int num_m, int num_n, int& mb, int& nb)
+{
+    const int per_group = 8 * num_n, group = tile / per_group, first = group * 8;
+    const int gsize = min(num_m - first, 8), t = tile - group * per_group;
+    mb = first + t % gsize;
+    nb = t / gsize;
+}
+
+// Persistent CTA pairs. Warp 0 of each CTA loads its 128 rows of x and its half of the W tile by TMA, the leader's warp 1
+// issues 256 x BN x 32 MMAs into one of two accumulators, warps 2-5 of both CTAs drain the other: a thread a row, 32
+// columns at a time, through a 4 KB box a warp that leaves as a TMA store.
+template <int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(const __grid_constant__ I8Params P)
+{
+    using C = PairCfg<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* boxes = smem + C::kStages * C::kStageBytes;
+    float* vec = reinterpret_cast<float*>(boxes + 8 * C::kBox);  // [2][w_scale, bias][BN]
+    uint64_t* full = reinterpret_cast<uint64_t*>(boxes + 8 * C::kBox + C::kVec);
+    uint64_t* empty = full + C::kStages;
+    uint64_t* acc_full = empty + C::kStages;
+    uint64_t* acc_empty = acc_full + 2;
+    uint64_t* drain = acc_empty + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const GemmI8Args& a = P.a;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int pair = blockIdx.x / 2, npairs = gridDim.x / 2;
+    const int num_m = (a.M + 255) / 256, num_n = (a.N + BN - 1) / BN, num_k = (a.K + kBK - 1) / kBK;
+    const int num_tiles = num_m * num_n;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], 2 * 128);  // the epilogue threads of both CTAs (leader's barrier)
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&P.tx);
+        prefetch_tmap(&P.tw);
+    }
+    grid_dep_wait();  // before TMEM allocation and the first global access
+    if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, C::kTmemCols);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // both CTAs' barriers exist before either signals the other's
+    tc_fence_after();
+    grid_dep_launch();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int tile = pair; tile < num_tiles && ok; tile += npairs) {
+                int mb, nb;
+                tile_of(tile, num_m, num_n, mb, nb);
+                for (int kb = 0; kb < num_k; ++kb, ++it) {
+                    const int s = it % C::kStages;
+                    if (!mbar_wait(&empty[s], ((it / C::kStages) & 1) ^ 1, a.status, kErrWaitEmpty, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* sa = smem + s * C::kStageBytes;
+                    if (leader)
+                        mbar_arrive_expect_tx(&full[s], 2 * C::kStageBytes);  // both CTAs' loads land on it
+                    tma_load_2d_pair(sa, &P.tx, &full[s], kb * kBK, mb * 256 + int(rank) * 128);
+                    tma_load_2d_pair(sa + C::kABytes, &P.tw, &full[s], kb * kBK, nb * BN + int(rank) * (BN / 2));
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && leader) {
+            constexpr uint32_t idesc = idesc_i8_s32(256, BN);
+            uint32_t it = 0, lt = 0;
+            bool ok = true;
+            for (int tile = pair; tile < num_tiles && ok; tile += npairs, ++lt) {
+                const uint32_t acc = lt & 1, acc_ph = (lt >> 1) & 1;
+                if (!mbar_wait(&acc_empty[acc], acc_ph ^ 1, a.status, kErrWaitAccEmpty, abort_flag))
+                    break;
+                tc_fence_after();
+                for (int kb = 0; kb < num_k; ++kb, ++it) {
+                    const int s = it % C::kStages;
+                    if (!mbar_wait(&full[s], (it / C::kStages) & 1, a.status, kErrWaitFull, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t aa = smem_u32(smem + s * C::kStageBytes), bb = aa + C::kABytes;
+#pragma unroll
+                    for (int k = 0; k < kBK / 32; ++k)
+                        mma_i8_ss_pair(tmem + acc * BN, desc_kmajor_sw128(aa + k * 32), desc_kmajor_sw128(bb + k * 32),
+                                       idesc, (kb | k) != 0);
+                    mma_commit_pair(&empty[s]);
+                }
+                if (ok)
+                    mma_commit_pair(&acc_full[acc]);
+            }
+            mma_commit_pair(drain);
+            mbar_wait(drain, 0, a.status, kErrWaitDrain, nullptr);
+        }
+    } else {
+        const int q = warp & 3, et = int(threadIdx.x) - 64;
+        const uint32_t acc_empty0 = map_to_cta(smem_u32(&acc_empty[0]), 0);
+        uint8_t* box = boxes + (warp - 2) * 2 * C::kBox;
+        uint32_t lt = 0, nbox = 0;
+        for (int tile = pair; tile < num_tiles; tile += npairs, ++lt) {
+            int mb, nb;
+            tile_of(tile, num_m, num_n, mb, nb);
+            const uint32_t acc = lt & 1, acc_ph = (lt >> 1) & 1;
+            const int n0 = nb * BN, row0 = mb * 256 + int(rank) * 128 + q * 32, row = row0 + lane;
+            // The tile's column vectors, into the copy that the tile before last read.
+            float* sw = vec + acc * 2 * BN;
+            for (int i = et; i < BN; i += 128) {
+                const bool in = n0 + i < a.N;
+                sw[i] = in ? __ldg(a.w_scale + n0 + i) : 0.0f;
+                sw[BN + i] = in && a.bias ? __ldg(a.bias + n0 + i) : 0.0f;
+            }
+            const float sx = row < a.M ? __ldg(a.x_scale + row) : 0.0f;
+            const bool got = mbar_wait(&acc_full[acc], acc_ph, a.status, kErrWaitAccFull, abort_flag);
+            // Also publishes the vectors; the four warps leave together or not at all.
+            if (named_barrier_or<1, 128>(!got))
+                break;
+            tc_fence_after();
+            const uint32_t t_row = tmem + (uint32_t(q * 32) << 16) + acc * BN;
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 32) {
+                if (n0 + c >= a.N)
+                    break;
+                uint32_t t[32];
+                tmem_ld32(t_row + c, t);
+                tmem_wait_ld();
+                float v[32];
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 s = *reinterpret_cast<const float4*>(sw + c + j);
+                    const float4 b = *reinterpret_cast<const float4*>(sw + BN + c + j);
+                    v[j] = fmaf(float(int(t[j])) * sx, s.x, b.x);
+                    v[j + 1] = fmaf(float(int(t[j + 1])) * sx, s.y, b.y);
+                    v[j + 2] = fmaf(float(int(t[j + 2])) * sx, s.z, b.z);
+                    v[j + 3] = fmaf(float(int(t[j + 3])) * sx, s.w, b.w);
+                }
+                act_out(v, a.act, a.out_f32);
+                if (!P.boxes) {
+                    if (row < a.M)
+                        store_row(a, row, n0 + c, v);
+                    continue;
+                }
+                // A box holds 128 bytes of each row: 32 fp32 columns, or two rounds of 32 bf16 ones.
+                const int half = a.out_f32 ? 0 : (c >> 5) & 1;
+                uint8_t* bx = box + (nbox & 1) * C::kBox + lane * 128;
+                if (half == 0) {
+                    if (lane == 0)
+                        bulk_wait_read<1>();  // the store before last has read this box
+                    __syncwarp();
+                }
+                if (a.out_f32) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        *reinterpret_cast<float4*>(bx + ((j ^ (lane & 7)) << 4)) =
+                            make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *reinterpret_cast<uint4*>(bx + (((4 * half + j) ^ (lane & 7)) << 4)) =
+                            make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                                       pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+                }
+                if (a.out_f32 || half == 1 || n0 + c + 32 >= a.N) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (row0 < a.M)
+                            tma_store_2d(&P.ty, box + (nbox & 1) * C::kBox, a.out_f32 ? n0 + c : n0 + c - 32 * half, row0);
+                        bulk_commit();
+                    }
+                    ++nbox;
+                }
+            }
+            tc_fence_before();
+            if (leader)
+                mbar_arrive(&acc_empty[acc]);
+            else
+                mbar_arrive_cluster(acc_empty0 + acc * 8);
+        }
+        if (lane == 0)
+            bulk_wait_all();  // the last boxes are written before the CTA and its shared memory go
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // the leader's MMAs read this CTA's shared memory until here
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, C::kTmemCols);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
+{
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) ==
+                cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    });
+    return fn;
+}
+
+bool encode_2d(CUtensorMap* m, CUtensorMapDataType type, const void* p, long inner, long outer, long row_bytes,
+               int box_inner, int box_outer)
+{
+    auto fn = encode_fn();
+    const cuuint64_t dims[2] = {cuuint64_t(inner), cuuint64_t(outer)};
+    const cuuint64_t strides[1] = {cuuint64_t(row_bytes)};
+    const cuuint32_t box[2] = {cuuint32_t(box_inner), cuuint32_t(box_outer)};
+    const cuuint32_t es[2] = {1, 1};
+    return fn && fn(m, type, 2, const_cast<void*>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int MR>
+cudaError_t launch_rows(const GemmI8Args& a, cudaStream_t st)
+{
+    // Few rows of W and a long K: a block a pair of rows, its warps along K. Otherwise a warp takes 4 rows of W where that
+    // still gives every SM eight warps, else one.
+    const int warps = 8 * num_sms();
+    if (a.N < 4 * warps && a.K >= 4096)
+        return launch_k(k_i8_rows<MR, 2, 8>, dim3((a.N + 1) / 2), 256, 0, st, a);
+    if (a.N >= 4 * warps)
+        return launch_k(k_i8_rows<MR, 4, 1>, dim3((a.N + 31) / 32), 256, 0, st, a);
+    return launch_k(k_i8_rows<MR, 1, 1>, dim3((a.N + 7) / 8), 256, 0, st, a);
+}
+
+template <int BN>
+cudaError_t launch_split(const I8Params& P, int tiles, cudaStream_t st)
+{
+    static std::atomic<uint64_t> devs{0};
+    const cudaError_t e = smem_limit_once(devs, k_i8_split<BN>, SplitCfg<BN>::kSmem);
+    if (e != cudaSuccess)
+        return e;
+    return launch_k_cluster(k_i8_split<BN>, dim3(unsigned(tiles) * P.splits), P.splits, 192, SplitCfg<BN>::kSmem, st, P);
+}
+
+template <int BN>
+cudaError_t launch_pair(const I8Params& P, int tiles, cudaStream_t st)
+{
+    static std::atomic<uint64_t> devs{0};
+    const cudaError_t e = smem_limit_once(devs, k_i8_pair<BN>, PairCfg<BN>::kSmem);
+    if (e != cudaSuccess)
+        return e;
+    const int pairs = std::min(tiles, num_sms() / 2);
+    return launch_k(k_i8_pair<BN>, dim3(2 * pairs), 192, PairCfg<BN>::kSmem, st, P);
 }
 
 }  // namespace
 
 cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
 {
-    (void)err;
-    const cudaError_t e = launch_k(k_gemm_i8_simple, dim3((a.N + 63) / 64, (a.M + 63) / 64), 256, 0, st, a);
+    cudaError_t e;
+    if (a.M <= kRowsMax) {
+        e = a.M == 1   ? launch_rows<1>(a, st)
+            : a.M == 2 ? launch_rows<2>(a, st)
+            : a.M <= 4 ? launch_rows<4>(a, st)
+                       : launch_rows<8>(a, st);
+    } else {
+        I8Params P{};
+        P.a = a;
+        const long sms = num_sms(), num_k = (a.K + kBK - 1) / kBK;
+        const auto tiles = [&](int rows, int bn) { return ((a.M + rows - 1L) / rows) * ((a.N + bn - 1L) / bn); };
+        // Single-SM tiles when they fit one round (or one row of tiles is all there is), cut along K as far as the SMs and whole stages allow (at least four
+        // stages a part: below that the exchange of the sums costs more than the loads it saves).
+        const bool split = tiles(128, 64) <= sms || a.M <= 128;
+        const int sbn = tiles(128, 64) <= sms ? 64 : 128;
+        if (split) {
+            P.splits = 1;
+            while (P.splits < 8 && tiles(128, sbn) * P.splits * 2 <= sms && num_k >= 8 * P.splits)
+                P.splits *= 2;
+        }
+        // Pair tiles of 256 or 128 columns: whichever has the shorter last-round cost.
+        const long slots = sms / 2;
+        const int pbn = (tiles(256, 256) + slots - 1) / slots * 2 <= (tiles(256, 128) + slots - 1) / slots ? 256 : 128;
+        const int rows = 128, cols = split ? sbn : pbn / 2;
+        const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+        if (!encode_2d(&P.tx, u8, a.x, a.K, a.M, a.ldx, kBK, rows) ||
+            !encode_2d(&P.tw, u8, a.w, a.K, a.N, a.ldw, kBK, cols)) {
+            *err = "proj_i8: tensor map encoding failed";
+            return cudaErrorInvalidValue;
+        }
+        if (split) {
+            e = sbn == 64 ? launch_split<64>(P, int(tiles(128, 64)), st) : launch_split<128>(P, int(tiles(128, 128)), st);
+        } else {
+            const int size = a.out_f32 ? 4 : 2;
+            P.boxes = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.ldy * size) % 16 == 0;
+            if (P.boxes && !encode_2d(&P.ty, a.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                      a.y, a.N, a.M, a.ldy * size, 128 / size, 32)) {
+                *err = "proj_i8: tensor map encoding failed";
+                return cudaErrorInvalidValue;
+            }
+            e = pbn == 256 ? launch_pair<256>(P, int(tiles(256, 256)), st) : launch_pair<128>(P, int(tiles(256, 128)), st);
+        }
+    }
     if (e != cudaSuccess)
         return e;
     count_launch();

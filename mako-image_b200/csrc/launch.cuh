@@ -44,10 +44,10 @@ inline cudaError_t launch_k(void (*kernel)(KArgs...), dim3 grid, dim3 block, siz
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
-// The same launch as clusters of two CTAs along x (a kernel written for CTA pairs without __cluster_dims__).
+// The same launch as clusters of `size` CTAs along x (a kernel written for clusters without __cluster_dims__).
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_k_pairs(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                                  Args&&... args)
+inline cudaError_t launch_k_cluster(void (*kernel)(KArgs...), dim3 grid, unsigned size, dim3 block, size_t smem,
+                                    cudaStream_t st, Args&&... args)
 {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
@@ -56,7 +56,7 @@ inline cudaError_t launch_k_pairs(void (*kernel)(KArgs...), dim3 grid, dim3 bloc
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.x = size;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -64,6 +64,14 @@ inline cudaError_t launch_k_pairs(void (*kernel)(KArgs...), dim3 grid, dim3 bloc
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+
+// Clusters of two: CTA pairs.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_k_pairs(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                                  Args&&... args)
+{
+    return launch_k_cluster(kernel, grid, 2, block, smem, st, std::forward<Args>(args)...);
 }
 
 // Raises a kernel's dynamic shared-memory limit to `bytes` on the current device. cudaFuncSetAttribute acts on the

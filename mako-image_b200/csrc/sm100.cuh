@@ -309,6 +309,19 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
         : "memory");
 }
 
+// D[tmem] (+)= A[smem desc] * B[smem desc]^T, kind::i8 (signed 8-bit operands, 32-bit integer accumulate, 32 values of K
+// each). Single thread.
+__device__ __forceinline__ void mma_i8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
 // Arrive once on *bar when every tcgen05.mma issued so far by this thread has completed.
 __device__ __forceinline__ void mma_commit(uint64_t* bar)
 {
@@ -392,6 +405,16 @@ __host__ __device__ constexpr uint32_t idesc_bf16_f32(int M, int N, int a_mn = 0
            | (1u << 10)                // B format: bf16
            | (uint32_t(a_mn) << 15)    // A major
            | (uint32_t(b_mn) << 16)    // B major
+           | (uint32_t(N >> 3) << 17)  // N / 8
+           | (uint32_t(M >> 4) << 24); // M / 16
+}
+
+// Instruction descriptor of kind::i8: signed 8-bit A and B, both K-major, 32-bit integer accumulator.
+__host__ __device__ constexpr uint32_t idesc_i8_s32(int M, int N)
+{
+    return (2u << 4)                   // D format: s32
+           | (1u << 7)                 // A format: s8
+           | (1u << 10)                // B format: s8
            | (uint32_t(N >> 3) << 17)  // N / 8
            | (uint32_t(M >> 4) << 24); // M / 16
 }
@@ -482,6 +505,18 @@ __device__ __forceinline__ void mma_bf16_ss_pair(uint32_t d_tmem, uint64_t a_des
         "{\n\t.reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// The same on 8-bit integers (kind::i8): one 256 x N x 32 MMA.
+__device__ __forceinline__ void mma_i8_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }

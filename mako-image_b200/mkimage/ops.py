@@ -212,37 +212,53 @@ NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 OUT_NONE, OUT_BF16, OUT_F32, OUT_I8 = 0, 1, 2, 3
 
 
-def _need(ok, what):
-    if not ok:
-        raise MkbError(1, what)
+def _fail(what):
+    raise MkbError(1, what)
 
 
-def _on(name, device, **tensors):
-    """Every given tensor lives on the CUDA device `device`."""
-    for k, t in tensors.items():
-        _need(t is None or t.device == device, f"{name}: {k} is on {getattr(t, 'device', None)}, not on {device}")
-    _need(device.type == "cuda", f"{name}: tensors must be CUDA tensors")
+def _device_of(name, *tensors):
+    """The one CUDA device that the given tensors live on."""
+    dev = tensors[0].get_device()
+    if dev < 0:
+        _fail(f"{name}: tensors must be CUDA tensors")
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            _fail(f"{name}: a tensor is on {t.device}, not on cuda:{dev}")
+    return dev
 
 
-def _launch(fn, device, *args):
+def _launch(fn, dev, *args):
     """fn(*args, stream) on the tensors' device and its current stream, whatever device is current."""
     import torch
 
-    if torch.cuda.current_device() == device.index:
-        return check(fn(*args, stream_ptr()))
-    with torch.cuda.device(device):
-        return check(fn(*args, stream_ptr()))
+    if torch._C._cuda_getDevice() == dev:
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if code:
+        check(code)
 
 
-def _row_stride(t):
-    """Elements between rows of a 2-D tensor (a single row may come with any stride)."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
-def _rows_i8(rows, n, device):
+def _row_stride(t, n):
+    """Elements between the rows of a 2-D tensor of n columns (a single row may come with any stride)."""
+    s = t.stride(0)
+    return s if s >= n else n if t.shape[0] <= 1 else s
+
+
+def _rows_i8(rows, n, dev):
     import torch
 
-    return torch.empty(rows, -(-n // 16) * 16, device=device, dtype=torch.int8)[:, :n]
+    return torch.empty_strided((rows, n), (-(-n // 16) * 16, 1), device=dev, dtype=torch.int8)
+
+
+def _vector(t, n, f32, what):
+    if t is not None and (t.dtype != f32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1)):
+        _fail(what)
 
 
 def quantize_rows(x, q=None, scale=None):
@@ -250,20 +266,23 @@ def quantize_rows(x, q=None, scale=None):
     is x to half a step (see mkb_quantize_rows). q's rows are 16 bytes aligned, as proj_i8 wants them."""
     import torch
 
-    _need(x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float32), "quantize_rows: x must be 2-D bf16 or fp32")
+    dtype = x.dtype
+    if x.dim() != 2 or (dtype != torch.bfloat16 and dtype != torch.float32):
+        _fail("quantize_rows: x must be 2-D bf16 or fp32")
     rows, n = x.shape
+    if n == 0 or (n > 1 and x.stride(1) != 1):
+        _fail("quantize_rows: the values of a row must be contiguous, one at least")
     if q is None:
         q = _rows_i8(rows, n, x.device)
+    elif q.shape != x.shape or q.dtype != torch.int8 or (n > 1 and q.stride(1) != 1):
+        _fail("quantize_rows: q must be int8 rows of x's shape")
     if scale is None:
         scale = torch.empty(rows, device=x.device, dtype=torch.float32)
-    _on("quantize_rows", x.device, x=x, q=q, scale=scale)
-    _need(n > 0 and x.stride(1) == 1 or n == 1, "quantize_rows: the values of a row must be contiguous")
-    _need(q.shape == x.shape and q.dtype == torch.int8 and (q.stride(1) == 1 or n == 1),
-          "quantize_rows: q must be int8 rows of x's shape")
-    _need(scale.shape == (rows,) and scale.dtype == torch.float32 and scale.is_contiguous(),
-          "quantize_rows: scale must be contiguous fp32 [rows]")
-    _launch(lib.mkb_quantize_rows, x.device, _p(x), _row_stride(x), int(x.dtype == torch.float32), _p(q),
-            _row_stride(q), _p(scale), rows, n)
+    else:
+        _vector(scale, rows, torch.float32, "quantize_rows: scale must be contiguous fp32 [rows]")
+    dev = _device_of("quantize_rows", x, q, scale)
+    _launch(lib.mkb_quantize_rows, dev, x.data_ptr(), _row_stride(x, n), dtype == torch.float32, q.data_ptr(),
+            _row_stride(q, n), scale.data_ptr(), rows, n)
     return q, scale
 
 
@@ -272,22 +291,27 @@ def proj_i8(x, x_scale, w, w_scale, bias=None, act=ACT_NONE, out=None, out_f32=F
     (quantize_rows makes such rows), scales fp32, exact integer sums (see mkb_proj_i8)."""
     import torch
 
-    _need(x.dim() == 2 and w.dim() == 2 and x.dtype == torch.int8 and w.dtype == torch.int8 and
-          x.shape[1] == w.shape[1], "proj_i8: x [M][K] and w [N][K] must be int8")
+    f32 = torch.float32
+    if x.dtype != torch.int8 or w.dtype != torch.int8 or x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        _fail("proj_i8: x [M][K] and w [N][K] must be int8")
     M, K = x.shape
     N = w.shape[0]
     if out is None:
-        out = torch.empty(M, N, device=x.device, dtype=torch.float32 if out_f32 else torch.bfloat16)
-    _on("proj_i8", x.device, x=x, x_scale=x_scale, w=w, w_scale=w_scale, bias=bias, out=out)
-    for t in (x, w, out):
-        _need(t.stride(1) == 1 or t.shape[1] == 1, "proj_i8: the values of a row must be contiguous")
-    _need(out.shape == (M, N) and out.dtype in (torch.float32, torch.bfloat16), "proj_i8: out must be [M][N] fp32 or bf16")
-    for t, n in ((x_scale, M), (w_scale, N), (bias, N)):
-        _need(t is None or (t.shape == (n,) and t.dtype == torch.float32 and t.is_contiguous()),
-              "proj_i8: scales and bias must be contiguous fp32 vectors, one value a row of x or w")
-    ldx, ldw = (t.stride(0) if t.shape[0] > 1 else -(-max(t.stride(0), K) // 16) * 16 for t in (x, w))
-    _launch(lib.mkb_proj_i8, x.device, _p(x), ldx, _p(x_scale), _p(w), ldw, _p(w_scale), _p(bias), _p(out),
-            _row_stride(out), M, N, K, act, int(out.dtype == torch.float32))
+        out = torch.empty(M, N, device=x.device, dtype=f32 if out_f32 else torch.bfloat16)
+    else:
+        out_f32 = out.dtype == f32
+        if out.shape != (M, N) or (not out_f32 and out.dtype != torch.bfloat16) or (N > 1 and out.stride(1) != 1):
+            _fail("proj_i8: out must be [M][N] fp32 or bf16 with contiguous rows")
+    if K > 1 and (x.stride(1) != 1 or w.stride(1) != 1):
+        _fail("proj_i8: the values of a row must be contiguous")
+    _vector(x_scale, M, f32, "proj_i8: x_scale must be contiguous fp32 [M]")
+    _vector(w_scale, N, f32, "proj_i8: w_scale must be contiguous fp32 [N]")
+    _vector(bias, N, f32, "proj_i8: bias must be contiguous fp32 [N]")
+    dev = _device_of("proj_i8", x, x_scale, w, w_scale, bias, out)
+    ldx = x.stride(0) if M > 1 else -(-K // 16) * 16
+    ldw = w.stride(0) if N > 1 else -(-K // 16) * 16
+    _launch(lib.mkb_proj_i8, dev, x.data_ptr(), ldx, x_scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(),
+            _ptr(bias), out.data_ptr(), _row_stride(out, N), M, N, K, act, out_f32)
     return out
 
 
@@ -304,47 +328,69 @@ def gate_add_norm(x, y=None, y_norm=NORM_NONE, y_weight=None, gate=None, tanh_ga
     import torch
 
     f32 = torch.float32
-    _need(x.dim() == 2 and x.dtype == f32, "gate_add_norm: x must be 2-D fp32")
+    if x.dim() != 2 or x.dtype != f32:
+        _fail("gate_add_norm: x must be 2-D fp32")
     rows, n = x.shape
     rps = rows_per_sample or max(rows, 1)
     samples = -(-rows // rps)
-    if x_out is None:
-        x_out = x
-    if out_type == OUT_I8:
-        if out is None:
-            out = _rows_i8(rows, n, x.device)
-        if out_scale is None:
-            out_scale = torch.empty(rows, device=x.device, dtype=f32)
-    elif out_type != OUT_NONE and out is None:
-        out = torch.empty(rows, n, device=x.device, dtype=f32 if out_type == OUT_F32 else torch.bfloat16)
-    _on("gate_add_norm", x.device, x=x, y=y, y_weight=y_weight, gate=gate, x_weight=x_weight, scale=scale, shift=shift,
-        x_out=x_out, out=out, out_scale=out_scale)
-    want = {OUT_BF16: torch.bfloat16, OUT_F32: f32, OUT_I8: torch.int8}.get(out_type)
-    _need(x_out.dtype == f32 and (y is None or y.dtype in (f32, torch.bfloat16)) and
-          (out is None) == (want is None) and (out is None or out.dtype == want), "gate_add_norm: wrong type")
-    for t in (x, x_out, y, out):
-        _need(t is None or (t.shape == x.shape and (n == 1 or t.stride(1) == 1)),
-              "gate_add_norm: x, x_out, y and out must be [rows][n] with contiguous rows")
-    for t in (y_weight, x_weight):
-        _need(t is None or (t.shape == (n,) and t.dtype == f32 and t.is_contiguous()),
-              "gate_add_norm: weights must be contiguous fp32 [n]")
-    for t in (gate, scale, shift):
-        _need(t is None or (t.dtype == f32 and t.shape[-1] == n and t.stride(-1) == 1 and
-                            (t.dim() == 1 or (t.dim() == 2 and t.shape[0] in (1, samples) or rows == 0))),
-              "gate_add_norm: gate, scale and shift must be fp32 [n] or [samples][n]")
-    _need(out_scale is None or (out_type == OUT_I8 and out_scale.shape == (rows,) and out_scale.dtype == f32 and
-                                out_scale.is_contiguous()), "gate_add_norm: out_scale must be contiguous fp32 [rows]")
+
+    def rows_of(t, dtype):
+        if t.shape != x.shape or t.dtype != dtype or (n > 1 and t.stride(1) != 1):
+            _fail("gate_add_norm: x, x_out, y and out must be [rows][n] of their types with contiguous rows")
+        return _row_stride(t, n)
 
     def per_sample(t):
-        return t.stride(0) if t is not None and t.dim() == 2 and t.shape[0] > 1 else 0
+        if t is None:
+            return 0
+        if t.dtype != f32 or t.shape[-1] != n or (n > 1 and t.stride(-1) != 1):
+            _fail("gate_add_norm: gate, scale and shift must be fp32 [n] or [samples][n]")
+        if t.dim() == 1:
+            return 0
+        if t.dim() != 2 or (t.shape[0] != samples and t.shape[0] != 1):
+            _fail("gate_add_norm: gate, scale and shift must be fp32 [n] or [samples][n]")
+        return t.stride(0) if t.shape[0] > 1 else 0
 
-    _need(scale is None or shift is None or samples <= 1 or per_sample(scale) == per_sample(shift),
-          "gate_add_norm: scale and shift must have the same strides")
-    _launch(lib.mkb_gate_add_norm, x.device, _p(x), _row_stride(x), _p(x_out), _row_stride(x_out), _p(y),
-            _row_stride(y) if y is not None else 0, int(y is not None and y.dtype == f32), y_norm, _p(y_weight),
-            _p(gate), per_sample(gate), int(tanh_gate), x_norm if out_type != OUT_NONE else NORM_NONE, _p(x_weight),
-            _p(scale), _p(shift), per_sample(scale if scale is not None else shift), rps, eps, _p(out),
-            _row_stride(out) if out is not None else 0, out_type, _p(out_scale), rows, n)
+    ldx = rows_of(x, f32)
+    if x_out is None:
+        x_out, ldxo = x, ldx
+    else:
+        ldxo = rows_of(x_out, f32)
+    ldy, y_f32 = 0, False
+    if y is not None:
+        y_f32 = y.dtype == f32
+        ldy = rows_of(y, f32 if y_f32 else torch.bfloat16)
+    if out_type == OUT_NONE:
+        if out is not None:
+            _fail("gate_add_norm: out without an out_type")
+        x_norm, ldo = NORM_NONE, 0
+    else:
+        dtype = torch.bfloat16 if out_type == OUT_BF16 else f32 if out_type == OUT_F32 else torch.int8
+        if out is not None:
+            ldo = rows_of(out, dtype)
+        elif out_type == OUT_I8:
+            out = _rows_i8(rows, n, x.device)
+            ldo = -(-n // 16) * 16
+        else:
+            out = torch.empty(rows, n, device=x.device, dtype=dtype)
+            ldo = n
+    if out_type == OUT_I8:
+        if out_scale is None:
+            out_scale = torch.empty(rows, device=x.device, dtype=f32)
+        else:
+            _vector(out_scale, rows, f32, "gate_add_norm: out_scale must be contiguous fp32 [rows]")
+    elif out_scale is not None:
+        _fail("gate_add_norm: out_scale goes with 8-bit outputs alone")
+    _vector(y_weight, n, f32, "gate_add_norm: weights must be contiguous fp32 [n]")
+    _vector(x_weight, n, f32, "gate_add_norm: weights must be contiguous fp32 [n]")
+    gate_stride, mod_stride, shift_stride = per_sample(gate), per_sample(scale), per_sample(shift)
+    if scale is None:
+        mod_stride = shift_stride
+    elif shift is not None and shift_stride != mod_stride and samples > 1:
+        _fail("gate_add_norm: scale and shift must have the same strides")
+    dev = _device_of("gate_add_norm", x, y, y_weight, gate, x_weight, scale, shift, x_out, out, out_scale)
+    _launch(lib.mkb_gate_add_norm, dev, x.data_ptr(), ldx, x_out.data_ptr(), ldxo, _ptr(y), ldy, y_f32, y_norm,
+            _ptr(y_weight), _ptr(gate), gate_stride, tanh_gate, x_norm, _ptr(x_weight), _ptr(scale), _ptr(shift),
+            mod_stride, rps, eps, _ptr(out), ldo, out_type, _ptr(out_scale), rows, n)
     return (out, out_scale) if out_type == OUT_I8 else out
 
 
@@ -355,24 +401,41 @@ def cross_attention(q, k, v, key_len=None, key_mask=None, scale=None, out=None):
     [B][Lq][H][d] or [B][Lq][H * d] bf16)."""
     import torch
 
-    _need(q.dim() == 4 and k.dim() == 4 and v.shape == k.shape and q.shape[0] == k.shape[0] and q.shape[3] == k.shape[3],
-          "cross_attention: q must be [B][H][Lq][d], k and v [B][Hkv][Lk][d]")
+    bf16 = torch.bfloat16
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+        _fail("cross_attention: q must be [B][H][Lq][d], k and v [B][Hkv][Lk][d]")
     B, H, Lq, d = q.shape
-    Hkv, Lk = k.shape[1], k.shape[2]
+    Bk, Hkv, Lk, dk = k.shape
+    if Bk != B or dk != d:
+        _fail("cross_attention: q must be [B][H][Lq][d], k and v [B][Hkv][Lk][d]")
     if out is None:
-        out = torch.empty(B, Lq, H * d, device=q.device, dtype=torch.bfloat16)
-    _need(tuple(out.shape) in ((B, Lq, H * d), (B, Lq, H, d)), "cross_attention: out must be [B][Lq][H * d]")
-    heads = (out.stride(0), out.stride(2) if out.dim() == 4 else d, out.stride(1))
-    _on("cross_attention", q.device, q=q, k=k, v=v, out=out, key_len=key_len, key_mask=key_mask)
+        out = torch.empty(B, Lq, H * d, device=q.device, dtype=bf16)
+        o_row, o_head, o_sample = H * d, d, Lq * H * d
+    elif out.shape == (B, Lq, H * d):
+        o_sample, o_row, o_last = out.stride()
+        o_head = d
+    elif out.shape == (B, Lq, H, d):
+        o_sample, o_row, o_head, o_last = out.stride()
+    else:
+        _fail("cross_attention: out must be [B][Lq][H * d]")
+    q_sample, q_head, q_row, q_last = q.stride()
+    k_sample, k_head, k_row, k_last = k.stride()
+    v_sample, v_head, v_row, v_last = v.stride()
     for t in (q, k, v, out):
-        _need(t.dtype == torch.bfloat16 and t.stride(-1) == 1, "cross_attention: tensors must be bf16 with contiguous heads")
-    _need(key_len is None or (key_len.shape == (B,) and key_len.dtype == torch.int32 and key_len.is_contiguous()),
-          "cross_attention: key_len must be contiguous int32 [B]")
-    _need(key_mask is None or (key_mask.shape == (B, Lk) and key_mask.dtype in (torch.bool, torch.uint8) and
-                               (key_mask.stride(1) == 1 or Lk <= 1)), "cross_attention: key_mask must be bool [B][Lk]")
-    _need(scale is None or scale > 0, "cross_attention: the scale must be positive")
-    _launch(lib.mkb_cross_attention, q.device, _p(q), q.stride(2), q.stride(1), q.stride(0), _p(k), k.stride(2),
-            k.stride(1), k.stride(0), _p(v), v.stride(2), v.stride(1), v.stride(0), _p(out), heads[2], heads[1],
-            heads[0], B, H, Hkv, Lq, Lk, d, _p(key_len), _p(key_mask),
-            key_mask.stride(0) if key_mask is not None else 0, scale or 0.0)
+        if t.dtype != bf16 or t.stride(-1) != 1:
+            _fail("cross_attention: tensors must be bf16 with contiguous heads")
+    if key_len is not None and (key_len.dtype != torch.int32 or key_len.shape != (B,) or (B > 1 and key_len.stride(0) != 1)):
+        _fail("cross_attention: key_len must be contiguous int32 [B]")
+    mask_stride = 0
+    if key_mask is not None:
+        if key_mask.shape != (B, Lk) or key_mask.dtype not in (torch.bool, torch.uint8) or \
+                (Lk > 1 and key_mask.stride(1) != 1):
+            _fail("cross_attention: key_mask must be bool [B][Lk]")
+        mask_stride = key_mask.stride(0)
+    if scale is not None and not scale > 0:
+        _fail("cross_attention: the scale must be positive")
+    dev = _device_of("cross_attention", q, k, v, out, key_len, key_mask)
+    _launch(lib.mkb_cross_attention, dev, q.data_ptr(), q_row, q_head, q_sample, k.data_ptr(), k_row, k_head, k_sample,
+            v.data_ptr(), v_row, v_head, v_sample, out.data_ptr(), o_row, o_head, o_sample, B, H, Hkv, Lq, Lk, d,
+            _ptr(key_len), _ptr(key_mask), mask_stride, scale or 0.0)
     return out
