@@ -3,10 +3,14 @@
 // Keys are few and queries many, so the work is a stream of query tiles past small sets of keys: persistent CTAs walk
 // items of (sample, head, 256 query rows) as two 128-row tiles A and B, and every stage runs ahead into the next item, so
 // that one item's loads, another's products and a third's stores overlap. Twelve warps:
-//   warp 0     TMA: Q tiles (double-buffered) and K and V tiles of 128 keys into one ring
-//   warp 1     MMA: S = Q K^T, then O += P V with P in tensor memory, for A and B in turn
-//   warp 2     with key lengths or masks: clears the V rows of keys that no query sees (0 * NaN would spread)
-//   warps 4-7  softmax of tile A, 8-11 of tile B: a thread a row, the running maximum and sum of one pass
+//   warp 0     TMA: Q tiles (two buffers for each of A and B), K and V tiles of 128 keys in one ring
+//   warp 1     MMA: S = Q K^T, then O += P V with P in tensor memory, for A and B in turn (a warp for each of A and B, whose
+//              products then mix on the tensor pipe, was slower: 603 against 455 us at 2 x 24 x 4096 x 4096 x 128)
+//   warp 2     where keys are hidden (lengths, masks, an odd Lk): a bound for each key's score, -inf for a hidden one, and
+//              zeros over the hidden rows of V (0 * NaN would spread)
+//   warps 4-7  softmax of tile A, 8-11 of tile B: a thread a row, the running maximum and sum of one pass; the output rows
+//              are staged in the Q tile that made them and leave as TMA stores (a thread storing its row directly touches
+//              32 lines an instruction)
 // Only ceil(visible / 16) * 16 keys of the last tile are multiplied and exponentiated (77 keys cost 80, not 128).
 // TMEM columns: S_A [0, 128), S_B [128, 256), O_A [256, 384), O_B [384, 512); P takes the first half of its S.
 #include "cross_attention.cuh"
@@ -19,6 +23,7 @@
 #include <cudaTypedefs.h>
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 namespace mkb {
 
@@ -28,27 +33,28 @@ constexpr int kThreads = 384;
 // The launch gives every thread 168 registers; the control warpgroup drops to kRegsCtl and the softmax warpgroups rise to
 // kRegsSoftmax, enough for a row's 128 scores.
 constexpr int kLaunchRegs = (65536 / kThreads) / 8 * 8;
-constexpr int kRegsCtl = 56, kRegsSoftmax = 216;
+constexpr int kRegsCtl = 88, kRegsSoftmax = 208;
 static_assert(128 * kRegsCtl + 256 * kRegsSoftmax <= kThreads * kLaunchRegs, "register split exceeds the CTA pool");
 constexpr int kTile = 128;              // query rows a tile, keys a tile
 constexpr int kPanel = kTile * 64 * 2;  // 64 bf16 columns of 128 rows
 constexpr int kSteps = 4;               // full barriers of K and of V: no more key steps than that are ever in flight
+constexpr int kHideSteps = 2;           // key steps whose hidden keys are kept ready
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: O is rescaled only when a row's maximum grows by more
 
 template <int D>
 struct Cfg {
     static constexpr int kTileBytes = (D / 64) * kPanel;
-    static constexpr int kSlots = D == 64 ? 8 : 3;  // K and V tiles in flight beside the four Q tiles
-    static constexpr int kSmem = 1024 + (4 + kSlots) * kTileBytes + 512;
+    static constexpr int kSlots = D == 64 ? 8 : 3;  // K and V tiles beside the four Q tiles
+    static constexpr int kSmem = 1024 + (4 + kSlots) * kTileBytes + 512 + kHideSteps * (kTile * 4 + 16);
     static_assert(kSmem <= 227 * 1024);
     static_assert((kSlots + 1) / 2 <= kSteps);
 };
 
 struct CrossParams {
-    CUtensorMap tq, tk, tv;
+    CUtensorMap tq, tk, tv, to;
     CrossArgs a;
     // 0 where a dimension is shared (stride 0): its coordinate stays 0.
-    int q_head, q_sample, kv_head_k, kv_sample_k, kv_head_v, kv_sample_v;
+    int q_head, q_sample, kv_head_k, kv_sample_k, kv_head_v, kv_sample_v, o_head, o_sample;
     int items, blocks;  // work items, query blocks of 256 rows
 };
 
@@ -106,16 +112,99 @@ struct Walk {
     __device__ __forceinline__ int width() const { return min(kTile, (it.n - j * kTile + 15) & ~15); }
 };
 
-// Bit i of the 32 keys from `key` on: visible (below n and not masked). All lanes of a warp take part and get the word.
-__device__ __forceinline__ uint32_t visible_word(const CrossArgs& a, int b, int n, int key)
+// Bit i of word c: key + 32 c + i is visible (below n and not masked). All lanes of a warp take part and get the words.
+__device__ __forceinline__ void visible_words(const CrossArgs& a, int b, int n, int key, uint32_t (&see)[4])
 {
-    const int left = n - key;
-    uint32_t w = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1;
-    if (a.key_mask) {
-        const int k = key + int(threadIdx.x & 31);
-        w &= __ballot_sync(0xffffffffu, k < n && __ldg(a.key_mask + b * a.mask_stride + k) != 0);
+    uint8_t byte[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const int k = key + 32 * c + int(threadIdx.x & 31);
+        byte[c] = k < n ? 1 : 0;
+        if (a.key_mask && k < n)
+            byte[c] = __ldg(a.key_mask + b * a.mask_stride + k);
     }
-    return w;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+        see[c] = __ballot_sync(0xffffffffu, byte[c] != 0);
+}
+
+// A row's step over CH chunks of 32 keys: its scores in tensor memory at ts to weights 2^(s sc - m), bf16, over the first
+// half of the same columns; the row's maximum m and sum l; O at `to` rescaled where the maximum grew. Chunk c has hidden keys
+// where bit c of `hidden` is set: then each score is cut at its key's bound, +inf or -inf (the minimum drops a NaN, and a
+// visible NaN comes back as inf - inf). Straight code for each CH: the chunks' loads, exponentials and stores interleave.
+template <int D, int CH>
+__device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, uint32_t hidden, const float* bound, float sc,
+                                             bool first, float& m, float& l)
+{
+    uint32_t s[32 * CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+        tmem_ld32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
+    tmem_wait_ld();
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+        if ((hidden >> c) & 1) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+                const float4 b = *reinterpret_cast<const float4*>(bound + 32 * c + i);
+                s[32 * c + i] = __float_as_uint(fminf(__uint_as_float(s[32 * c + i]), b.x));
+                s[32 * c + i + 1] = __float_as_uint(fminf(__uint_as_float(s[32 * c + i + 1]), b.y));
+                s[32 * c + i + 2] = __float_as_uint(fminf(__uint_as_float(s[32 * c + i + 2]), b.z));
+                s[32 * c + i + 3] = __float_as_uint(fminf(__uint_as_float(s[32 * c + i + 3]), b.w));
+            }
+        }
+    // The maximum as 8 independent chains.
+    float mc[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+        mc[u] = fmaxf(__uint_as_float(s[2 * u]), __uint_as_float(s[2 * u + 1]));
+#pragma unroll
+    for (int i = 16; i < 32 * CH; i += 16)
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            mc[u] = fmax3(mc[u], __uint_as_float(s[i + 2 * u]), __uint_as_float(s[i + 2 * u + 1]));
+    const float mx = fmax3(fmax3(mc[0], mc[1], mc[2]), fmax3(mc[3], mc[4], mc[5]), fmaxf(mc[6], mc[7])) * sc;
+    const bool need = mx > m + kRescaleThreshold;  // also the first step with a visible key
+    if (__any_sync(0xffffffffu, need)) {
+        const float m_new = need ? mx : m;
+        const float f = m == -INFINITY ? 0.0f : ex2(m - m_new);
+        l *= f;
+        if (!first) {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(to + c * 32, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    tmem_st16(to + c * 32 + 16 * i, *reinterpret_cast<uint32_t(*)[16]>(&o[16 * i]));
+            }
+        }
+        m = m_new;
+    }
+    // A row that has seen no key yet: 2^(-inf - 0) = 0 for all of them.
+    const float shift = m == -INFINITY ? 0.0f : -m;
+    const float2 sc2 = make_float2(sc, sc), sh2 = make_float2(shift, shift);
+    float2 ls[4] = {};
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        uint32_t p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int k = 32 * c + 2 * i;
+            const float2 x = ffma2(make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), sc2, sh2);
+            const float2 e = make_float2(ex2(x.x), ex2(x.y));
+            ls[i & 3] = fadd2(ls[i & 3], e);
+            p[i] = pack_bf16x2(e.x, e.y);
+        }
+        tmem_st16(ts + 16 * c, p);
+    }
+    tmem_wait_st();
+    const float2 l2 = fadd2(fadd2(ls[0], ls[1]), fadd2(ls[2], ls[3]));
+    l += l2.x + l2.y;
 }
 
 template <int D>
@@ -125,18 +214,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
     constexpr int TB = C::kTileBytes, NS = C::kSlots;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sQ = smem;            // [2 buffers][2 tiles]
-    uint8_t* sKV = smem + 4 * TB;  // [slots]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (4 + NS) * TB);
-    uint64_t* q_full = bars;             // [2 buffers][2 tiles]
-    uint64_t* q_empty = q_full + 4;      // [2 buffers][2 tiles]
-    uint64_t* kv_empty = q_empty + 4;    // [slots]
+    uint8_t* sQ = smem;            // [2 tiles][2 buffers]
+    uint8_t* sKV = smem + 4 * TB;  // [NS]
+    float* bounds = reinterpret_cast<float*>(smem + (4 + NS) * TB);  // [kHideSteps][kTile]
+    volatile uint32_t* hiddens = reinterpret_cast<volatile uint32_t*>(bounds + kHideSteps * kTile);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(bounds + kHideSteps * (kTile + 4));
+    uint64_t* q_full = bars;             // [2 tiles][2 buffers]
+    uint64_t* q_empty = q_full + 4;      // [2 tiles][2 buffers]
+    uint64_t* kv_empty = q_empty + 4;    // [NS]
     // By key step, not by slot: where K and V take turns in a slot, a warp that follows only the V tiles would miss phases
     // of the slot's barrier.
     uint64_t* k_full = kv_empty + NS;    // [kSteps]
     uint64_t* v_full = k_full + kSteps;  // [kSteps]
-    uint64_t* v_ready = v_full + kSteps; // [kSteps] V with its unseen rows cleared
-    uint64_t* s_full = v_ready + kSteps; // [tiles]
+    uint64_t* v_ready = v_full + kSteps; // [kSteps] V with its hidden rows cleared
+    uint64_t* h_full = v_ready + kSteps; // [kHideSteps]
+    uint64_t* h_empty = h_full + kHideSteps;
+    uint64_t* s_full = h_empty + kHideSteps;  // [tiles]
     uint64_t* p_full = s_full + 2;       // [tiles]
     uint64_t* o_full = p_full + 2;       // [tiles]
     uint64_t* drain = o_full + 2;
@@ -144,12 +237,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const CrossArgs& a = P.a;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const bool clear_v = a.key_len || a.key_mask;
+    const bool clear_v = a.key_len || a.key_mask, hide = clear_v || a.Lk % 32;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 4; ++i) {
             mbar_init(&q_full[i], 1);
-            mbar_init(&q_empty[i], 1);
+            mbar_init(&q_empty[i], 4);  // the warps whose output rows have left the tile
         }
         for (int i = 0; i < NS; ++i)
             mbar_init(&kv_empty[i], 1);
@@ -157,6 +250,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             mbar_init(&k_full[i], 1);
             mbar_init(&v_full[i], 1);
             mbar_init(&v_ready[i], 1);
+        }
+        for (int i = 0; i < kHideSteps; ++i) {
+            mbar_init(&h_full[i], 1);
+            mbar_init(&h_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
@@ -171,6 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
         prefetch_tmap(&P.tq);
         prefetch_tmap(&P.tk);
         prefetch_tmap(&P.tv);
+        prefetch_tmap(&P.to);
     }
     grid_dep_wait();  // before TMEM allocation and the first global access
     if (warp == 1) {
@@ -188,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
     if (warp == 0) {
         if (lane == 0) {
             Walk w;
-            uint32_t seq = 0, nq[2] = {0, 0};  // ring position; Q tiles issued of A and B
+            uint32_t seq = 0, nq0 = 0, nq1 = 0;  // K and V tiles, Q tiles of A and of B loaded
             bool ok = true;
             const auto load = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int row, int h, int b) {
                 mbar_arrive_expect_tx(bar, TB);
@@ -198,16 +296,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             };
             for (w.first(P); w.more(P) && ok; w.next(P)) {
                 const int hk = w.it.h / (a.H / a.Hkv);
-                if (w.j == 0)
-                    for (int t = 0; t < w.it.tiles && ok; ++t) {
-                        const uint32_t buf = nq[t] & 1, i = buf * 2 + t;
-                        ok = mbar_wait(&q_empty[i], ((nq[t] >> 1) & 1) ^ 1, a.status, kErrAttnWait, abort_flag);
-                        if (ok) {
-                            load(sQ + i * TB, &P.tq, &q_full[i], w.it.q0 + t * kTile, w.it.h * P.q_head,
-                                 w.it.b * P.q_sample);
-                            ++nq[t];
-                        }
-                    }
+                for (int t = 0; w.j == 0 && t < w.it.tiles && ok; ++t) {
+                    const uint32_t n = t ? nq1++ : nq0++, i = 2 * t + (n & 1);
+                    ok = mbar_wait(&q_empty[i], ((n >> 1) & 1) ^ 1, a.status, kErrAttnWait, abort_flag);
+                    if (ok)
+                        load(sQ + i * TB, &P.tq, &q_full[i], w.it.q0 + t * kTile, w.it.h * P.q_head, w.it.b * P.q_sample);
+                    else
+                        --(t ? nq1 : nq0);
+                }
                 for (int kv = 0; kv < 2 && ok; ++kv) {
                     const uint32_t s = seq % NS;
                     ok = mbar_wait(&kv_empty[s], ((seq / NS) & 1) ^ 1, a.status, kErrAttnWait, abort_flag);
@@ -222,9 +318,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 }
             }
             if (!ok) {  // let the loads already issued land before the CTA can exit
-                for (int t = 0; t < 2; ++t)
-                    for (uint32_t i = nq[t] > 2 ? nq[t] - 2 : 0; i < nq[t]; ++i)
-                        mbar_wait(&q_full[(i & 1) * 2 + t], (i >> 1) & 1, a.status, kErrWaitDrain, nullptr);
+                for (int t = 0; t < 2; ++t) {
+                    const uint32_t n = t ? nq1 : nq0;
+                    for (uint32_t i = n > 2 ? n - 2 : 0; i < n; ++i)
+                        mbar_wait(&q_full[2 * t + (i & 1)], (i >> 1) & 1, a.status, kErrWaitDrain, nullptr);
+                }
                 for (uint32_t i = seq > NS ? seq - NS : 0; i < seq; ++i)
                     mbar_wait(&(i & 1 ? v_full : k_full)[(i >> 1) % kSteps], ((i >> 1) / kSteps) & 1, a.status,
                               kErrWaitDrain, nullptr);
@@ -233,72 +331,76 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
     } else if (warp == 1) {
         if (lane == 0) {
             constexpr uint32_t idesc_s0 = idesc_bf16_f32(128, 0), idesc_o = idesc_bf16_f32(128, D, 0, 1);
-            const uint32_t q_addr = smem_u32(sQ), kv_addr = smem_u32(sKV);
-            uint32_t seq = 0, nq[2] = {0, 0}, np[2] = {0, 0};  // as the producer's; P tiles taken of A and B
+            const uint64_t dq0 = desc_kmajor_sw128(smem_u32(sQ)), dk0 = desc_kmajor_sw128(smem_u32(sKV)),
+                           dv0 = desc_mnmajor_sw128(smem_u32(sKV), kPanel, 1024);  // in units of 16 bytes
+            constexpr uint32_t kUnit = TB >> 4;
+            uint32_t step = 0, nq[2] = {0, 0}, np[2] = {0, 0};  // key steps; Q and P tiles taken of A and B
             bool ok = true;
-            // S_t of step w, K in slot s. The item's first step waits for Q, its last frees it.
-            const auto scores = [&](const Walk& w, int t, uint32_t s) {
-                const uint32_t i = (nq[t] & 1) * 2 + t;
-                if (w.j == 0 && !mbar_wait(&q_full[i], (nq[t] >> 1) & 1, a.status, kErrAttnWait, abort_flag))
+            const auto wait = [&](uint64_t* bar, uint32_t phase) {
+                return mbar_wait(bar, phase & 1, a.status, kErrAttnWait, abort_flag);
+            };
+            constexpr std::integral_constant<int, 0> kA;
+            constexpr std::integral_constant<int, 1> kB;
+            // S_t = Q_t K^T; Q is waited for at an item's first step.
+            const auto scores = [&](auto tile, bool first, bool last, uint64_t dk, uint32_t idesc) {
+                constexpr int t = decltype(tile)::value;
+                const uint64_t dq = dq0 + (2 * t + (nq[t] & 1)) * kUnit;
+                if (first && !wait(&q_full[2 * t + (nq[t] & 1)], nq[t] >> 1))
                     return false;
                 tc_fence_after();
-                const uint32_t idesc = idesc_s0 | uint32_t(w.width() >> 3) << 17;
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (k >> 2) * kPanel + (k & 3) * 32;
-                    mma_bf16_ss(tmem + t * 128, desc_kmajor_sw128(q_addr + i * TB + off),
-                                desc_kmajor_sw128(kv_addr + s * TB + off), idesc, k > 0);
+                    const uint32_t off = ((k >> 2) * kPanel + (k & 3) * 32) >> 4;
+                    mma_bf16_ss(tmem + t * 128, dq + off, dk + off, idesc, k > 0);
                 }
                 mma_commit(&s_full[t]);
-                if (w.last()) {
-                    mma_commit(&q_empty[i]);
-                    ++nq[t];
-                }
+                nq[t] += last;
                 return true;
             };
-            const auto wait_kv = [&](uint64_t* bars, uint32_t step) {
-                return mbar_wait(&bars[step % kSteps], (step / kSteps) & 1, a.status, kErrAttnWait, abort_flag);
+            // O_t += P_t V.
+            const auto outputs = [&](auto tile, bool first, bool last, uint64_t dv, int width) {
+                constexpr int t = decltype(tile)::value;
+                if (!wait(&p_full[t], np[t]))
+                    return false;
+                ++np[t];
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (16 * k < width)
+                        mma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * k, dv + k * (2048 >> 4), idesc_o,
+                                    !first || k > 0);
+                if (last)
+                    mma_commit(&o_full[t]);
+                return true;
             };
             Walk w, x;
             w.first(P);
             if (w.more(P)) {
-                ok = wait_kv(k_full, 0);
-                for (int t = 0; t < w.it.tiles && ok; ++t)
-                    ok = scores(w, t, 0);
+                const uint32_t idesc = idesc_s0 | uint32_t(w.width() >> 3) << 17;
+                ok = wait(&k_full[0], 0) && scores(kA, true, w.last(), dk0, idesc) &&
+                     (w.it.tiles < 2 || scores(kB, true, w.last(), dk0, idesc));
                 if (ok)
                     mma_commit(&kv_empty[0]);
             }
-            // Per step: O_A += P_A V, S_A of the next step, then B: one tile's softmax runs under the other's products.
-            for (; w.more(P) && ok; w = x, seq += 2) {
+            // Per step: O_A += P_A V, S_A of the next step, then B: one tile's softmax runs under the other's products. What
+            // the products need is worked out before the wait for P.
+            for (; w.more(P) && ok; w = x, ++step) {
                 x = w;
                 x.next(P);
-                const bool more = x.more(P);
-                const uint32_t sv = (seq + 1) % NS, sk = (seq + 2) % NS;
-                ok = wait_kv(clear_v ? v_ready : v_full, seq >> 1);
-                const int tiles = more ? max(w.it.tiles, x.it.tiles) : w.it.tiles;
-                for (int t = 0; t < tiles && ok; ++t) {
-                    if (t < w.it.tiles) {
-                        ok = mbar_wait(&p_full[t], np[t] & 1, a.status, kErrAttnWait, abort_flag);
-                        if (!ok)
-                            break;
-                        ++np[t];
-                        tc_fence_after();
-                        const int steps = w.width() >> 4;
-#pragma unroll 1
-                        for (int k = 0; k < steps; ++k)
-                            mma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * k,
-                                        desc_mnmajor_sw128(kv_addr + sv * TB + k * 2048, kPanel, 1024), idesc_o,
-                                        (w.j > 0) || (k > 0));
-                        if (w.last())
-                            mma_commit(&o_full[t]);
-                    }
-                    if (more && t == 0)
-                        ok = wait_kv(k_full, (seq >> 1) + 1);
-                    if (more && ok && t < x.it.tiles)
-                        ok = scores(x, t, sk);
-                }
+                const bool more = x.more(P), first = w.j == 0, last = w.last(), xfirst = x.j == 0, xlast = x.last();
+                const bool b = w.it.tiles > 1, xb = more && x.it.tiles > 1;
+                const int width = w.width();
+                const uint32_t sv = (2 * step + 1) % NS, sk = (2 * step + 2) % NS;
+                const uint64_t dv = dv0 + sv * kUnit, dk = dk0 + sk * kUnit;
+                const uint32_t idesc = idesc_s0 | uint32_t(x.width() >> 3) << 17;
+                const auto next_k = [&] { return wait(&k_full[(step + 1) % kSteps], (step + 1) / kSteps); };
+                ok = wait(&(clear_v ? v_ready : v_full)[step % kSteps], step / kSteps) &&
+                     outputs(kA, first, last, dv, width) && (!more || (next_k() && scores(kA, xfirst, xlast, dk, idesc))) &&
+                     (!b || outputs(kB, first, last, dv, width)) && (!xb || scores(kB, xfirst, xlast, dk, idesc));
                 if (!ok)
                     break;
+                if (hide)  // the step's weights are made, so its bounds have been read
+                    mma_commit(&h_empty[step % kHideSteps]);
                 mma_commit(&kv_empty[sv]);
                 if (more)
                     mma_commit(&kv_empty[sk]);
@@ -307,29 +409,42 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             mbar_wait(drain, 0, a.status, kErrWaitDrain, nullptr);
         }
     } else if (warp == 2) {
-        if (clear_v) {
+        if (hide) {
             Walk w;
             uint32_t step = 0;
             for (w.first(P); w.more(P); w.next(P), ++step) {
-                const uint32_t s = (2 * step + 1) % NS;
-                uint32_t hide[4];
+                const uint32_t s = (2 * step + 1) % NS, hs = step % kHideSteps;
+                const int width = w.width();
+                uint32_t see[4], hidden = 0;
+                visible_words(a, w.it.b, w.it.n, w.j * kTile, see);
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    hide[c] = ~visible_word(a, w.it.b, w.it.n, w.j * kTile + 32 * c);
+                    hidden |= see[c] != 0xffffffffu ? 1u << c : 0u;
+                if (!mbar_wait(&h_empty[hs], ((step / kHideSteps) & 1) ^ 1, a.status, kErrAttnWait, abort_flag))
+                    break;
+                if (hidden) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        bounds[hs * kTile + 32 * c + lane] = (see[c] >> lane) & 1 ? INFINITY : -INFINITY;
+                }
+                if (lane == 0)
+                    hiddens[hs] = hidden;
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(&h_full[hs]);
+                if (!clear_v)
+                    continue;
                 if (!mbar_wait(&v_full[step % kSteps], (step / kSteps) & 1, a.status, kErrAttnWait, abort_flag))
                     break;
-                const int width = w.width();
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    if (32 * c < width && hide[c]) {
-                        if ((hide[c] >> lane) & 1) {
-                            uint8_t* row = sKV + s * TB + (32 * c + lane) * 128;
+                    if (32 * c < width && !((see[c] >> lane) & 1)) {
+                        uint8_t* row = sKV + s * TB + (32 * c + lane) * 128;
 #pragma unroll
-                            for (int p = 0; p < D / 64; ++p)
+                        for (int p = 0; p < D / 64; ++p)
 #pragma unroll
-                                for (int i = 0; i < 8; ++i)
-                                    *reinterpret_cast<uint4*>(row + p * kPanel + i * 16) = make_uint4(0, 0, 0, 0);
-                        }
+                            for (int i = 0; i < 8; ++i)
+                                *reinterpret_cast<uint4*>(row + p * kPanel + i * 16) = make_uint4(0, 0, 0, 0);
                     }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -339,132 +454,97 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
         }
     } else if (warp >= 4) {
         regs_increase<kRegsSoftmax>();
-        const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
-        const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
+        const int t = (warp - 4) >> 2, w32 = (warp & 3) * 32, r = w32 + lane;
+        const uint32_t lanes = tmem + (uint32_t(w32) << 16);
         const uint32_t ts = lanes + t * 128, to = lanes + 256 + t * 128;
-        const float sc = a.scale_log2;
-        uint32_t ns = 0, no = 0;  // S and O tiles taken
+        uint32_t ns = 0, no = 0, step = 0;  // S and O tiles taken; key steps of all items so far
         Item it;
-        for (int item = blockIdx.x; item < P.items; item += gridDim.x) {
+        bool ok = true;
+        for (int item = blockIdx.x; item < P.items && ok; item += gridDim.x) {
             it.set(P, item);
-            if (t >= it.tiles)
+            if (t >= it.tiles) {
+                step += it.steps;
                 continue;
+            }
+            const int row0 = it.q0 + t * kTile + w32;  // of the warp
+            if (it.steps == 0) {  // no keys: zeros, a row's 16-byte pieces side by side
+                constexpr int per = D / 8;
+                for (int i = lane; i < 32 * per; i += 32) {
+                    const long row = row0 + i / per;
+                    if (row < a.Lq)
+                        *reinterpret_cast<uint4*>(a.out + it.b * a.so.sample + it.h * a.so.head + row * a.so.row +
+                                                  i % per * 8) = make_uint4(0, 0, 0, 0);
+                }
+                continue;
+            }
             float m = -INFINITY, l = 0.0f;
-            bool ok = true;
-            for (int j = 0; j < it.steps; ++j) {
-                uint32_t see[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    see[c] = visible_word(a, it.b, it.n, j * kTile + 32 * c);
-                const int chunks = min(4, (it.n - j * kTile + 31) >> 5);
+            for (int j = 0; j < it.steps; ++j, ++step) {
                 if (!mbar_wait(&s_full[t], ns & 1, a.status, kErrAttnWait, abort_flag)) {
                     ok = false;
                     break;
                 }
                 ++ns;
                 tc_fence_after();
-                uint32_t s[128];
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (c < chunks)
-                        tmem_ld32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
-                tmem_wait_ld();
-                float mc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (c < chunks) {
-                        if (see[c] != 0xffffffffu) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (!((see[c] >> i) & 1))
-                                    s[32 * c + i] = __float_as_uint(-INFINITY);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8)
-#pragma unroll
-                            for (int u = 0; u < 4; ++u)
-                                mc[u] = fmax3(mc[u], __uint_as_float(s[32 * c + i + 2 * u]),
-                                              __uint_as_float(s[32 * c + i + 2 * u + 1]));
-                    }
-                const float mx = fmaxf(fmax3(mc[0], mc[1], mc[2]), mc[3]) * sc;
-                const bool need = mx > m + kRescaleThreshold;  // also the first tile with a visible key
-                if (__any_sync(0xffffffffu, need)) {
-                    const float m_new = need ? mx : m;
-                    const float f = m == -INFINITY ? 0.0f : ex2(m - m_new);
-                    l *= f;
-                    if (j > 0) {
-#pragma unroll 1
-                        for (int c = 0; c < D / 16; ++c) {
-                            uint32_t o[16];
-                            tmem_ld16(to + c * 16, o);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_st16(to + c * 16, o);
-                        }
-                    }
-                    m = m_new;
+                if (j == 0 && no > 0 && lane == 0) {  // the last item's rows are out by now: its Q tile is free
+                    bulk_wait_read<0>();
+                    mbar_arrive(&q_empty[2 * t + ((no - 1) & 1)]);
                 }
-                // A row that has seen no key yet: 2^(-inf - 0) = 0 for all of them.
-                const float shift = m == -INFINITY ? 0.0f : -m;
-                const float2 sc2 = make_float2(sc, sc), sh2 = make_float2(shift, shift);
-                float2 ls[4] = {};
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (c < chunks) {
-                        uint32_t p[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int k = 32 * c + 2 * i;
-                            const float2 x = ffma2(make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), sc2, sh2);
-                            const float2 e = make_float2(ex2(x.x), ex2(x.y));
-                            ls[i & 3] = fadd2(ls[i & 3], e);
-                            p[i] = pack_bf16x2(e.x, e.y);
-                        }
-                        tmem_st16(ts + 16 * c, p);
+                __syncwarp();
+                uint32_t hidden = 0;
+                const float* bound = bounds + step % kHideSteps * kTile;
+                if (hide) {  // after the scores: a tile that skipped items may be phases ahead of the bounds until then
+                    const uint32_t s = step % kHideSteps;
+                    if (!mbar_wait(&h_full[s], (step / kHideSteps) & 1, a.status, kErrAttnWait, abort_flag)) {
+                        ok = false;
+                        break;
                     }
-                tmem_wait_st();
+                    hidden = hiddens[s];
+                }
+                switch (min(4, (it.n - j * kTile + 31) >> 5)) {
+                case 1: softmax_step<D, 1>(ts, to, hidden, bound, a.scale_log2, j == 0, m, l); break;
+                case 2: softmax_step<D, 2>(ts, to, hidden, bound, a.scale_log2, j == 0, m, l); break;
+                case 3: softmax_step<D, 3>(ts, to, hidden, bound, a.scale_log2, j == 0, m, l); break;
+                default: softmax_step<D, 4>(ts, to, hidden, bound, a.scale_log2, j == 0, m, l); break;
+                }
                 tc_fence_before();
                 mbar_arrive(&p_full[t]);
-                const float2 l2 = fadd2(fadd2(ls[0], ls[1]), fadd2(ls[2], ls[3]));
-                l += l2.x + l2.y;
             }
-            if (!ok)
+            if (!ok || !mbar_wait(&o_full[t], no & 1, a.status, kErrAttnWait, abort_flag))
                 break;
-            const int row = it.q0 + t * kTile + r;
-            __nv_bfloat16* dst = a.out + it.b * a.so.sample + it.h * a.so.head + long(row) * a.so.row;
-            const bool in = row < a.Lq;
-            if (it.steps == 0) {
-                if (in)
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
-                        reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
-                continue;
-            }
-            if (!mbar_wait(&o_full[t], no & 1, a.status, kErrAttnWait, abort_flag))
-                break;
-            ++no;
             tc_fence_after();
+            // The item's scores are all made, so its Q tile takes the output rows on their way out.
+            uint8_t* stage = sQ + (2 * t + (no & 1)) * TB;
+            ++no;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t o[32];
                 tmem_ld32(to + c * 32, o);
                 tmem_wait_ld();
-                if (in) {
-                    uint4* d = reinterpret_cast<uint4*>(dst + c * 32);
+                uint8_t* dst = stage + (c >> 1) * kPanel + r * 128;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        d[i] = make_uint4(
-                            pack_bf16x2(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv),
-                            pack_bf16x2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv),
-                            pack_bf16x2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv),
-                            pack_bf16x2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv));
-                }
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<uint4*>(dst + ((((c & 1) * 4 + i) ^ (r & 7)) << 4)) = make_uint4(
+                        pack_bf16x2(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv),
+                        pack_bf16x2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv),
+                        pack_bf16x2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv),
+                        pack_bf16x2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv));
             }
             tc_fence_before();  // O has been read before the P that lets the next item's product overwrite it
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (row0 < a.Lq)
+#pragma unroll
+                    for (int p = 0; p < D / 64; ++p)
+                        tma_store_4d(&P.to, stage + p * kPanel + w32 * 128, p * 64, row0, it.h * P.o_head,
+                                     it.b * P.o_sample);
+                bulk_commit();
+            }
+            __syncwarp();
         }
+        if (lane == 0)
+            bulk_wait_all();  // the last rows are written before the CTA and its shared memory go
     }
 
     tc_fence_before();
@@ -492,9 +572,9 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
     return fn;
 }
 
-// [samples][heads][rows][d] with its strides as a 4-D map, box 64 x 128 rows with the 128-byte swizzle; rows past the
+// [samples][heads][rows][d] with its strides as a 4-D map, box 64 x box_rows with the 128-byte swizzle; rows past the
 // tensor read as zeros. A shared dimension (stride 0) is one element long and its use flag 0.
-bool encode_heads(CUtensorMap* m, const void* p, const HeadStrides& s, int rows, int heads, int samples, int d,
+bool encode_heads(CUtensorMap* m, const void* p, const HeadStrides& s, int rows, int heads, int samples, int d, int box_rows,
                   int* use_head, int* use_sample)
 {
     auto fn = encode_fn();
@@ -504,7 +584,7 @@ bool encode_heads(CUtensorMap* m, const void* p, const HeadStrides& s, int rows,
                                 cuuint64_t(*use_sample ? samples : 1)};
     const cuuint64_t strides[3] = {cuuint64_t(s.row) * 2, cuuint64_t(*use_head ? s.head : s.row) * 2,
                                    cuuint64_t(*use_sample ? s.sample : s.row) * 2};
-    const cuuint32_t box[4] = {64, kTile, 1, 1}, es[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, cuuint32_t(box_rows), 1, 1}, es[4] = {1, 1, 1, 1};
     return fn && fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, strides, box, es,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -548,9 +628,10 @@ cudaError_t cross_attention(const CrossArgs& a, const char** err, cudaStream_t s
     P.items = a.B * a.H * P.blocks;
     const void* k = a.Lk ? a.k : a.q;  // no keys: the maps are not used
     const void* v = a.Lk ? a.v : a.q;
-    if (!encode_heads(&P.tq, a.q, a.sq, a.Lq, a.H, a.B, a.d, &P.q_head, &P.q_sample) ||
-        !encode_heads(&P.tk, k, a.sk, a.Lk, a.Hkv, a.B, a.d, &P.kv_head_k, &P.kv_sample_k) ||
-        !encode_heads(&P.tv, v, a.sv, a.Lk, a.Hkv, a.B, a.d, &P.kv_head_v, &P.kv_sample_v)) {
+    if (!encode_heads(&P.tq, a.q, a.sq, a.Lq, a.H, a.B, a.d, kTile, &P.q_head, &P.q_sample) ||
+        !encode_heads(&P.tk, k, a.sk, a.Lk, a.Hkv, a.B, a.d, kTile, &P.kv_head_k, &P.kv_sample_k) ||
+        !encode_heads(&P.tv, v, a.sv, a.Lk, a.Hkv, a.B, a.d, kTile, &P.kv_head_v, &P.kv_sample_v) ||
+        !encode_heads(&P.to, a.out, a.so, a.Lq, a.H, a.B, a.d, 32, &P.o_head, &P.o_sample)) {
         *err = "cross_attention: tensor map encoding failed";
         return cudaErrorInvalidValue;
     }
