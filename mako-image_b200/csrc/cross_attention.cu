@@ -6,11 +6,11 @@
 //   warp 0     TMA: Q tiles (two buffers for each of A and B), K and V tiles of 128 keys in one ring
 //   warp 1     MMA: S = Q K^T, then O += P V with P in tensor memory, for A and B in turn (a warp for each of A and B, whose
 //              products then mix on the tensor pipe, was slower: 603 against 455 us at 2 x 24 x 4096 x 4096 x 128)
-//   warp 2     where keys are hidden (lengths, masks, an odd Lk): a bound for each key's score, -inf for a hidden one, and
-//              zeros over the hidden rows of V (0 * NaN would spread)
-//   warps 4-7  softmax of tile A, 8-11 of tile B: a thread a row, the running maximum and sum of one pass; the output rows
-//              are staged in the Q tile that made them and leave as TMA stores (a thread storing its row directly touches
-//              32 lines an instruction)
+//   warp 2     with a mask: a bound for each key's score, -inf for a hidden one, ahead of the softmax
+//   warps 4-7  softmax of tile A, 8-11 of tile B: a thread a row, the running maximum and sum of one pass; where a step has
+//              hidden keys each thread also clears its row of V if that is one (0 * NaN would spread); the output rows are
+//              staged in the Q tile that made them and leave as TMA stores (a thread storing its row directly touches 32
+//              lines an instruction)
 // Only ceil(visible / 16) * 16 keys of the last tile are multiplied and exponentiated (77 keys cost 80, not 128).
 // TMEM columns: S_A [0, 128), S_B [128, 256), O_A [256, 384), O_B [384, 512); P takes the first half of its S.
 #include "cross_attention.cuh"
@@ -112,29 +112,14 @@ struct Walk {
     __device__ __forceinline__ int width() const { return min(kTile, (it.n - j * kTile + 15) & ~15); }
 };
 
-// Bit i of word c: key + 32 c + i is visible (below n and not masked). All lanes of a warp take part and get the words.
-__device__ __forceinline__ void visible_words(const CrossArgs& a, int b, int n, int key, uint32_t (&see)[4])
-{
-    uint8_t byte[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const int k = key + 32 * c + int(threadIdx.x & 31);
-        byte[c] = k < n ? 1 : 0;
-        if (a.key_mask && k < n)
-            byte[c] = __ldg(a.key_mask + b * a.mask_stride + k);
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-        see[c] = __ballot_sync(0xffffffffu, byte[c] != 0);
-}
-
 // A row's step over CH chunks of 32 keys: its scores in tensor memory at ts to weights 2^(s sc - m), bf16, over the first
-// half of the same columns; the row's maximum m and sum l; O at `to` rescaled where the maximum grew. Chunk c has hidden keys
-// where bit c of `hidden` is set: then each score is cut at its key's bound, +inf or -inf (the minimum drops a NaN, and a
-// visible NaN comes back as inf - inf). Straight code for each CH: the chunks' loads, exponentials and stores interleave.
+// half of the same columns; the row's maximum m and sum l; O at `to` rescaled where the maximum grew. Of the last chunk only the
+// first `tail` keys are visible. Chunk c has masked keys where bit c of `masked` is set: then each score is cut at its key's
+// bound, +inf or -inf (the minimum drops a NaN, and a visible NaN comes back as inf - inf). Straight code for each CH: the
+// chunks' loads, exponentials and stores interleave.
 template <int D, int CH>
-__device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, uint32_t hidden, const float* bound, float sc,
-                                             bool first, float& m, float& l)
+__device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int tail, uint32_t masked, const float* bound,
+                                             float sc, bool first, float& m, float& l)
 {
     uint32_t s[32 * CH];
 #pragma unroll
@@ -143,7 +128,7 @@ __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, uint32_t 
     tmem_wait_ld();
 #pragma unroll
     for (int c = 0; c < CH; ++c)
-        if ((hidden >> c) & 1) {
+        if ((masked >> c) & 1) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
                 const float4 b = *reinterpret_cast<const float4*>(bound + 32 * c + i);
@@ -153,6 +138,12 @@ __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, uint32_t 
                 s[32 * c + i + 3] = __float_as_uint(fminf(__uint_as_float(s[32 * c + i + 3]), b.w));
             }
         }
+    if (tail < 32) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i >= tail)
+                s[32 * (CH - 1) + i] = __float_as_uint(-INFINITY);
+    }
     // The maximum as 8 independent chains.
     float mc[8];
 #pragma unroll
@@ -217,17 +208,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
     uint8_t* sQ = smem;            // [2 tiles][2 buffers]
     uint8_t* sKV = smem + 4 * TB;  // [NS]
     float* bounds = reinterpret_cast<float*>(smem + (4 + NS) * TB);  // [kHideSteps][kTile]
-    volatile uint32_t* hiddens = reinterpret_cast<volatile uint32_t*>(bounds + kHideSteps * kTile);
+    volatile uint32_t* maskeds = reinterpret_cast<volatile uint32_t*>(bounds + kHideSteps * kTile);
     uint64_t* bars = reinterpret_cast<uint64_t*>(bounds + kHideSteps * (kTile + 4));
     uint64_t* q_full = bars;             // [2 tiles][2 buffers]
     uint64_t* q_empty = q_full + 4;      // [2 tiles][2 buffers]
     uint64_t* kv_empty = q_empty + 4;    // [NS]
-    // By key step, not by slot: where K and V take turns in a slot, a warp that follows only the V tiles would miss phases
+    // By key step, not by slot: where K and V take turns in a slot, threads that follow only the V tiles would miss phases
     // of the slot's barrier.
     uint64_t* k_full = kv_empty + NS;    // [kSteps]
     uint64_t* v_full = k_full + kSteps;  // [kSteps]
-    uint64_t* v_ready = v_full + kSteps; // [kSteps] V with its hidden rows cleared
-    uint64_t* h_full = v_ready + kSteps; // [kHideSteps]
+    uint64_t* h_full = v_full + kSteps;  // [kHideSteps]
     uint64_t* h_empty = h_full + kHideSteps;
     uint64_t* s_full = h_empty + kHideSteps;  // [tiles]
     uint64_t* p_full = s_full + 2;       // [tiles]
@@ -237,7 +227,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const CrossArgs& a = P.a;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const bool clear_v = a.key_len || a.key_mask, hide = clear_v || a.Lk % 32;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 4; ++i) {
@@ -249,7 +238,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
         for (int i = 0; i < kSteps; ++i) {
             mbar_init(&k_full[i], 1);
             mbar_init(&v_full[i], 1);
-            mbar_init(&v_ready[i], 1);
         }
         for (int i = 0; i < kHideSteps; ++i) {
             mbar_init(&h_full[i], 1);
@@ -394,12 +382,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 const uint64_t dv = dv0 + sv * kUnit, dk = dk0 + sk * kUnit;
                 const uint32_t idesc = idesc_s0 | uint32_t(x.width() >> 3) << 17;
                 const auto next_k = [&] { return wait(&k_full[(step + 1) % kSteps], (step + 1) / kSteps); };
-                ok = wait(&(clear_v ? v_ready : v_full)[step % kSteps], step / kSteps) &&
+                ok = wait(&v_full[step % kSteps], step / kSteps) &&
                      outputs(kA, first, last, dv, width) && (!more || (next_k() && scores(kA, xfirst, xlast, dk, idesc))) &&
                      (!b || outputs(kB, first, last, dv, width)) && (!xb || scores(kB, xfirst, xlast, dk, idesc));
                 if (!ok)
                     break;
-                if (hide)  // the step's weights are made, so its bounds have been read
+                if (a.key_mask)  // the step's weights are made, so its bounds have been read
                     mma_commit(&h_empty[step % kHideSteps]);
                 mma_commit(&kv_empty[sv]);
                 if (more)
@@ -409,47 +397,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             mbar_wait(drain, 0, a.status, kErrWaitDrain, nullptr);
         }
     } else if (warp == 2) {
-        if (hide) {
+        if (a.key_mask) {
             Walk w;
             uint32_t step = 0;
             for (w.first(P); w.more(P); w.next(P), ++step) {
-                const uint32_t s = (2 * step + 1) % NS, hs = step % kHideSteps;
-                const int width = w.width();
-                uint32_t see[4], hidden = 0;
-                visible_words(a, w.it.b, w.it.n, w.j * kTile, see);
+                const uint32_t hs = step % kHideSteps;
+                const uint8_t* bytes = a.key_mask + w.it.b * a.mask_stride + w.j * kTile;
+                const int left = w.it.n - w.j * kTile;
+                bool see[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    hidden |= see[c] != 0xffffffffu ? 1u << c : 0u;
+                    see[c] = 32 * c + lane < left && __ldg(bytes + 32 * c + lane) != 0;
+                uint32_t masked = 0;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    masked |= __all_sync(0xffffffffu, see[c]) ? 0u : 1u << c;
                 if (!mbar_wait(&h_empty[hs], ((step / kHideSteps) & 1) ^ 1, a.status, kErrAttnWait, abort_flag))
                     break;
-                if (hidden) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        bounds[hs * kTile + 32 * c + lane] = (see[c] >> lane) & 1 ? INFINITY : -INFINITY;
-                }
+                for (int c = 0; c < 4; ++c)
+                    bounds[hs * kTile + 32 * c + lane] = see[c] ? INFINITY : -INFINITY;
                 if (lane == 0)
-                    hiddens[hs] = hidden;
+                    maskeds[hs] = masked;
                 __syncwarp();
                 if (lane == 0)
                     mbar_arrive(&h_full[hs]);
-                if (!clear_v)
-                    continue;
-                if (!mbar_wait(&v_full[step % kSteps], (step / kSteps) & 1, a.status, kErrAttnWait, abort_flag))
-                    break;
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (32 * c < width && !((see[c] >> lane) & 1)) {
-                        uint8_t* row = sKV + s * TB + (32 * c + lane) * 128;
-#pragma unroll
-                        for (int p = 0; p < D / 64; ++p)
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                *reinterpret_cast<uint4*>(row + p * kPanel + i * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0)
-                    mbar_arrive(&v_ready[step % kSteps]);
             }
         }
     } else if (warp >= 4) {
@@ -490,21 +462,41 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                     mbar_arrive(&q_empty[2 * t + ((no - 1) & 1)]);
                 }
                 __syncwarp();
-                uint32_t hidden = 0;
+                const int valid = it.n - j * kTile;
+                int tail = valid >= kTile || valid % 32 == 0 ? 32 : valid % 32;
+                uint32_t masked = 0;
                 const float* bound = bounds + step % kHideSteps * kTile;
-                if (hide) {  // after the scores: a tile that skipped items may be phases ahead of the bounds until then
+                if (a.key_mask) {  // after the scores: a tile that skipped items may be phases ahead of the bounds until then
                     const uint32_t s = step % kHideSteps;
                     if (!mbar_wait(&h_full[s], (step / kHideSteps) & 1, a.status, kErrAttnWait, abort_flag)) {
                         ok = false;
                         break;
                     }
-                    hidden = hiddens[s];
+                    masked = maskeds[s];
+                    tail = 32;  // the bounds know of it
                 }
-                switch (min(4, (it.n - j * kTile + 31) >> 5)) {
-                case 1: softmax_step<D, 1>(ts, to, hidden, bound, a.scale_log2, j == 0, m, l); break;
-                case 2: softmax_step<D, 2>(ts, to, hidden, bound, a.scale_log2, j == 0, m, l); break;
-                case 3: softmax_step<D, 3>(ts, to, hidden, bound, a.scale_log2, j == 0, m, l); break;
-                default: softmax_step<D, 4>(ts, to, hidden, bound, a.scale_log2, j == 0, m, l); break;
+                switch (min(4, (valid + 31) >> 5)) {
+                case 1: softmax_step<D, 1>(ts, to, tail, masked, bound, a.scale_log2, j == 0, m, l); break;
+                case 2: softmax_step<D, 2>(ts, to, tail, masked, bound, a.scale_log2, j == 0, m, l); break;
+                case 3: softmax_step<D, 3>(ts, to, tail, masked, bound, a.scale_log2, j == 0, m, l); break;
+                default: softmax_step<D, 4>(ts, to, tail, masked, bound, a.scale_log2, j == 0, m, l); break;
+                }
+                if (masked || (valid < kTile && it.n < a.Lk)) {
+                    // Rows of V that are multiplied (those up to valid, in sixteens) and belong to hidden keys: both tiles'
+                    // threads clear them, whichever comes first. V stays until both tiles' products have read it.
+                    if (!mbar_wait(&v_full[step % kSteps], (step / kSteps) & 1, a.status, kErrAttnWait, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    if (r < ((valid + 15) & ~15) && (a.key_mask ? bound[r] < 0.0f : r >= valid)) {
+                        uint8_t* row = sKV + (2 * step + 1) % NS * TB + r * 128;
+#pragma unroll
+                        for (int p = 0; p < D / 64; ++p)
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                *reinterpret_cast<uint4*>(row + p * kPanel + ((i ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
                 }
                 tc_fence_before();
                 mbar_arrive(&p_full[t]);
