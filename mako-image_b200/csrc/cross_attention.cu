@@ -65,48 +65,79 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
-// One (sample, head, query block) and its keys.
-struct Item {
-    int b, h, q0, n, steps, tiles;  // n: keys up to the last that may be visible; steps of 128; 1 or 2 query tiles
-    __device__ __forceinline__ void set(const CrossParams& P, int item)
+// A CTA's items, gridDim.x apart: (sample, head, query block) and its keys. The digits of the item number are advanced by
+// the digits of the stride (a division for each item would sit in every role's way).
+struct Items {
+    int item, b, h, blk, db, dh, dblk;
+    int n, steps, tiles;  // n: keys up to the last that may be visible; steps of 128 of them; 1 or 2 query tiles
+    __device__ __forceinline__ void keys(const CrossArgs& a)
     {
-        const CrossArgs& a = P.a;
-        const int bh = item / P.blocks;
-        q0 = (item - bh * P.blocks) * 2 * kTile;
-        b = bh / a.H;
-        h = bh - b * a.H;
-        n = a.key_len ? min(max(__ldg(a.key_len + b), 0), a.Lk) : a.Lk;
-        steps = (n + kTile - 1) / kTile;
-        tiles = q0 + kTile < a.Lq ? 2 : 1;
+        n = a.key_len ? min(max(__ldg(a.key_len + min(b, a.B - 1)), 0), a.Lk) : a.Lk;
     }
-};
-
-// The walk over all key steps of a CTA's items that have keys.
-struct Walk {
-    Item it;
-    int item, j;
-    __device__ __forceinline__ void settle(const CrossParams& P)  // on to an item with keys
+    __device__ __forceinline__ void sizes(const CrossParams& P)
     {
-        j = 0;
-        for (; item < P.items; item += gridDim.x) {
-            it.set(P, item);
-            if (it.steps > 0)
-                return;
-        }
+        steps = (n + kTile - 1) / kTile;
+        tiles = blk * 2 * kTile + kTile < P.a.Lq ? 2 : 1;
     }
     __device__ __forceinline__ void first(const CrossParams& P)
     {
         item = blockIdx.x;
+        const int bh = item / P.blocks, dbh = int(gridDim.x) / P.blocks;
+        blk = item - bh * P.blocks;
+        b = bh / P.a.H;
+        h = bh - b * P.a.H;
+        dblk = int(gridDim.x) - dbh * P.blocks;
+        db = dbh / P.a.H;
+        dh = dbh - db * P.a.H;
+        keys(P.a);
+        sizes(P);
+    }
+    __device__ __forceinline__ void next(const CrossParams& P)
+    {
+        const int was = b;
+        item += gridDim.x;
+        blk += dblk;
+        h += dh;
+        b += db;
+        if (blk >= P.blocks) {
+            blk -= P.blocks;
+            ++h;
+        }
+        if (h >= P.a.H) {
+            h -= P.a.H;
+            ++b;
+        }
+        if (b != was)
+            keys(P.a);
+        sizes(P);
+    }
+    __device__ __forceinline__ bool more(const CrossParams& P) const { return item < P.items; }
+    __device__ __forceinline__ int q0() const { return blk * 2 * kTile; }
+};
+
+// The walk over all key steps of a CTA's items that have keys.
+struct Walk {
+    Items it;
+    int j;
+    __device__ __forceinline__ void settle(const CrossParams& P)  // on to an item with keys
+    {
+        j = 0;
+        while (it.more(P) && it.steps == 0)
+            it.next(P);
+    }
+    __device__ __forceinline__ void first(const CrossParams& P)
+    {
+        it.first(P);
         settle(P);
     }
     __device__ __forceinline__ void next(const CrossParams& P)
     {
         if (++j == it.steps) {
-            item += gridDim.x;
+            it.next(P);
             settle(P);
         }
     }
-    __device__ __forceinline__ bool more(const CrossParams& P) const { return item < P.items; }
+    __device__ __forceinline__ bool more(const CrossParams& P) const { return it.more(P); }
     __device__ __forceinline__ bool last() const { return j + 1 == it.steps; }
     // Keys of the step that are multiplied: those up to n, in sixteens.
     __device__ __forceinline__ int width() const { return min(kTile, (it.n - j * kTile + 15) & ~15); }
@@ -114,11 +145,10 @@ struct Walk {
 
 // A row's step over CH chunks of 32 keys: its scores in tensor memory at ts to weights 2^(s sc - m), bf16, over the first
 // half of the same columns; the row's maximum m and sum l; O at `to` rescaled where the maximum grew. Of the last chunk only the
-// first `tail` keys are visible. Chunk c has masked keys where bit c of `masked` is set: then each score is cut at its key's
-// bound, +inf or -inf (the minimum drops a NaN, and a visible NaN comes back as inf - inf). Straight code for each CH: the
+// first `tail` keys are visible. With `masked` each score is cut at its key's bound, +inf or -inf (the minimum drops a NaN, and a visible NaN comes back as inf - inf). Straight code for each CH: the
 // chunks' loads, exponentials and stores interleave.
 template <int D, int CH>
-__device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int tail, uint32_t masked, const float* bound,
+__device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int tail, bool masked, const float* bound,
                                              float sc, bool first, float& m, float& l)
 {
     uint32_t s[32 * CH];
@@ -126,19 +156,16 @@ __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int tail,
     for (int c = 0; c < CH; ++c)
         tmem_ld32(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&s[32 * c]));
     tmem_wait_ld();
+    if (masked) {
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-        if ((masked >> c) & 1) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-                const float4 b = *reinterpret_cast<const float4*>(bound + 32 * c + i);
-                s[32 * c + i] = __float_as_uint(fminf(__uint_as_float(s[32 * c + i]), b.x));
-                s[32 * c + i + 1] = __float_as_uint(fminf(__uint_as_float(s[32 * c + i + 1]), b.y));
-                s[32 * c + i + 2] = __float_as_uint(fminf(__uint_as_float(s[32 * c + i + 2]), b.z));
-                s[32 * c + i + 3] = __float_as_uint(fminf(__uint_as_float(s[32 * c + i + 3]), b.w));
-            }
+        for (int i = 0; i < 32 * CH; i += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(bound + i);
+            s[i] = __float_as_uint(fminf(__uint_as_float(s[i]), b.x));
+            s[i + 1] = __float_as_uint(fminf(__uint_as_float(s[i + 1]), b.y));
+            s[i + 2] = __float_as_uint(fminf(__uint_as_float(s[i + 2]), b.z));
+            s[i + 3] = __float_as_uint(fminf(__uint_as_float(s[i + 3]), b.w));
         }
-    if (tail < 32) {
+    } else if (tail < 32) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
             if (i >= tail)
@@ -288,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                     const uint32_t n = t ? nq1++ : nq0++, i = 2 * t + (n & 1);
                     ok = mbar_wait(&q_empty[i], ((n >> 1) & 1) ^ 1, a.status, kErrAttnWait, abort_flag);
                     if (ok)
-                        load(sQ + i * TB, &P.tq, &q_full[i], w.it.q0 + t * kTile, w.it.h * P.q_head, w.it.b * P.q_sample);
+                        load(sQ + i * TB, &P.tq, &q_full[i], w.it.q0() + t * kTile, w.it.h * P.q_head, w.it.b * P.q_sample);
                     else
                         --(t ? nq1 : nq0);
                 }
@@ -317,7 +344,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        // The whole warp walks and waits, so that addresses and descriptors stay in uniform registers; one lane issues.
+        {
             constexpr uint32_t idesc_s0 = idesc_bf16_f32(128, 0), idesc_o = idesc_bf16_f32(128, D, 0, 1);
             const uint64_t dq0 = desc_kmajor_sw128(smem_u32(sQ)), dk0 = desc_kmajor_sw128(smem_u32(sKV)),
                            dv0 = desc_mnmajor_sw128(smem_u32(sKV), kPanel, 1024);  // in units of 16 bytes
@@ -325,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             uint32_t step = 0, nq[2] = {0, 0}, np[2] = {0, 0};  // key steps; Q and P tiles taken of A and B
             bool ok = true;
             const auto wait = [&](uint64_t* bar, uint32_t phase) {
-                return mbar_wait(bar, phase & 1, a.status, kErrAttnWait, abort_flag);
+                return bool(__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, a.status, kErrAttnWait, abort_flag)));
             };
             constexpr std::integral_constant<int, 0> kA;
             constexpr std::integral_constant<int, 1> kB;
@@ -336,12 +364,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 if (first && !wait(&q_full[2 * t + (nq[t] & 1)], nq[t] >> 1))
                     return false;
                 tc_fence_after();
+                if (elect_one_sync()) {
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = ((k >> 2) * kPanel + (k & 3) * 32) >> 4;
-                    mma_bf16_ss(tmem + t * 128, dq + off, dk + off, idesc, k > 0);
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint32_t off = ((k >> 2) * kPanel + (k & 3) * 32) >> 4;
+                        mma_bf16_ss(tmem + t * 128, dq + off, dk + off, idesc, k > 0);
+                    }
+                    mma_commit(&s_full[t]);
                 }
-                mma_commit(&s_full[t]);
+                __syncwarp();
                 nq[t] += last;
                 return true;
             };
@@ -352,13 +383,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                     return false;
                 ++np[t];
                 tc_fence_after();
+                if (elect_one_sync()) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (16 * k < width)
-                        mma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * k, dv + k * (2048 >> 4), idesc_o,
-                                    !first || k > 0);
-                if (last)
-                    mma_commit(&o_full[t]);
+                    for (int k = 0; k < 8; ++k)
+                        if (16 * k < width)
+                            mma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * k, dv + k * (2048 >> 4), idesc_o,
+                                        !first || k > 0);
+                    if (last)
+                        mma_commit(&o_full[t]);
+                }
+                __syncwarp();
                 return true;
             };
             Walk w, x;
@@ -367,8 +401,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 const uint32_t idesc = idesc_s0 | uint32_t(w.width() >> 3) << 17;
                 ok = wait(&k_full[0], 0) && scores(kA, true, w.last(), dk0, idesc) &&
                      (w.it.tiles < 2 || scores(kB, true, w.last(), dk0, idesc));
-                if (ok)
+                if (ok && elect_one_sync())
                     mma_commit(&kv_empty[0]);
+                __syncwarp();
             }
             // Per step: O_A += P_A V, S_A of the next step, then B: one tile's softmax runs under the other's products. What
             // the products need is worked out before the wait for P.
@@ -387,13 +422,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                      (!b || outputs(kB, first, last, dv, width)) && (!xb || scores(kB, xfirst, xlast, dk, idesc));
                 if (!ok)
                     break;
-                if (a.key_mask)  // the step's weights are made, so its bounds have been read
-                    mma_commit(&h_empty[step % kHideSteps]);
-                mma_commit(&kv_empty[sv]);
-                if (more)
-                    mma_commit(&kv_empty[sk]);
+                if (elect_one_sync()) {
+                    if (a.key_mask)  // the step's weights are made, so its bounds have been read
+                        mma_commit(&h_empty[step % kHideSteps]);
+                    mma_commit(&kv_empty[sv]);
+                    if (more)
+                        mma_commit(&kv_empty[sk]);
+                }
+                __syncwarp();
             }
-            mma_commit(drain);  // arrives once every MMA issued above has completed
+            if (elect_one_sync())
+                mma_commit(drain);  // arrives once every MMA issued above has completed
+            __syncwarp();
             mbar_wait(drain, 0, a.status, kErrWaitDrain, nullptr);
         }
     } else if (warp == 2) {
@@ -430,15 +470,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
         const uint32_t lanes = tmem + (uint32_t(w32) << 16);
         const uint32_t ts = lanes + t * 128, to = lanes + 256 + t * 128;
         uint32_t ns = 0, no = 0, step = 0;  // S and O tiles taken; key steps of all items so far
-        Item it;
+        Items it;
         bool ok = true;
-        for (int item = blockIdx.x; item < P.items && ok; item += gridDim.x) {
-            it.set(P, item);
+        for (it.first(P); it.more(P) && ok; it.next(P)) {
             if (t >= it.tiles) {
                 step += it.steps;
                 continue;
             }
-            const int row0 = it.q0 + t * kTile + w32;  // of the warp
+            const int row0 = it.q0() + t * kTile + w32;  // of the warp
             if (it.steps == 0) {  // no keys: zeros, a row's 16-byte pieces side by side
                 constexpr int per = D / 8;
                 for (int i = lane; i < 32 * per; i += 32) {
@@ -457,11 +496,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 }
                 ++ns;
                 tc_fence_after();
-                if (j == 0 && no > 0 && lane == 0) {  // the last item's rows are out by now: its Q tile is free
-                    bulk_wait_read<0>();
-                    mbar_arrive(&q_empty[2 * t + ((no - 1) & 1)]);
-                }
-                __syncwarp();
                 const int valid = it.n - j * kTile;
                 int tail = valid >= kTile || valid % 32 == 0 ? 32 : valid % 32;
                 uint32_t masked = 0;
@@ -500,6 +534,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 }
                 tc_fence_before();
                 mbar_arrive(&p_full[t]);
+                if (j == 0 && no > 0 && lane == 0) {  // the last item's rows are out by now: its Q tile is free
+                    bulk_wait_read<0>();
+                    mbar_arrive(&q_empty[2 * t + ((no - 1) & 1)]);
+                }
+                __syncwarp();
             }
             if (!ok || !mbar_wait(&o_full[t], no & 1, a.status, kErrAttnWait, abort_flag))
                 break;

