@@ -470,9 +470,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
         const uint32_t lanes = tmem + (uint32_t(w32) << 16);
         const uint32_t ts = lanes + t * 128, to = lanes + 256 + t * 128;
         uint32_t ns = 0, no = 0, step = 0;  // S and O tiles taken; key steps of all items so far
-        Items it;
+        Items it, nx;  // this item and, worked out while its scores are on their way, the next
         bool ok = true;
-        for (it.first(P); it.more(P) && ok; it.next(P)) {
+        it.first(P);
+        for (; it.more(P) && ok; it = nx) {
+            nx = it;
+            nx.next(P);
             if (t >= it.tiles) {
                 step += it.steps;
                 continue;
