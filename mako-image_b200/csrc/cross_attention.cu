@@ -11,6 +11,8 @@
 //              hidden keys each thread also clears its row of V if that is one (0 * NaN would spread); the output rows are
 //              staged in the Q tile that made them and leave as TMA stores (a thread storing its row directly touches 32
 //              lines an instruction)
+// Where the items leave most of the GPU idle and the keys are many, SPLIT runs one item a cluster, whose CTAs take a run of
+// the key steps each and put the parts together through distributed shared memory: no workspace, no second launch.
 // Only ceil(visible / 16) * 16 keys of the last tile are multiplied and exponentiated (77 keys cost 80, not 128).
 // TMEM columns: S_A [0, 128), S_B [128, 256), O_A [256, 384), O_B [384, 512); P takes the first half of its S.
 #include "cross_attention.cuh"
@@ -48,6 +50,8 @@ struct Cfg {
     static constexpr int kSmem = 1024 + (4 + kSlots) * kTileBytes + 512 + kHideSteps * (kTile * 4 + 16);
     static_assert(kSmem <= 227 * 1024);
     static_assert((kSlots + 1) / 2 <= kSteps);
+    // SPLIT: two tiles' parts and (m, l) pairs for up to 8 CTAs (S * ceil(128 / S) <= 133 rows for S <= 8) fit the stages.
+    static_assert(2 * 133 * D * 4 + 2 * 8 * kTile * 8 <= (4 + kSlots) * kTileBytes);
 };
 
 struct CrossParams {
@@ -56,6 +60,7 @@ struct CrossParams {
     // 0 where a dimension is shared (stride 0): its coordinate stays 0.
     int q_head, q_sample, kv_head_k, kv_sample_k, kv_head_v, kv_sample_v, o_head, o_sample;
     int items, blocks;  // work items, query blocks of 256 rows
+    int splits;         // SPLIT: CTAs of a cluster
 };
 
 __device__ __forceinline__ float ex2(float x)
@@ -67,21 +72,29 @@ __device__ __forceinline__ float ex2(float x)
 
 // A CTA's items, gridDim.x apart: (sample, head, query block) and its keys. The digits of the item number are advanced by
 // the digits of the stride (a division for each item would sit in every role's way).
+template <bool SPLIT>
 struct Items {
     int item, b, h, blk, db, dh, dblk;
-    int n, steps, tiles;  // n: keys up to the last that may be visible; steps of 128 of them; 1 or 2 query tiles
+    // n: keys up to the last that may be visible; lo, hi: this CTA's steps of 128 of them; tiles: 1 or 2 query tiles
+    int n, lo, hi, tiles;
     __device__ __forceinline__ void keys(const CrossArgs& a)
     {
         n = a.key_len ? min(max(__ldg(a.key_len + min(b, a.B - 1)), 0), a.Lk) : a.Lk;
     }
     __device__ __forceinline__ void sizes(const CrossParams& P)
     {
-        steps = (n + kTile - 1) / kTile;
+        lo = 0;
+        hi = (n + kTile - 1) / kTile;
+        if constexpr (SPLIT) {
+            const int part = int(cluster_ctarank()), steps = hi;
+            lo = int(long(steps) * part / P.splits);
+            hi = int(long(steps) * (part + 1) / P.splits);
+        }
         tiles = blk * 2 * kTile + kTile < P.a.Lq ? 2 : 1;
     }
     __device__ __forceinline__ void first(const CrossParams& P)
     {
-        item = blockIdx.x;
+        item = SPLIT ? int(blockIdx.x) / P.splits : int(blockIdx.x);
         const int bh = item / P.blocks, dbh = int(gridDim.x) / P.blocks;
         blk = item - bh * P.blocks;
         b = bh / P.a.H;
@@ -94,6 +107,10 @@ struct Items {
     }
     __device__ __forceinline__ void next(const CrossParams& P)
     {
+        if constexpr (SPLIT) {
+            item = P.items;
+            return;
+        }
         const int was = b;
         item += gridDim.x;
         blk += dblk;
@@ -116,14 +133,15 @@ struct Items {
 };
 
 // The walk over all key steps of a CTA's items that have keys.
+template <bool SPLIT>
 struct Walk {
-    Items it;
+    Items<SPLIT> it;
     int j;
     __device__ __forceinline__ void settle(const CrossParams& P)  // on to an item with keys
     {
-        j = 0;
-        while (it.more(P) && it.steps == 0)
+        while (it.more(P) && it.lo == it.hi)
             it.next(P);
+        j = it.lo;
     }
     __device__ __forceinline__ void first(const CrossParams& P)
     {
@@ -132,13 +150,14 @@ struct Walk {
     }
     __device__ __forceinline__ void next(const CrossParams& P)
     {
-        if (++j == it.steps) {
+        if (++j == it.hi) {
             it.next(P);
             settle(P);
         }
     }
     __device__ __forceinline__ bool more(const CrossParams& P) const { return it.more(P); }
-    __device__ __forceinline__ bool last() const { return j + 1 == it.steps; }
+    __device__ __forceinline__ bool start() const { return j == it.lo; }
+    __device__ __forceinline__ bool last() const { return j + 1 == it.hi; }
     // Keys of the step that are multiplied: those up to n, in sixteens.
     __device__ __forceinline__ int width() const { return min(kTile, (it.n - j * kTile + 15) & ~15); }
 };
@@ -225,7 +244,20 @@ __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int tail,
     l += l2.x + l2.y;
 }
 
-template <int D>
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v)
+{
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+__device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, float4 v)
+{
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
+                 : "memory");
+}
+
+constexpr int kMaxSplits = 8;
+
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ CrossParams P)
 {
     using C = Cfg<D>;
@@ -237,6 +269,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
     float* bounds = reinterpret_cast<float*>(smem + (4 + NS) * TB);  // [kHideSteps][kTile]
     volatile uint32_t* maskeds = reinterpret_cast<volatile uint32_t*>(bounds + kHideSteps * kTile);
     uint64_t* bars = reinterpret_cast<uint64_t*>(bounds + kHideSteps * (kTile + 4));
+    // SPLIT: the rows' parts overlay the stages, this CTA's own result of a row stays in its softmax thread until then.
+    float part_m = -INFINITY, part_l = 0.0f;
+    bool part_here = false, part_any = false;
     uint64_t* q_full = bars;             // [2 tiles][2 buffers]
     uint64_t* q_empty = q_full + 4;      // [2 tiles][2 buffers]
     uint64_t* kv_empty = q_empty + 4;    // [NS]
@@ -300,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
         regs_decrease<kRegsCtl>();
     if (warp == 0) {
         if (lane == 0) {
-            Walk w;
+            Walk<SPLIT> w;
             uint32_t seq = 0, nq0 = 0, nq1 = 0;  // K and V tiles, Q tiles of A and of B loaded
             bool ok = true;
             const auto load = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int row, int h, int b) {
@@ -311,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             };
             for (w.first(P); w.more(P) && ok; w.next(P)) {
                 const int hk = w.it.h / (a.H / a.Hkv);
-                for (int t = 0; w.j == 0 && t < w.it.tiles && ok; ++t) {
+                for (int t = 0; w.start() && t < w.it.tiles && ok; ++t) {
                     const uint32_t n = t ? nq1++ : nq0++, i = 2 * t + (n & 1);
                     ok = mbar_wait(&q_empty[i], ((n >> 1) & 1) ^ 1, a.status, kErrAttnWait, abort_flag);
                     if (ok)
@@ -395,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 __syncwarp();
                 return true;
             };
-            Walk w, x;
+            Walk<SPLIT> w, x;
             w.first(P);
             if (w.more(P)) {
                 const uint32_t idesc = idesc_s0 | uint32_t(w.width() >> 3) << 17;
@@ -410,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             for (; w.more(P) && ok; w = x, ++step) {
                 x = w;
                 x.next(P);
-                const bool more = x.more(P), first = w.j == 0, last = w.last(), xfirst = x.j == 0, xlast = x.last();
+                const bool more = x.more(P), first = w.start(), last = w.last(), xfirst = x.start(), xlast = x.last();
                 const bool b = w.it.tiles > 1, xb = more && x.it.tiles > 1;
                 const int width = w.width();
                 const uint32_t sv = (2 * step + 1) % NS, sk = (2 * step + 2) % NS;
@@ -438,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
         }
     } else if (warp == 2) {
         if (a.key_mask) {
-            Walk w;
+            Walk<SPLIT> w;
             uint32_t step = 0;
             for (w.first(P); w.more(P); w.next(P), ++step) {
                 const uint32_t hs = step % kHideSteps;
@@ -470,18 +505,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
         const uint32_t lanes = tmem + (uint32_t(w32) << 16);
         const uint32_t ts = lanes + t * 128, to = lanes + 256 + t * 128;
         uint32_t ns = 0, no = 0, step = 0;  // S and O tiles taken; key steps of all items so far
-        Items it, nx;  // this item and, worked out while its scores are on their way, the next
+        Items<SPLIT> it, nx;  // this item and, worked out while its scores are on their way, the next
         bool ok = true;
         it.first(P);
         for (; it.more(P) && ok; it = nx) {
             nx = it;
             nx.next(P);
             if (t >= it.tiles) {
-                step += it.steps;
+                step += it.hi - it.lo;
                 continue;
             }
             const int row0 = it.q0() + t * kTile + w32;  // of the warp
-            if (it.steps == 0) {  // no keys: zeros, a row's 16-byte pieces side by side
+            if (it.n == 0) {  // no keys: zeros, a row's 16-byte pieces side by side
                 constexpr int per = D / 8;
                 for (int i = lane; i < 32 * per; i += 32) {
                     const long row = row0 + i / per;
@@ -492,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 continue;
             }
             float m = -INFINITY, l = 0.0f;
-            for (int j = 0; j < it.steps; ++j, ++step) {
+            for (int j = it.lo; j < it.hi; ++j, ++step) {
                 if (!mbar_wait(&s_full[t], ns & 1, a.status, kErrAttnWait, abort_flag)) {
                     ok = false;
                     break;
@@ -513,10 +548,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                     tail = 32;  // the bounds know of it
                 }
                 switch (min(4, (valid + 31) >> 5)) {
-                case 1: softmax_step<D, 1>(ts, to, tail, masked, bound, a.scale_log2, j == 0, m, l); break;
-                case 2: softmax_step<D, 2>(ts, to, tail, masked, bound, a.scale_log2, j == 0, m, l); break;
-                case 3: softmax_step<D, 3>(ts, to, tail, masked, bound, a.scale_log2, j == 0, m, l); break;
-                default: softmax_step<D, 4>(ts, to, tail, masked, bound, a.scale_log2, j == 0, m, l); break;
+                case 1: softmax_step<D, 1>(ts, to, tail, masked, bound, a.scale_log2, j == it.lo, m, l); break;
+                case 2: softmax_step<D, 2>(ts, to, tail, masked, bound, a.scale_log2, j == it.lo, m, l); break;
+                case 3: softmax_step<D, 3>(ts, to, tail, masked, bound, a.scale_log2, j == it.lo, m, l); break;
+                default: softmax_step<D, 4>(ts, to, tail, masked, bound, a.scale_log2, j == it.lo, m, l); break;
                 }
                 if (masked || (valid < kTile && it.n < a.Lk)) {
                     // Rows of V that are multiplied (those up to valid, in sixteens) and belong to hidden keys: both tiles'
@@ -537,15 +572,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 }
                 tc_fence_before();
                 mbar_arrive(&p_full[t]);
-                if (j == 0 && no > 0 && lane == 0) {  // the last item's rows are out by now: its Q tile is free
+                if (j == it.lo && no > 0 && lane == 0) {  // the last item's rows are out by now: its Q tile is free
                     bulk_wait_read<0>();
                     mbar_arrive(&q_empty[2 * t + ((no - 1) & 1)]);
                 }
                 __syncwarp();
             }
-            if (!ok || !mbar_wait(&o_full[t], no & 1, a.status, kErrAttnWait, abort_flag))
+            if (!ok || (it.lo < it.hi && !mbar_wait(&o_full[t], no & 1, a.status, kErrAttnWait, abort_flag))) {
+                ok = false;
                 break;
+            }
             tc_fence_after();
+            if constexpr (SPLIT) {  // merged below
+                part_m = m;
+                part_l = l;
+                part_here = true;
+                part_any = it.lo < it.hi;
+                break;
+            }
             // The item's scores are all made, so its Q tile takes the output rows on their way out.
             uint8_t* stage = sQ + (2 * t + (no & 1)) * TB;
             ++no;
@@ -579,6 +623,82 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
         }
         if (lane == 0)
             bulk_wait_all();  // the last rows are written before the CTA and its shared memory go
+    }
+
+    if constexpr (SPLIT) {
+        // Each CTA holds, for every row, its part's maximum m, sum l and O. With M the largest m, the row's result is
+        // sum O 2^(m - M) / sum l 2^(m - M). The tiles' valid rows are dealt out over the CTAs; every CTA sends its scaled
+        // rows to their owners, and those add and write them. The stages' memory takes the parts: all products that read it
+        // are done (o_full) before the first cluster barrier.
+        const int S = P.splits, me = int(cluster_ctarank());
+        const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
+        Items<true> it;
+        it.first(P);
+        const int rows = min(kTile, a.Lq - it.q0() - max(t, 0) * kTile);  // of tile t
+        const int per = (kTile + S - 1) / S;                               // owned rows at most
+        float* parts = reinterpret_cast<float*>(smem) + max(t, 0) * (S * per * D);  // [S][per][D]
+        float* ml = reinterpret_cast<float*>(smem) + 2 * (S * per * D);    // [tiles][S][kTile][2]
+        __syncwarp();
+        __syncthreads();
+        cluster_sync_all();
+        if (part_here && r < rows)
+            for (int o = 0; o < S; ++o) {
+                const uint32_t at = map_to_cta(smem_u32(ml + ((t * S + me) * kTile + r) * 2), o);
+                st_cluster_f32(at, part_m);
+                st_cluster_f32(at + 4, part_l);
+            }
+        cluster_sync_all();
+        if (part_here && __any_sync(0xffffffffu, r < rows)) {
+            float M = -INFINITY, L = 0.0f;
+            for (int o = 0; o < S && r < rows; ++o)
+                M = fmaxf(M, ml[((t * S + o) * kTile + r) * 2]);
+            const auto weight = [&](float m) { return m == -INFINITY ? 0.0f : ex2(m - M); };
+            for (int o = 0; o < S && r < rows; ++o) {
+                const float* e = ml + ((t * S + o) * kTile + r) * 2;
+                L += e[1] * weight(e[0]);
+            }
+            // A part without a visible key adds nothing (its O may never have been written); NaN parts stay NaN.
+            const bool add = part_any && !(part_m == -INFINITY && part_l == 0.0f);
+            const float f = weight(part_m) * (L == 0.0f ? 0.0f : 1.0f / L);
+            int owner = 0;  // of row r: rows * owner / S <= r < rows * (owner + 1) / S
+            while (owner + 1 < S && rows * (owner + 1) / S <= r)
+                ++owner;
+            const int lr = r - rows * owner / S;
+            const uint32_t dst = map_to_cta(smem_u32(parts + (me * per + lr) * D), owner);
+            const uint32_t to = tmem + (uint32_t((warp & 3) * 32) << 16) + 256 + t * 128;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t v[32];
+                tmem_ld32(to + c, v);
+                tmem_wait_ld();
+                if (r < rows) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        st_cluster_f32x4(dst + (c + i) * 4,
+                                         add ? make_float4(__uint_as_float(v[i]) * f, __uint_as_float(v[i + 1]) * f,
+                                                           __uint_as_float(v[i + 2]) * f, __uint_as_float(v[i + 3]) * f)
+                                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();
+        if (part_here) {
+            const int first = rows * me / S, count = rows * (me + 1) / S - first;
+            __nv_bfloat16* out = a.out + it.b * a.so.sample + it.h * a.so.head;
+            for (int i = r; i < count * (D / 8); i += kTile) {
+                const int lr = i / (D / 8), c = i % (D / 8) * 8;
+                float4 x = make_float4(0, 0, 0, 0), y = x;
+                for (int o = 0; o < S; ++o) {
+                    const float4* e = reinterpret_cast<const float4*>(parts + (o * per + lr) * D + c);
+                    const float4 u = e[0], v = e[1];
+                    x = make_float4(x.x + u.x, x.y + u.y, x.z + u.z, x.w + u.w);
+                    y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
+                }
+                *reinterpret_cast<uint4*>(out + long(it.q0() + t * kTile + first + lr) * a.so.row + c) =
+                    make_uint4(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w), pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+            }
+        }
     }
 
     tc_fence_before();
@@ -626,12 +746,12 @@ bool encode_heads(CUtensorMap* m, const void* p, const HeadStrides& s, int rows,
 
 // A one-time check that the compiled register count holds the warpgroups' split (otherwise the softmax groups' increase
 // could never be granted), and the shared memory limit on each device.
-template <int D>
+template <int D, bool SPLIT>
 cudaError_t setup()
 {
     static const cudaError_t regs = [] {
         cudaFuncAttributes fa{};
-        const cudaError_t e = cudaFuncGetAttributes(&fa, k_cross<D>);
+        const cudaError_t e = cudaFuncGetAttributes(&fa, k_cross<D, SPLIT>);
         if (e != cudaSuccess)
             return e;
         return fa.numRegs * kThreads < 128 * kRegsCtl + 256 * kRegsSoftmax ? cudaErrorInvalidConfiguration
@@ -640,16 +760,22 @@ cudaError_t setup()
     if (regs != cudaSuccess)
         return regs;
     static std::atomic<uint64_t> devs{0};
-    return smem_limit_once(devs, k_cross<D>, Cfg<D>::kSmem);
+    return smem_limit_once(devs, k_cross<D, SPLIT>, Cfg<D>::kSmem);
 }
 
 template <int D>
 cudaError_t launch(const CrossParams& P, cudaStream_t st)
 {
-    const cudaError_t e = setup<D>();
-    if (e != cudaSuccess)
-        return e;
-    return launch_k(k_cross<D>, dim3(std::min(P.items, num_sms())), kThreads, Cfg<D>::kSmem, st, P);
+    if (P.splits > 1) {
+        const cudaError_t e = setup<D, true>();
+        return e != cudaSuccess ? e
+                                : launch_k_cluster(k_cross<D, true>, dim3(P.items * P.splits), P.splits, kThreads,
+                                                   Cfg<D>::kSmem, st, P);
+    }
+    const cudaError_t e = setup<D, false>();
+    return e != cudaSuccess
+               ? e
+               : launch_k(k_cross<D, false>, dim3(std::min(P.items, num_sms())), kThreads, Cfg<D>::kSmem, st, P);
 }
 
 }  // namespace
@@ -660,6 +786,8 @@ cudaError_t cross_attention(const CrossArgs& a, const char** err, cudaStream_t s
     P.a = a;
     P.blocks = (a.Lq + 2 * kTile - 1) / (2 * kTile);
     P.items = a.B * a.H * P.blocks;
+    // Clusters where at least two CTAs an item fit the GPU at once and each gets two key steps or more.
+    P.splits = std::max(1, std::min({kMaxSplits, num_sms() / P.items, (a.Lk + kTile - 1) / kTile / 2}));
     const void* k = a.Lk ? a.k : a.q;  // no keys: the maps are not used
     const void* v = a.Lk ? a.v : a.q;
     if (!encode_heads(&P.tq, a.q, a.sq, a.Lq, a.H, a.B, a.d, kTile, &P.q_head, &P.q_sample) ||
