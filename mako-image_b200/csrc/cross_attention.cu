@@ -1,6 +1,7 @@
-// Attention to another stream's keys (see cross_attention.cuh) on tcgen05.
+// Attention to another stream's keys (see cross_attention.cuh): k_cross on tcgen05, and for a handful of query rows
+// k_cross_few on the CUDA cores.
 //
-// Keys are few and queries many, so the work is a stream of query tiles past small sets of keys: persistent CTAs walk
+// k_cross: keys are few and queries many, so the work is a stream of query tiles past small sets of keys: persistent CTAs walk
 // items of (sample, head, 256 query rows) as two 128-row tiles A and B, and every stage runs ahead into the next item, so
 // that one item's loads, another's products and a third's stores overlap. Twelve warps:
 //   warp 0     TMA: Q tiles (two buffers for each of A and B), K and V tiles of 128 keys in one ring
@@ -39,19 +40,20 @@ constexpr int kRegsCtl = 88, kRegsSoftmax = 208;
 static_assert(128 * kRegsCtl + 256 * kRegsSoftmax <= kThreads * kLaunchRegs, "register split exceeds the CTA pool");
 constexpr int kTile = 128;              // query rows a tile, keys a tile
 constexpr int kPanel = kTile * 64 * 2;  // 64 bf16 columns of 128 rows
-constexpr int kSteps = 4;               // full barriers of K and of V: no more key steps than that are ever in flight
+constexpr int kSteps = 5;               // full barriers of K and of V: no more key steps than that are ever in flight
 constexpr int kHideSteps = 2;           // key steps whose hidden keys are kept ready
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: O is rescaled only when a row's maximum grows by more
 
-template <int D>
+template <int D, bool SPLIT>
 struct Cfg {
     static constexpr int kTileBytes = (D / 64) * kPanel;
-    static constexpr int kSlots = D == 64 ? 8 : 3;  // K and V tiles beside the four Q tiles
-    static constexpr int kSmem = 1024 + (4 + kSlots) * kTileBytes + 512 + kHideSteps * (kTile * 4 + 16);
+    static constexpr int kQ = SPLIT ? 1 : 2;  // Q buffers of each tile: with a single item nothing is fetched ahead
+    static constexpr int kSlots = D == 64 ? (SPLIT ? 10 : 8) : (SPLIT ? 5 : 3);  // K and V tiles
+    static constexpr int kSmem = 1024 + (2 * kQ + kSlots) * kTileBytes + 512 + kHideSteps * (kTile * 4 + 16);
     static_assert(kSmem <= 227 * 1024);
     static_assert((kSlots + 1) / 2 <= kSteps);
     // SPLIT: two tiles' parts and (m, l) pairs for up to 8 CTAs (S * ceil(128 / S) <= 133 rows for S <= 8) fit the stages.
-    static_assert(2 * 133 * D * 4 + 2 * 8 * kTile * 8 <= (4 + kSlots) * kTileBytes);
+    static_assert(2 * 133 * D * 4 + 2 * 8 * kTile * 8 <= (2 * kQ + kSlots) * kTileBytes);
 };
 
 struct CrossParams {
@@ -260,20 +262,21 @@ constexpr int kMaxSplits = 8;
 template <int D, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ CrossParams P)
 {
-    using C = Cfg<D>;
+    using C = Cfg<D, SPLIT>;
     constexpr int TB = C::kTileBytes, NS = C::kSlots;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* sQ = smem;            // [2 tiles][2 buffers]
-    uint8_t* sKV = smem + 4 * TB;  // [NS]
-    float* bounds = reinterpret_cast<float*>(smem + (4 + NS) * TB);  // [kHideSteps][kTile]
+    constexpr uint32_t QB = C::kQ;
+    uint8_t* sQ = smem;                 // [2 tiles][QB]
+    uint8_t* sKV = smem + 2 * QB * TB;  // [NS]
+    float* bounds = reinterpret_cast<float*>(smem + (2 * QB + NS) * TB);  // [kHideSteps][kTile]
     volatile uint32_t* maskeds = reinterpret_cast<volatile uint32_t*>(bounds + kHideSteps * kTile);
     uint64_t* bars = reinterpret_cast<uint64_t*>(bounds + kHideSteps * (kTile + 4));
     // SPLIT: the rows' parts overlay the stages, this CTA's own result of a row stays in its softmax thread until then.
     float part_m = -INFINITY, part_l = 0.0f;
     bool part_here = false, part_any = false;
-    uint64_t* q_full = bars;             // [2 tiles][2 buffers]
-    uint64_t* q_empty = q_full + 4;      // [2 tiles][2 buffers]
+    uint64_t* q_full = bars;             // [2 tiles][QB]
+    uint64_t* q_empty = q_full + 4;      // [2 tiles][QB]
     uint64_t* kv_empty = q_empty + 4;    // [NS]
     // By key step, not by slot: where K and V take turns in a slot, threads that follow only the V tiles would miss phases
     // of the slot's barrier.
@@ -347,8 +350,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             for (w.first(P); w.more(P) && ok; w.next(P)) {
                 const int hk = w.it.h / (a.H / a.Hkv);
                 for (int t = 0; w.start() && t < w.it.tiles && ok; ++t) {
-                    const uint32_t n = t ? nq1++ : nq0++, i = 2 * t + (n & 1);
-                    ok = mbar_wait(&q_empty[i], ((n >> 1) & 1) ^ 1, a.status, kErrAttnWait, abort_flag);
+                    const uint32_t n = t ? nq1++ : nq0++, i = QB * t + n % QB;
+                    ok = mbar_wait(&q_empty[i], ((n / QB) & 1) ^ 1, a.status, kErrAttnWait, abort_flag);
                     if (ok)
                         load(sQ + i * TB, &P.tq, &q_full[i], w.it.q0() + t * kTile, w.it.h * P.q_head, w.it.b * P.q_sample);
                     else
@@ -370,8 +373,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             if (!ok) {  // let the loads already issued land before the CTA can exit
                 for (int t = 0; t < 2; ++t) {
                     const uint32_t n = t ? nq1 : nq0;
-                    for (uint32_t i = n > 2 ? n - 2 : 0; i < n; ++i)
-                        mbar_wait(&q_full[2 * t + (i & 1)], (i >> 1) & 1, a.status, kErrWaitDrain, nullptr);
+                    for (uint32_t i = n > QB ? n - QB : 0; i < n; ++i)
+                        mbar_wait(&q_full[QB * t + i % QB], (i / QB) & 1, a.status, kErrWaitDrain, nullptr);
                 }
                 for (uint32_t i = seq > NS ? seq - NS : 0; i < seq; ++i)
                     mbar_wait(&(i & 1 ? v_full : k_full)[(i >> 1) % kSteps], ((i >> 1) / kSteps) & 1, a.status,
@@ -395,8 +398,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             // S_t = Q_t K^T; Q is waited for at an item's first step.
             const auto scores = [&](auto tile, bool first, bool last, uint64_t dk, uint32_t idesc) {
                 constexpr int t = decltype(tile)::value;
-                const uint64_t dq = dq0 + (2 * t + (nq[t] & 1)) * kUnit;
-                if (first && !wait(&q_full[2 * t + (nq[t] & 1)], nq[t] >> 1))
+                const uint32_t qi = QB * t + nq[t] % QB;
+                const uint64_t dq = dq0 + qi * kUnit;
+                if (first && !wait(&q_full[qi], nq[t] / QB))
                     return false;
                 tc_fence_after();
                 if (elect_one_sync()) {
@@ -574,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 mbar_arrive(&p_full[t]);
                 if (j == it.lo && no > 0 && lane == 0) {  // the last item's rows are out by now: its Q tile is free
                     bulk_wait_read<0>();
-                    mbar_arrive(&q_empty[2 * t + ((no - 1) & 1)]);
+                    mbar_arrive(&q_empty[QB * t + (no - 1) % QB]);
                 }
                 __syncwarp();
             }
@@ -591,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 break;
             }
             // The item's scores are all made, so its Q tile takes the output rows on their way out.
-            uint8_t* stage = sQ + (2 * t + (no & 1)) * TB;
+            uint8_t* stage = sQ + (QB * t + no % QB) * TB;
             ++no;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
@@ -709,6 +713,204 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
     }
 }
 
+// ------------------------------------------------------------------------------------------------ few query rows
+
+constexpr int kFewRows = 8;    // query rows that share a key head
+constexpr int kFewWarps = 8;
+constexpr int kFewDepth = 4;   // K and V rows a lane has in flight, each
+
+__device__ __forceinline__ void unpack8(uint4 u, float (&f)[8])
+{
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
+// A few query rows of the heads that share a key head: with so few, K and V pass the CUDA cores once and HBM is the bound. A
+// cluster takes one (sample, key head), each CTA a run of its keys; D / 8 lanes take a key, 8 values each, so that a warp's
+// load is whole rows. Each warp keeps its own running maximum, sum and outputs; the warps' parts meet in shared memory, the
+// CTAs' in the first CTA's.
+template <int D, int R>
+__global__ void __launch_bounds__(32 * kFewWarps) k_cross_few(const CrossArgs a, int splits)
+{
+    constexpr int kLanes = D / 8, kKeys = 32 / kLanes;  // lanes a key, keys a load
+    __shared__ float po[kFewWarps][R][D];
+    __shared__ float pm[kFewWarps][R], pl[kFewWarps][R];
+    grid_dep_wait();
+    grid_dep_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int part = splits > 1 ? int(cluster_ctarank()) : 0, pair = blockIdx.x / splits;
+    const int b = pair / a.Hkv, hk = pair % a.Hkv, group = a.H / a.Hkv, rows = group * a.Lq;
+    const int n = a.key_len ? min(max(__ldg(a.key_len + b), 0), a.Lk) : a.Lk;
+    const int lo = int(long(n) * part / splits), hi = int(long(n) * (part + 1) / splits);
+    const int dim = lane % kLanes * 8;  // of this lane
+    const auto head = [&](int r) { return hk * group + r / a.Lq; };
+
+    float q[R][8], o[R][8] = {}, m[R], l[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.0f;
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (r < rows)
+            u = __ldg(reinterpret_cast<const uint4*>(a.q + b * a.sq.sample + head(r) * a.sq.head + r % a.Lq * a.sq.row + dim));
+        unpack8(u, q[r]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            q[r][i] *= a.scale_log2;
+    }
+    const __nv_bfloat16* kb = a.k + b * a.sk.sample + hk * a.sk.head + dim;
+    const __nv_bfloat16* vb = a.v + b * a.sv.sample + hk * a.sv.head + dim;
+    const uint8_t* mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
+    for (int j0 = lo + warp * kKeys; j0 < hi; j0 += kFewWarps * kKeys * kFewDepth) {
+        uint4 ku[kFewDepth], vu[kFewDepth];
+        bool see[kFewDepth];
+#pragma unroll
+        for (int u = 0; u < kFewDepth; ++u) {
+            const int j = j0 + u * kFewWarps * kKeys + lane / kLanes;
+            see[u] = j < hi && (!mask || __ldg(mask + j) != 0);
+            ku[u] = vu[u] = make_uint4(0, 0, 0, 0);  // a hidden key is not read
+            if (see[u]) {
+                ku[u] = __ldg(reinterpret_cast<const uint4*>(kb + j * a.sk.row));
+                vu[u] = __ldg(reinterpret_cast<const uint4*>(vb + j * a.sv.row));
+            }
+        }
+        float s[kFewDepth][R];
+#pragma unroll
+        for (int u = 0; u < kFewDepth; ++u) {
+            float k[8];
+            unpack8(ku[u], k);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float x = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    x = fmaf(q[r][i], k[i], x);
+                s[u][r] = x;
+            }
+        }
+#pragma unroll
+        for (int w = kLanes / 2; w > 0; w >>= 1)
+#pragma unroll
+            for (int u = 0; u < kFewDepth; ++u)
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                    s[u][r] += __shfl_xor_sync(0xffffffffu, s[u][r], w);
+        float shift[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float top = m[r];
+#pragma unroll
+            for (int u = 0; u < kFewDepth; ++u) {
+                if (!see[u])
+                    s[u][r] = -INFINITY;
+                top = fmaxf(top, s[u][r]);
+            }
+#pragma unroll
+            for (int w = 16; w >= kLanes; w >>= 1)
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            const float f = m[r] == -INFINITY ? 0.0f : ex2(m[r] - top);
+            m[r] = top;
+            shift[r] = top == -INFINITY ? 0.0f : top;  // no visible key yet: 2^(-inf - 0) = 0
+            l[r] *= f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                o[r][i] *= f;
+        }
+#pragma unroll
+        for (int u = 0; u < kFewDepth; ++u) {
+            float v[8];
+            unpack8(vu[u], v);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float p = ex2(s[u][r] - shift[r]);
+                l[r] += p;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    o[r][i] = fmaf(p, v[i], o[r][i]);
+            }
+        }
+    }
+    // Sum over the keys that the warp's lane groups took; every lane of a group has the same l.
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int w = 16; w >= kLanes; w >>= 1) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                o[r][i] += __shfl_xor_sync(0xffffffffu, o[r][i], w);
+        }
+        if (lane < kLanes) {
+#pragma unroll
+            for (int i = 0; i < 8; i += 4)
+                *reinterpret_cast<float4*>(&po[warp][r][dim + i]) = make_float4(o[r][i], o[r][i + 1], o[r][i + 2], o[r][i + 3]);
+        }
+        if (lane == 0) {
+            pm[warp][r] = m[r];
+            pl[warp][r] = l[r];
+        }
+    }
+    __syncthreads();
+    // The parts of `count` warps or CTAs to one: element e of R * D, with the row's maximum and sum.
+    const auto join = [&](int count, int e, float& M, float& L) {
+        const int r = e / D;
+        M = -INFINITY;
+        for (int w = 0; w < count; ++w)
+            M = fmaxf(M, pm[w][r]);
+        float x = 0.0f;
+        L = 0.0f;
+        for (int w = 0; w < count; ++w) {
+            const float f = pm[w][r] == -INFINITY ? 0.0f : ex2(pm[w][r] - M);
+            L = fmaf(pl[w][r], f, L);
+            x = fmaf(po[w][r][e % D], f, x);
+        }
+        return x;
+    };
+    constexpr int kPer = (R * D + 32 * kFewWarps - 1) / (32 * kFewWarps);
+    float x[kPer], M[kPer], L[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int e = threadIdx.x + i * 32 * kFewWarps;
+        if (e < R * D)
+            x[i] = join(kFewWarps, e, M[i], L[i]);
+    }
+    if (splits > 1) {
+        __syncthreads();
+        cluster_sync_all();  // every CTA has read its warps' parts
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int e = threadIdx.x + i * 32 * kFewWarps;
+            if (e < R * D) {
+                st_cluster_f32(map_to_cta(smem_u32(&po[part][e / D][e % D]), 0), x[i]);
+                if (e % D == 0) {
+                    st_cluster_f32(map_to_cta(smem_u32(&pm[part][e / D]), 0), M[i]);
+                    st_cluster_f32(map_to_cta(smem_u32(&pl[part][e / D]), 0), L[i]);
+                }
+            }
+        }
+        cluster_sync_all();
+        if (part)
+            return;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int e = threadIdx.x + i * 32 * kFewWarps;
+            if (e < R * D)
+                x[i] = join(splits, e, M[i], L[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int e = threadIdx.x + i * 32 * kFewWarps, r = e / D;
+        if (e < R * D && r < rows)
+            a.out[b * a.so.sample + head(r) * a.so.head + r % a.Lq * a.so.row + e % D] =
+                __float2bfloat16(x[i] * (L[i] == 0.0f ? 0.0f : 1.0f / L[i]));
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ host
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
@@ -760,7 +962,7 @@ cudaError_t setup()
     if (regs != cudaSuccess)
         return regs;
     static std::atomic<uint64_t> devs{0};
-    return smem_limit_once(devs, k_cross<D, SPLIT>, Cfg<D>::kSmem);
+    return smem_limit_once(devs, k_cross<D, SPLIT>, Cfg<D, SPLIT>::kSmem);
 }
 
 template <int D>
@@ -770,18 +972,44 @@ cudaError_t launch(const CrossParams& P, cudaStream_t st)
         const cudaError_t e = setup<D, true>();
         return e != cudaSuccess ? e
                                 : launch_k_cluster(k_cross<D, true>, dim3(P.items * P.splits), P.splits, kThreads,
-                                                   Cfg<D>::kSmem, st, P);
+                                                   Cfg<D, true>::kSmem, st, P);
     }
     const cudaError_t e = setup<D, false>();
     return e != cudaSuccess
                ? e
-               : launch_k(k_cross<D, false>, dim3(std::min(P.items, num_sms())), kThreads, Cfg<D>::kSmem, st, P);
+               : launch_k(k_cross<D, false>, dim3(std::min(P.items, num_sms())), kThreads, Cfg<D, false>::kSmem, st, P);
+}
+
+template <int D, int R>
+cudaError_t launch_few(const CrossArgs& a, cudaStream_t st)
+{
+    // Keys over as many CTAs as keep four on each SM, 128 keys each or more.
+    const int pairs = a.B * a.Hkv;
+    const int splits = std::max(1, std::min({kMaxSplits, kFewWarps, 4 * num_sms() / pairs, a.Lk / 128}));
+    return launch_k_cluster(k_cross_few<D, R>, dim3(pairs * splits), splits, 32 * kFewWarps, 0, st, a, splits);
+}
+
+template <int D>
+cudaError_t launch_few(const CrossArgs& a, cudaStream_t st)
+{
+    const int rows = a.H / a.Hkv * a.Lq;
+    return rows == 1   ? launch_few<D, 1>(a, st)
+           : rows == 2 ? launch_few<D, 2>(a, st)
+           : rows <= 4 ? launch_few<D, 4>(a, st)
+                       : launch_few<D, 8>(a, st);
 }
 
 }  // namespace
 
 cudaError_t cross_attention(const CrossArgs& a, const char** err, cudaStream_t st)
 {
+    if (long(a.H / a.Hkv) * a.Lq <= kFewRows) {
+        const cudaError_t e = a.d == 64 ? launch_few<64>(a, st) : launch_few<128>(a, st);
+        if (e != cudaSuccess)
+            return e;
+        count_launch();
+        return cudaGetLastError();
+    }
     CrossParams P;
     P.a = a;
     P.blocks = (a.Lq + 2 * kTile - 1) / (2 * kTile);
