@@ -309,28 +309,34 @@ __global__ void __launch_bounds__(192, 1) k_i8_split(const __grid_constant__ I8P
                     mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1, a.status, kErrWaitDrain, nullptr);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_i8_s32(128, BN);
-            int it = 0;
-            for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
-                const int s = it % C::kStages;
-                if (!mbar_wait(&full[s], (it / C::kStages) & 1, a.status, kErrWaitFull, abort_flag)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t aa = smem_u32(smem + s * C::kStageBytes), bb = aa + C::kABytes;
+        // The whole warp walks and waits, so that descriptors stay in uniform registers; one lane issues.
+        constexpr uint32_t idesc = idesc_i8_s32(128, BN);
+        int it = 0;
+        for (int kb = k_lo; kb < k_hi; ++kb, ++it) {
+            const int s = it % C::kStages;
+            if (!__all_sync(0xffffffffu,
+                            mbar_wait(&full[s], (it / C::kStages) & 1, a.status, kErrWaitFull, abort_flag))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint64_t da = desc_kmajor_sw128(smem_u32(smem + s * C::kStageBytes)),
+                           db = desc_kmajor_sw128(smem_u32(smem + s * C::kStageBytes + C::kABytes));
+            if (elect_one_sync()) {
 #pragma unroll
-                for (int k = 0; k < kBK / 32; ++k)
-                    mma_i8_ss(tmem, desc_kmajor_sw128(aa + k * 32), desc_kmajor_sw128(bb + k * 32), idesc,
-                              (it | k) != 0);
+                for (int k = 0; k < kBK / 32; ++k)  // 32 bytes are 2 units of a descriptor's address
+                    mma_i8_ss(tmem, da + 2 * k, db + 2 * k, idesc, (it | k) != 0);
                 mma_commit(&empty[s]);
             }
+            __syncwarp();
+        }
+        if (elect_one_sync()) {
             if (ok)
                 mma_commit(acc_full);
             mma_commit(drain);
-            mbar_wait(drain, 0, a.status, kErrWaitDrain, nullptr);
         }
+        __syncwarp();
+        mbar_wait(drain, 0, a.status, kErrWaitDrain, nullptr);
     } else {
         ok = mbar_wait(acc_full, 0, a.status, kErrWaitAccFull, abort_flag);
         tc_fence_after();
@@ -490,33 +496,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(co
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && leader) {
+        // The leader's whole warp walks and waits, so that descriptors stay in uniform registers; one lane issues.
+        if (leader) {
             constexpr uint32_t idesc = idesc_i8_s32(256, BN);
             uint32_t it = 0, lt = 0;
             bool ok = true;
             for (int tile = pair; tile < num_tiles && ok; tile += npairs, ++lt) {
                 const uint32_t acc = lt & 1, acc_ph = (lt >> 1) & 1;
-                if (!mbar_wait(&acc_empty[acc], acc_ph ^ 1, a.status, kErrWaitAccEmpty, abort_flag))
+                if (!__all_sync(0xffffffffu,
+                                mbar_wait(&acc_empty[acc], acc_ph ^ 1, a.status, kErrWaitAccEmpty, abort_flag)))
                     break;
                 tc_fence_after();
                 for (int kb = 0; kb < num_k; ++kb, ++it) {
                     const int s = it % C::kStages;
-                    if (!mbar_wait(&full[s], (it / C::kStages) & 1, a.status, kErrWaitFull, abort_flag)) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (it / C::kStages) & 1, a.status, kErrWaitFull,
+                                                           abort_flag))) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t aa = smem_u32(smem + s * C::kStageBytes), bb = aa + C::kABytes;
+                    const uint64_t da = desc_kmajor_sw128(smem_u32(smem + s * C::kStageBytes)),
+                                   db = desc_kmajor_sw128(smem_u32(smem + s * C::kStageBytes + C::kABytes));
+                    if (elect_one_sync()) {
 #pragma unroll
-                    for (int k = 0; k < kBK / 32; ++k)
-                        mma_i8_ss_pair(tmem + acc * BN, desc_kmajor_sw128(aa + k * 32), desc_kmajor_sw128(bb + k * 32),
-                                       idesc, (kb | k) != 0);
-                    mma_commit_pair(&empty[s]);
+                        for (int k = 0; k < kBK / 32; ++k)  // 32 bytes are 2 units of a descriptor's address
+                            mma_i8_ss_pair(tmem + acc * BN, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+                        mma_commit_pair(&empty[s]);
+                    }
+                    __syncwarp();
                 }
-                if (ok)
+                if (ok && elect_one_sync())
                     mma_commit_pair(&acc_full[acc]);
+                __syncwarp();
             }
-            mma_commit_pair(drain);
+            if (elect_one_sync())
+                mma_commit_pair(drain);
+            __syncwarp();
             mbar_wait(drain, 0, a.status, kErrWaitDrain, nullptr);
         }
     } else {
