@@ -1,66 +1,69 @@
-// Row kernels of a quantised block (see gate_norm.cuh). A row belongs to one block, a thread holds up to 24 (32 for
-// plain quantising) of its values in registers between the passes over it, so each byte crosses HBM once.
+// Row kernels of a quantised block (see gate_norm.cuh). Bounded by HBM: a row's values stay in its block's registers between
+// the passes over them, so each byte crosses HBM once. Where there are rows enough a block walks a run of one sample's rows
+// with the vectors (weights, gate, modulation: five values for each of a row's elements, out of L2, and the gate's tanh)
+// folded into three and kept in registers.
 #include "gate_norm.cuh"
 #include "common.cuh"
+#include "gemm.cuh"
 #include "launch.cuh"
 #include "quant.cuh"
+
+#include <algorithm>
 
 namespace mkb {
 
 namespace {
 
-__device__ __forceinline__ float warp_sum(float v)
+// Sum (or largest magnitude) over the block's threads, in the same order in every thread and call. `s`: a float for each of up
+// to 16 warps; a caller that comes back to the same ones has passed another reduction's barrier in between.
+__device__ __forceinline__ float block_sum(float v, float* s)
 {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
         v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (warps == 1)
+        return v;
+    if (lane == 0)
+        s[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = (lane & 15) < warps ? s[lane & 15] : 0.0f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+        v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
-// Sum over the block's threads, in the same order in every thread and call. `s`: a float for each warp, not used by
-// another reduction of the block (so no barrier has to guard its reuse).
-__device__ __forceinline__ float block_sum(float v, float* s)
+__device__ __forceinline__ float block_max_abs(float v, float* s)
 {
-    v = warp_sum(v);
-    const int warps = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        v = max_abs(v, __shfl_xor_sync(0xffffffffu, v, o));
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
     if (warps == 1)
         return v;
-    if ((threadIdx.x & 31) == 0)
+    if (lane == 0)
         s[threadIdx.x >> 5] = v;
     __syncthreads();
-    float t = 0.0f;
-    for (int i = 0; i < warps; ++i)
-        t += s[i];
-    return t;
+    v = (lane & 15) < warps ? s[lane & 15] : 0.0f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+        v = max_abs(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
 }
 
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* s)
-{
-    v = __reduce_max_sync(0xffffffffu, v);
-    const int warps = blockDim.x >> 5;
-    if (warps == 1)
-        return v;
-    if ((threadIdx.x & 31) == 0)
-        s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    uint32_t t = 0;
-    for (int i = 0; i < warps; ++i)
-        t = max(t, s[i]);
-    return t;
-}
-
-// VEC consecutive values as fp32.
+// VEC consecutive values as fp32. Rows pass once (streaming loads); the vectors, read by every block, stay cached.
 template <int VEC>
-__device__ __forceinline__ void load_f32(const float* p, float* v)
+__device__ __forceinline__ void load_vec(const float* p, float (&v)[VEC])
 {
     if constexpr (VEC == 4) {
-        const float4 t = *reinterpret_cast<const float4*>(p);
+        const float4 t = __ldg(reinterpret_cast<const float4*>(p));
         v[0] = t.x;
         v[1] = t.y;
         v[2] = t.z;
         v[3] = t.w;
     } else {
-        v[0] = *p;
+        v[0] = __ldg(p);
     }
 }
 
@@ -69,32 +72,71 @@ __device__ __forceinline__ float2 unpack_bf16(uint32_t u)
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 
+// VEC values of a row as they lie in memory, so that a load's registers are not touched before its data is wanted.
 template <int VEC>
-__device__ __forceinline__ void load_bf16(const __nv_bfloat16* p, float* v)
-{
-    if constexpr (VEC == 8) {
-        const uint4 t = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = unpack_bf16(w[i]);
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
+struct Raw {
+    uint32_t u[VEC];  // fp32: a word each; bf16: two to a word, VEC / 2 words (VEC = 1: its low half)
+    __device__ __forceinline__ void load(const float* p)
+    {
+        if constexpr (VEC == 4) {
+            const uint4 t = __ldcs(reinterpret_cast<const uint4*>(p));
+            u[0] = t.x;
+            u[1] = t.y;
+            u[2] = t.z;
+            u[3] = t.w;
+        } else {
+            u[0] = __ldcs(reinterpret_cast<const uint32_t*>(p));
         }
-    } else if constexpr (VEC == 4) {
-        const uint2 t = *reinterpret_cast<const uint2*>(p);
-        const float2 a = unpack_bf16(t.x), b = unpack_bf16(t.y);
-        v[0] = a.x;
-        v[1] = a.y;
-        v[2] = b.x;
-        v[3] = b.y;
-    } else {
-        v[0] = __bfloat162float(*p);
     }
-}
+    __device__ __forceinline__ void load(const __nv_bfloat16* p)
+    {
+        if constexpr (VEC == 8) {
+            const uint4 t = __ldcs(reinterpret_cast<const uint4*>(p));
+            u[0] = t.x;
+            u[1] = t.y;
+            u[2] = t.z;
+            u[3] = t.w;
+        } else if constexpr (VEC == 4) {
+            const uint2 t = __ldcs(reinterpret_cast<const uint2*>(p));
+            u[0] = t.x;
+            u[1] = t.y;
+        } else {
+            u[0] = __ldcs(reinterpret_cast<const unsigned short*>(p));
+        }
+    }
+    __device__ __forceinline__ void zero()
+    {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+            u[k] = 0;
+    }
+    __device__ __forceinline__ void values(bool f32, float (&v)[VEC]) const
+    {
+        if constexpr (VEC == 8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = unpack_bf16(u[k]);
+                v[2 * k] = f.x;
+                v[2 * k + 1] = f.y;
+            }
+        } else if (f32) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k)
+                v[k] = __uint_as_float(u[k]);
+        } else if constexpr (VEC == 4) {
+            const float2 a = unpack_bf16(u[0]), b = unpack_bf16(u[1]);
+            v[0] = a.x;
+            v[1] = a.y;
+            v[2] = b.x;
+            v[3] = b.y;
+        } else {
+            v[0] = __uint_as_float(u[0] << 16);
+        }
+    }
+};
 
 template <int VEC>
-__device__ __forceinline__ void store_f32(float* p, const float* v)
+__device__ __forceinline__ void store_row(float* p, const float (&v)[VEC])
 {
     if constexpr (VEC == 4)
         *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
@@ -108,12 +150,28 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi)
     return *reinterpret_cast<const uint32_t*>(&t);
 }
 
-// Standardises the row held in v (NC chunks of VEC values a thread; values past the row are 0 on entry).
-template <int VEC, int NC>
-__device__ __forceinline__ void normalise(float (&v)[NC][VEC], int kind, int n, float eps, float (*red)[32])
+template <int VEC>
+__device__ __forceinline__ void store_row(__nv_bfloat16* p, const float (&v)[VEC])
 {
-    const int tid = threadIdx.x, T = blockDim.x;
-    float mean = 0.0f;
+    if constexpr (VEC == 4)
+        *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+    else
+        *p = __float2bfloat16(v[0]);
+}
+
+// A row's chunks of 32 * VEC values: NC to a warp, one after another, so that a thread's places in the row are constants apart.
+template <int VEC, int NC>
+struct Place {
+    int first;  // the thread's first value
+    __device__ __forceinline__ Place() : first(int(threadIdx.x >> 5) * NC * 32 * VEC + int(threadIdx.x & 31) * VEC) {}
+    __device__ __forceinline__ bool in(int i, int n) const { return first + i * 32 * VEC < n; }
+};
+
+// Standardises the row held in v (values past the row are 0 on entry and stay so).
+template <int VEC, int NC>
+__device__ __forceinline__ void normalise(float (&v)[NC][VEC], const Place<VEC, NC>& at, int kind, int n, float inv_n,
+                                          float eps, float* red)
+{
     if (kind == kNormLayer) {  // mean first, then the squares about it: no cancellation where the mean is large
         float s = 0.0f;
 #pragma unroll
@@ -121,18 +179,21 @@ __device__ __forceinline__ void normalise(float (&v)[NC][VEC], int kind, int n, 
 #pragma unroll
             for (int k = 0; k < VEC; ++k)
                 s += v[i][k];
-        mean = block_sum(s, red[0]) / float(n);
+        const float mean = block_sum(s, red) * inv_n;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            if (at.in(i, n))
+#pragma unroll
+                for (int k = 0; k < VEC; ++k)
+                    v[i][k] -= mean;
     }
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
-        if ((i * T + tid) * VEC < n)
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                v[i][k] -= mean;
-                s = fmaf(v[i][k], v[i][k], s);
-            }
-    const float r = rsqrtf(block_sum(s, red[1]) / float(n) + eps);
+        for (int k = 0; k < VEC; ++k)
+            s = fmaf(v[i][k], v[i][k], s);
+    const float r = rsqrtf(fmaf(block_sum(s, red + 16), inv_n, eps));
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
@@ -140,237 +201,292 @@ __device__ __forceinline__ void normalise(float (&v)[NC][VEC], int kind, int n, 
             v[i][k] *= r;
 }
 
-// One block a row: VEC values at a time, NC chunks a thread. n is a multiple of VEC.
-template <int VEC, int NC>
-__global__ void __launch_bounds__(512) k_gate_norm(const GateNormArgs a)
+template <int VEC, int NC, typename T>
+__device__ __forceinline__ void load_row_at(Raw<VEC> (&v)[NC], const T* p, const Place<VEC, NC>& at, int n)
 {
-    __shared__ float red[5][32];
-    grid_dep_wait();
-    grid_dep_launch();
-    const long row = blockIdx.x;
-    const int tid = threadIdx.x, T = blockDim.x, n = a.n;
-    const long sample = row / a.rows_per_sample;
-    float x[NC][VEC], y[NC][VEC];
-    const float* xr = a.x + row * a.ldx;
+    p += at.first;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        const int c = (i * T + tid) * VEC;
-        if (c < n) {
-            load_f32<VEC>(xr + c, x[i]);
-        } else {
-#pragma unroll
-            for (int k = 0; k < VEC; ++k)
-                x[i][k] = 0.0f;
-        }
-    }
-    if (a.y) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int c = (i * T + tid) * VEC;
-            if (c >= n) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k)
-                    y[i][k] = 0.0f;
-            } else if (a.y_f32) {
-                load_f32<VEC>(static_cast<const float*>(a.y) + row * a.ldy + c, y[i]);
-            } else {
-                load_bf16<VEC>(static_cast<const __nv_bfloat16*>(a.y) + row * a.ldy + c, y[i]);
-            }
-        }
-        if (a.y_norm != kNormNone)
-            normalise<VEC, NC>(y, a.y_norm, n, a.eps, red);
-        const float* gate = a.gate ? a.gate + sample * a.gate_stride : nullptr;
-        float* xo = a.x_out + row * a.ldxo;
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int c = (i * T + tid) * VEC;
-            if (c < n) {
-                float g[VEC];
-#pragma unroll
-                for (int k = 0; k < VEC; ++k)
-                    g[k] = 1.0f;
-                if (gate) {
-                    load_f32<VEC>(gate + c, g);
-                    if (a.tanh_gate) {
-#pragma unroll
-                        for (int k = 0; k < VEC; ++k)
-                            g[k] = tanhf(g[k]);
-                    }
-                }
-                if (a.y_weight) {
-                    float w[VEC];
-                    load_f32<VEC>(a.y_weight + c, w);
-#pragma unroll
-                    for (int k = 0; k < VEC; ++k)
-                        y[i][k] *= w[k];
-                }
-#pragma unroll
-                for (int k = 0; k < VEC; ++k)
-                    x[i][k] = fmaf(g[k], y[i][k], x[i][k]);
-                store_f32<VEC>(xo + c, x[i]);
-            }
-        }
-    }
-    if (a.out_type == kOutNone)
-        return;
-    if (a.x_norm != kNormNone)
-        normalise<VEC, NC>(x, a.x_norm, n, a.eps, red + 2);
-    const float* scale = a.scale ? a.scale + sample * a.mod_stride : nullptr;
-    const float* shift = a.shift ? a.shift + sample * a.mod_stride : nullptr;
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const int c = (i * T + tid) * VEC;
-        if (c < n) {
-            float t[VEC];
-            if (a.x_weight) {
-                load_f32<VEC>(a.x_weight + c, t);
-#pragma unroll
-                for (int k = 0; k < VEC; ++k)
-                    x[i][k] *= t[k];
-            }
-            if (scale) {
-                load_f32<VEC>(scale + c, t);
-#pragma unroll
-                for (int k = 0; k < VEC; ++k)
-                    x[i][k] = fmaf(x[i][k], t[k], x[i][k]);
-            }
-            if (shift) {
-                load_f32<VEC>(shift + c, t);
-#pragma unroll
-                for (int k = 0; k < VEC; ++k)
-                    x[i][k] += t[k];
-            }
-            if (a.out_type == kOutBf16) {
-                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.out) + row * a.ldo + c;
-                if constexpr (VEC == 4)
-                    *reinterpret_cast<uint2*>(o) =
-                        make_uint2(pack_bf16(x[i][0], x[i][1]), pack_bf16(x[i][2], x[i][3]));
-                else
-                    *o = __float2bfloat16(x[i][0]);
-            } else if (a.out_type == kOutF32) {
-                store_f32<VEC>(static_cast<float*>(a.out) + row * a.ldo + c, x[i]);
-            } else {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k)
-                    top = max(top, abs_bits(x[i][k]));
-            }
-        }
-    }
-    if (a.out_type != kOutI8)
-        return;
-    const RowStep step(block_max(top, reinterpret_cast<uint32_t*>(red[4])));
-    if (tid == 0)
-        a.out_scale[row] = step.step;
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const int c = (i * T + tid) * VEC;
-        if (c < n) {
-            int8_t* o = static_cast<int8_t*>(a.out) + row * a.ldo + c;
-            if constexpr (VEC == 4)
-                *reinterpret_cast<uint32_t*>(o) = pack4_i8(step(x[i][0]), step(x[i][1]), step(x[i][2]), step(x[i][3]));
-            else
-                *o = int8_t(step(x[i][0]));
-        }
+        if (at.in(i, n))
+            v[i].load(p + i * 32 * VEC);
+        else
+            v[i].zero();
     }
 }
 
-// One block a row; rows up to blockDim * NC * VEC values stay in registers.
-template <typename XT, int VEC, int NC>
-__global__ void __launch_bounds__(512) k_quant_rows(const QuantRowsArgs a)
+template <int VEC, int NC>
+__device__ __forceinline__ void values(const Raw<VEC> (&r)[NC], bool f32, float (&v)[NC][VEC])
 {
-    __shared__ uint32_t red[32];
-    grid_dep_wait();
-    grid_dep_launch();
-    const long row = blockIdx.x;
-    const int tid = threadIdx.x, T = blockDim.x, n = a.n;
-    const XT* xr = static_cast<const XT*>(a.x) + row * a.ldx;
-    int8_t* qr = a.q + row * a.ldq;
-    float x[NC][VEC];
-    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const int c = (i * T + tid) * VEC;
-        if (c < n) {
-            if constexpr (sizeof(XT) == 4)
-                load_f32<VEC>(xr + c, x[i]);
-            else
-                load_bf16<VEC>(xr + c, x[i]);
-        } else {
+    for (int i = 0; i < NC; ++i)
+        r[i].values(f32, v[i]);
+}
+
+template <int VEC, int NC, typename T>
+__device__ __forceinline__ void store_row_at(const float (&v)[NC][VEC], T* p, const Place<VEC, NC>& at, int n)
+{
+    p += at.first;
 #pragma unroll
-            for (int k = 0; k < VEC; ++k)
-                x[i][k] = 0.0f;
-        }
-    }
+    for (int i = 0; i < NC; ++i)
+        if (at.in(i, n))
+            store_row(p + i * 32 * VEC, v[i]);
+}
+
+// The row as 8-bit integers with their step.
+template <int VEC, int NC>
+__device__ __forceinline__ void quant_row_at(const float (&v)[NC][VEC], int8_t* q, float* scale, const Place<VEC, NC>& at,
+                                             int n, float* red)
+{
+    float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < NC; ++i)
 #pragma unroll
         for (int k = 0; k < VEC; ++k)
-            top = max(top, abs_bits(x[i][k]));
-    const RowStep step(block_max(top, red));
-    if (tid == 0)
-        a.scale[row] = step.step;
+            top = max_abs(top, v[i][k]);
+    const RowStep step(block_max_abs(top, red));
+    if (threadIdx.x == 0)
+        *scale = step.step;
+    q += at.first;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const int c = (i * T + tid) * VEC;
-        if (c < n) {
+    for (int i = 0; i < NC; ++i)
+        if (at.in(i, n)) {
+            int8_t* o = q + i * 32 * VEC;
             if constexpr (VEC == 1) {
-                qr[c] = int8_t(step(x[i][0]));
+                *o = step.one(v[i][0]);
             } else {
                 uint32_t p[VEC / 4];
 #pragma unroll
-                for (int k = 0; k < VEC / 4; ++k)
-                    p[k] = pack4_i8(step(x[i][4 * k]), step(x[i][4 * k + 1]), step(x[i][4 * k + 2]),
-                                    step(x[i][4 * k + 3]));
+                for (int k = 0; k < VEC / 4; ++k) {
+                    const float u[4] = {v[i][4 * k], v[i][4 * k + 1], v[i][4 * k + 2], v[i][4 * k + 3]};
+                    p[k] = step.pack4(u);
+                }
                 if constexpr (VEC == 8)
-                    *reinterpret_cast<uint2*>(qr + c) = make_uint2(p[0], p[1]);
+                    *reinterpret_cast<uint2*>(o) = make_uint2(p[0], p[1]);
                 else
-                    *reinterpret_cast<uint32_t*>(qr + c) = p[0];
+                    *reinterpret_cast<uint32_t*>(o) = p[0];
             }
         }
+}
+
+// tanh(x) to a few units of 2^-24 of itself: below 0.4 its Taylor series to x^11 (the next term is under 2^-25 of the sum
+// there), else 1 - 2 / (e^2|x| + 1) with x's sign.
+__device__ __forceinline__ float tanh_near(float x)
+{
+    const float s = x * x, a = fabsf(x);
+    float p = fmaf(s, -8.8632355e-3f, 2.1869488e-2f);
+    p = fmaf(s, p, -5.3968254e-2f);
+    p = fmaf(s, p, 1.3333333e-1f);
+    p = fmaf(s, p, -3.3333333e-1f);
+    const float small = fmaf(x * s, p, x);
+    const float big = copysignf(1.0f - __fdividef(2.0f, __expf(2.0f * fminf(a, 20.0f)) + 1.0f), x);
+    return a < 0.4f ? small : a >= 0.4f ? big : x;  // a NaN comes back
+}
+
+// The vectors over a row's places, as far as one chunk of one thread goes: y's factor g(gate) * y_weight, and x's
+// h * factor + shift with factor = x_weight * (1 + scale).
+template <int VEC>
+struct Vectors {
+    float gate[VEC], factor[VEC], shift[VEC];
+    __device__ __forceinline__ void branch(const GateNormArgs& a, long sample, int c)
+    {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+            gate[k] = 1.0f;
+        if (a.gate) {
+            load_vec(a.gate + sample * a.gate_stride + c, gate);
+            if (a.tanh_gate)
+#pragma unroll
+                for (int k = 0; k < VEC; ++k)
+                    gate[k] = tanh_near(gate[k]);
+        }
+        if (a.y_weight) {
+            float w[VEC];
+            load_vec(a.y_weight + c, w);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k)
+                gate[k] *= w[k];
+        }
     }
+    __device__ __forceinline__ void stream(const GateNormArgs& a, long sample, int c)
+    {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            factor[k] = 1.0f;
+            shift[k] = 0.0f;
+        }
+        if (a.x_weight)
+            load_vec(a.x_weight + c, factor);
+        if (a.scale) {
+            float s[VEC];
+            load_vec(a.scale + sample * a.mod_stride + c, s);
+#pragma unroll
+            for (int k = 0; k < VEC; ++k)
+                factor[k] = fmaf(factor[k], s[k], factor[k]);
+        }
+        if (a.shift)
+            load_vec(a.shift + sample * a.mod_stride + c, shift);
+    }
+};
+
+// A block a run of `run` rows of one sample, NC chunks of 32 * VEC values a warp and row. n is a multiple of VEC. KEEP: the
+// vectors stay in registers from row to row and each row is loaded while the one before is worked on (otherwise a run is one
+// row).
+template <int VEC, int NC, bool KEEP>
+__global__ void __launch_bounds__(512) k_gate_norm(const GateNormArgs a, int run)
+{
+    __shared__ float red[2][5][16];
+    grid_dep_wait();
+    grid_dep_launch();
+    const unsigned blocks = (unsigned(a.rows_per_sample) + run - 1) / run;  // of a sample
+    const long sample = blockIdx.x / blocks;
+    const long lo = sample * a.rows_per_sample + long(blockIdx.x % blocks) * run;
+    const long hi = min(min(a.rows, (sample + 1) * a.rows_per_sample), lo + run);
+    const int n = a.n;
+    const float inv_n = 1.0f / float(n);
+    const Place<VEC, NC> at;
+    Vectors<VEC> kept[KEEP ? NC : 1];
+    if constexpr (KEEP)
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            if (at.in(i, n)) {
+                kept[i].branch(a, sample, at.first + i * 32 * VEC);
+                kept[i].stream(a, sample, at.first + i * 32 * VEC);
+            }
+    Raw<VEC> rx[NC], ry[NC];
+    const auto load = [&](long row) {
+        load_row_at(rx, a.x + row * a.ldx, at, n);
+        if (a.y && a.y_f32)
+            load_row_at(ry, static_cast<const float*>(a.y) + row * a.ldy, at, n);
+        else if (a.y)
+            load_row_at(ry, static_cast<const __nv_bfloat16*>(a.y) + row * a.ldy, at, n);
+    };
+    if (lo < hi)
+        load(lo);
+    int turn = 0;
+    for (long row = lo; row < hi; ++row, turn ^= 1) {
+        float x[NC][VEC], y[NC][VEC];
+        values(rx, true, x);
+        if (a.y)
+            values(ry, a.y_f32, y);
+        if (KEEP && row + 1 < hi)
+            load(row + 1);
+        if (a.y) {
+            if (a.y_norm != kNormNone)
+                normalise(y, at, a.y_norm, n, inv_n, a.eps, red[turn][0]);
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                if (at.in(i, n)) {
+                    Vectors<VEC>& v = kept[KEEP ? i : 0];
+                    if constexpr (!KEEP)
+                        v.branch(a, sample, at.first + i * 32 * VEC);
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k)
+                        x[i][k] = fmaf(y[i][k], v.gate[k], x[i][k]);
+                }
+            store_row_at(x, a.x_out + row * a.ldxo, at, n);
+        }
+        if (a.out_type == kOutNone)
+            continue;
+        if (a.x_norm != kNormNone)
+            normalise(x, at, a.x_norm, n, inv_n, a.eps, red[turn][2]);
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            if (at.in(i, n)) {
+                Vectors<VEC>& v = kept[KEEP ? i : 0];
+                if constexpr (!KEEP)
+                    v.stream(a, sample, at.first + i * 32 * VEC);
+#pragma unroll
+                for (int k = 0; k < VEC; ++k)
+                    x[i][k] = fmaf(x[i][k], v.factor[k], v.shift[k]);
+            }
+        if (a.out_type == kOutBf16)
+            store_row_at(x, static_cast<__nv_bfloat16*>(a.out) + row * a.ldo, at, n);
+        else if (a.out_type == kOutF32)
+            store_row_at(x, static_cast<float*>(a.out) + row * a.ldo, at, n);
+        else
+            quant_row_at(x, static_cast<int8_t*>(a.out) + row * a.ldo, a.out_scale + row, at, n, red[turn][4]);
+    }
+}
+
+// A block a row, NC chunks of 32 * VEC values a warp.
+template <typename XT, int VEC, int NC>
+__global__ void __launch_bounds__(512) k_quant_rows(const QuantRowsArgs a)
+{
+    __shared__ float red[16];
+    grid_dep_wait();
+    grid_dep_launch();
+    const long row = blockIdx.x;
+    const Place<VEC, NC> at;
+    Raw<VEC> r[NC];
+    load_row_at(r, static_cast<const XT*>(a.x) + row * a.ldx, at, a.n);
+    float x[NC][VEC];
+    values(r, sizeof(XT) == 4, x);
+    quant_row_at(x, a.q + row * a.ldq, a.scale + row, at, a.n, red);
 }
 
 // Rows too long for a block's registers: a pass for the step, a second one (out of L2) for the values.
 template <typename XT>
 __global__ void __launch_bounds__(512) k_quant_long(const QuantRowsArgs a)
 {
-    __shared__ uint32_t red[32];
+    __shared__ float red[16];
     grid_dep_wait();
     grid_dep_launch();
     const long row = blockIdx.x;
     const XT* xr = static_cast<const XT*>(a.x) + row * a.ldx;
     int8_t* qr = a.q + row * a.ldq;
-    uint32_t top = 0;
+    float top = 0.0f;
     for (int c = threadIdx.x; c < a.n; c += blockDim.x)
-        top = max(top, abs_bits(float(xr[c])));
-    const RowStep step(block_max(top, red));
+        top = max_abs(top, float(xr[c]));
+    const RowStep step(block_max_abs(top, red));
     if (threadIdx.x == 0)
         a.scale[row] = step.step;
     for (int c = threadIdx.x; c < a.n; c += blockDim.x)
-        qr[c] = int8_t(step(float(xr[c])));
+        qr[c] = step.one(float(xr[c]));
 }
 
 bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-template <int VEC, int NC>
-cudaError_t launch_gate_norm(const GateNormArgs& a, int threads, cudaStream_t st)
+// How a row of `chunks` chunks is dealt out: NC chunks a warp (at most `most`) on up to 16 warps, with few idle chunk places;
+// among equals more warps, which shortens the block's way from its loads to its stores.
+struct Deal {
+    int nc, warps;
+};
+Deal deal(int chunks, int most)
 {
-    return launch_k(k_gate_norm<VEC, NC>, dim3(unsigned(a.rows)), threads, 0, st, a);
+    Deal best{0, 0};
+    for (int nc = 1; nc <= most; ++nc) {
+        const int warps = (chunks + nc - 1) / nc;
+        if (warps <= 16 && (!best.nc || warps * nc < best.warps * best.nc))
+            best = Deal{nc, warps};
+    }
+    return best;
+}
+
+template <int VEC, int NC, bool KEEP>
+cudaError_t launch_gate_norm(const GateNormArgs& a, int warps, cudaStream_t st)
+{
+    const long samples = (a.rows + a.rows_per_sample - 1) / a.rows_per_sample;
+    // Runs as long as still leave one wave of blocks (24 warps an SM).
+    const long wave = long(num_sms()) * std::max(1, 24 / warps);
+    const int run = KEEP ? int(std::min(a.rows_per_sample, std::max(1L, (a.rows + wave - 1) / wave))) : 1;
+    return launch_k(k_gate_norm<VEC, NC, KEEP>, dim3(unsigned(samples * ((a.rows_per_sample + run - 1) / run))), 32 * warps,
+                    0, st, a, run);
 }
 
 template <typename XT, int VEC, int NC>
-cudaError_t launch_quant(const QuantRowsArgs& a, int threads, cudaStream_t st)
+cudaError_t launch_quant(const QuantRowsArgs& a, int warps, cudaStream_t st)
 {
-    return launch_k(k_quant_rows<XT, VEC, NC>, dim3(unsigned(a.rows)), threads, 0, st, a);
+    return launch_k(k_quant_rows<XT, VEC, NC>, dim3(unsigned(a.rows)), 32 * warps, 0, st, a);
 }
 
 }  // namespace
 
-cudaError_t gate_norm(const GateNormArgs& a, cudaStream_t st)
+cudaError_t gate_norm(const GateNormArgs& args, cudaStream_t st)
 {
-    if (a.rows == 0)
+    if (args.rows == 0)
         return cudaSuccess;
+    GateNormArgs a = args;
+    a.rows_per_sample = std::min(a.rows_per_sample, a.rows);
     // 16-byte accesses where every row and vector allows them, single values otherwise.
     const size_t yb = a.y_f32 ? 16 : 8, ob = a.out_type == kOutBf16 ? 8 : a.out_type == kOutF32 ? 16 : 4;
     const bool vec = a.n % 4 == 0 && aligned(a.x, 16) && a.ldx % 4 == 0 &&
@@ -378,22 +494,24 @@ cudaError_t gate_norm(const GateNormArgs& a, cudaStream_t st)
                      aligned(a.y_weight, 16) && aligned(a.gate, 16) && a.gate_stride % 4 == 0 &&
                      aligned(a.x_weight, 16) && aligned(a.scale, 16) && aligned(a.shift, 16) &&
                      a.mod_stride % 4 == 0 && (a.out_type == kOutNone || (aligned(a.out, ob) && a.ldo % 4 == 0));
-    // Up to 24 values a thread (both rows' values stay in registers), so as many warps as that takes.
-    int warps = 1;
-    while (warps * 32 * 24 < a.n && warps < 16)
-        warps *= 2;
-    const int per = (a.n + warps * 32 - 1) / (warps * 32), t = warps * 32;
     cudaError_t e;
     if (vec) {
-        const int nc = (a.n / 4 + t - 1) / t;
-        e = nc <= 1   ? launch_gate_norm<4, 1>(a, t, st)
-            : nc <= 2 ? launch_gate_norm<4, 2>(a, t, st)
-            : nc <= 4 ? launch_gate_norm<4, 4>(a, t, st)
-                      : launch_gate_norm<4, 6>(a, t, st);
+        const int chunks = (a.n + 127) / 128;
+        const Deal d = deal(chunks, chunks <= 48 ? 3 : 6);
+        e = d.nc == 1   ? launch_gate_norm<4, 1, true>(a, d.warps, st)
+            : d.nc == 2 ? launch_gate_norm<4, 2, true>(a, d.warps, st)
+            : d.nc == 3 ? launch_gate_norm<4, 3, true>(a, d.warps, st)
+            : d.nc == 4 ? launch_gate_norm<4, 4, false>(a, d.warps, st)
+            : d.nc == 5 ? launch_gate_norm<4, 5, false>(a, d.warps, st)
+                        : launch_gate_norm<4, 6, false>(a, d.warps, st);
     } else {
-        e = per <= 8    ? launch_gate_norm<1, 8>(a, t, st)
-            : per <= 16 ? launch_gate_norm<1, 16>(a, t, st)
-                        : launch_gate_norm<1, 24>(a, t, st);
+        const int chunks = (a.n + 31) / 32;
+        if (chunks <= 64)
+            e = launch_gate_norm<1, 4, true>(a, (chunks + 3) / 4, st);
+        else if (chunks <= 128)
+            e = launch_gate_norm<1, 8, true>(a, (chunks + 7) / 8, st);
+        else
+            e = launch_gate_norm<1, 24, false>(a, (chunks + 23) / 24, st);
     }
     if (e != cudaSuccess)
         return e;
@@ -405,33 +523,34 @@ cudaError_t quantize_rows(const QuantRowsArgs& a, cudaStream_t st)
 {
     if (a.rows == 0)
         return cudaSuccess;
-    int warps = 1;
-    while (warps * 32 * 32 < a.n && warps < 16)
-        warps *= 2;
-    const int t = warps * 32, v = a.x_f32 ? 4 : 8;
+    const int v = a.x_f32 ? 4 : 8;
     const bool vec = a.n % v == 0 && aligned(a.x, 16) && a.ldx % v == 0 && aligned(a.q, v) && a.ldq % v == 0;
-    const int per = (a.n + t - 1) / t;
+    const int chunks = (a.n + 32 * (vec ? v : 1) - 1) / (32 * (vec ? v : 1));
     cudaError_t e;
-    if (per > 32) {
+    if (a.n > 16384 || (!vec && chunks > 16 * 32)) {
         e = a.x_f32 ? launch_k(k_quant_long<float>, dim3(unsigned(a.rows)), 512, 0, st, a)
                     : launch_k(k_quant_long<__nv_bfloat16>, dim3(unsigned(a.rows)), 512, 0, st, a);
     } else if (!vec) {
         if (a.x_f32)
-            e = per <= 8 ? launch_quant<float, 1, 8>(a, t, st) : launch_quant<float, 1, 32>(a, t, st);
+            e = chunks <= 128 ? launch_quant<float, 1, 8>(a, (chunks + 7) / 8, st)
+                              : launch_quant<float, 1, 32>(a, (chunks + 31) / 32, st);
         else
-            e = per <= 8 ? launch_quant<__nv_bfloat16, 1, 8>(a, t, st) : launch_quant<__nv_bfloat16, 1, 32>(a, t, st);
+            e = chunks <= 128 ? launch_quant<__nv_bfloat16, 1, 8>(a, (chunks + 7) / 8, st)
+                              : launch_quant<__nv_bfloat16, 1, 32>(a, (chunks + 31) / 32, st);
     } else if (a.x_f32) {
-        const int nc = (a.n / 4 + t - 1) / t;
-        e = nc <= 2 ? launch_quant<float, 4, 2>(a, t, st)
-            : nc <= 4 ? launch_quant<float, 4, 4>(a, t, st)
-            : nc <= 6 ? launch_quant<float, 4, 6>(a, t, st)
-                      : launch_quant<float, 4, 8>(a, t, st);
+        const Deal d = deal(chunks, chunks <= 64 ? 4 : 8);
+        e = d.nc == 1   ? launch_quant<float, 4, 1>(a, d.warps, st)
+            : d.nc == 2 ? launch_quant<float, 4, 2>(a, d.warps, st)
+            : d.nc == 3 ? launch_quant<float, 4, 3>(a, d.warps, st)
+            : d.nc == 4 ? launch_quant<float, 4, 4>(a, d.warps, st)
+            : d.nc <= 6 ? launch_quant<float, 4, 6>(a, (chunks + 5) / 6, st)
+                        : launch_quant<float, 4, 8>(a, (chunks + 7) / 8, st);
     } else {
-        const int nc = (a.n / 8 + t - 1) / t;
-        e = nc <= 1 ? launch_quant<__nv_bfloat16, 8, 1>(a, t, st)
-            : nc <= 2 ? launch_quant<__nv_bfloat16, 8, 2>(a, t, st)
-            : nc <= 3 ? launch_quant<__nv_bfloat16, 8, 3>(a, t, st)
-                      : launch_quant<__nv_bfloat16, 8, 4>(a, t, st);
+        const Deal d = deal(chunks, 4);
+        e = d.nc == 1   ? launch_quant<__nv_bfloat16, 8, 1>(a, d.warps, st)
+            : d.nc == 2 ? launch_quant<__nv_bfloat16, 8, 2>(a, d.warps, st)
+            : d.nc == 3 ? launch_quant<__nv_bfloat16, 8, 3>(a, d.warps, st)
+                        : launch_quant<__nv_bfloat16, 8, 4>(a, d.warps, st);
     }
     if (e != cudaSuccess)
         return e;

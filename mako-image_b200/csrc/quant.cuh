@@ -10,39 +10,67 @@ namespace mkb {
 // Row steps below the smallest normal number are taken as 0 (the row's values all become 0): 1 / step stays finite.
 constexpr float kMinStep = 1.17549435e-38f;
 
-// |x| as an ordered integer: a maximum over these bits keeps infinities and NaN, which fmaxf would drop.
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// The larger magnitude, or NaN where there is one.
+__device__ __forceinline__ float max_abs(float m, float x)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+    return r;
+}
 
 struct RowStep {
+    static constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, ties to even
     float step, inv, half;
-    __device__ __forceinline__ explicit RowStep(uint32_t amax_bits)
+    __device__ __forceinline__ explicit RowStep(float amax)
     {
-        const float amax = __uint_as_float(amax_bits);
-        step = amax_bits >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __fdiv_rn(amax, 127.0f);
+        step = amax <= 3.4028235e38f ? __fdiv_rn(amax, 127.0f) : __uint_as_float(0x7fffffffu);
         if (step < kMinStep)
             step = 0.0f;
         // A row of zeros, or one with an infinity or a NaN in it (step NaN), has only zeros.
         inv = step > 0.0f ? 1.0f / step : 0.0f;
         half = 0.5f * step;
     }
-    // x / step to the nearest whole number, ties to even. rint(x * inv) may be one off next to a border of two whole
-    // numbers; the remainder x - q step decides. It is a multiple of the smaller of the two numbers' last places and no
-    // larger than about step / 2, so the fused multiply-add gives it without rounding.
-    __device__ __forceinline__ int operator()(float x) const
+    // x / step to the nearest whole number, ties to even, as the low byte of each result's bits. x * inv is off by a few
+    // roundings, so its nearest whole number may be one off next to a border of two; the remainder x - q step decides. It is
+    // a multiple of the smaller of the two numbers' last places and no larger than about step / 2, so the fused
+    // multiply-add gives it without rounding.
+    template <int N>
+    __device__ __forceinline__ void whole(const float (&x)[N], float (&t)[N]) const
     {
-        if (inv == 0.0f)
+        float far = -1.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            t[i] = fmaf(x[i], inv, kRound);
+            far = fmaxf(far, fabsf(fmaf(kRound - t[i], step, x[i])) - half);
+        }
+        if (far >= 0.0f) {  // on or beyond a border: rare
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float r = fmaf(kRound - t[i], step, x[i]), over = fabsf(r) - half;
+                if (over > 0.0f || (over == 0.0f && (__float_as_int(t[i]) & 1)))
+                    t[i] += copysignf(1.0f, r);
+            }
+        }
+    }
+    __device__ __forceinline__ uint32_t pack4(const float (&x)[4]) const
+    {
+        if (!(inv > 0.0f))
             return 0;
-        float q = rintf(x * inv);
-        const float r = fmaf(-q, step, x), d = fabsf(r) - half;
-        if (d > 0.0f || (d == 0.0f && (int(q) & 1)))
-            q += copysignf(1.0f, r);
-        return int(q);
+        float t[4];
+        whole(x, t);
+        const uint32_t lo = __byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040);
+        const uint32_t hi = __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040);
+        return __byte_perm(lo, hi, 0x5410);
+    }
+    __device__ __forceinline__ int8_t one(float x) const
+    {
+        if (!(inv > 0.0f))
+            return 0;
+        const float v[1] = {x};
+        float t[1];
+        whole(v, t);
+        return int8_t(__float_as_uint(t[0]) & 0xff);
     }
 };
-
-__device__ __forceinline__ uint32_t pack4_i8(int a, int b, int c, int d)
-{
-    return (uint32_t(a) & 0xff) | (uint32_t(b) & 0xff) << 8 | (uint32_t(c) & 0xff) << 16 | uint32_t(d) << 24;
-}
 
 }  // namespace mkb
