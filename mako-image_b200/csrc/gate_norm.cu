@@ -1,7 +1,7 @@
 // Row kernels of a quantised block (see gate_norm.cuh). Bounded by HBM: a row's values stay in its block's registers between
 // the passes over them, so each byte crosses HBM once. Where there are rows enough a block walks a run of one sample's rows
 // with the vectors (weights, gate, modulation: five values for each of a row's elements, out of L2, and the gate's tanh)
-// folded into three and kept in registers.
+// folded into three in shared memory.
 #include "gate_norm.cuh"
 #include "common.cuh"
 #include "gemm.cuh"
@@ -64,6 +64,20 @@ __device__ __forceinline__ void load_vec(const float* p, float (&v)[VEC])
         v[3] = t.w;
     } else {
         v[0] = __ldg(p);
+    }
+}
+
+template <int VEC>
+__device__ __forceinline__ void load_shared(const float* p, float (&v)[VEC])
+{
+    if constexpr (VEC == 4) {
+        const float4 t = *reinterpret_cast<const float4*>(p);
+        v[0] = t.x;
+        v[1] = t.y;
+        v[2] = t.z;
+        v[3] = t.w;
+    } else {
+        v[0] = *p;
     }
 }
 
@@ -329,10 +343,10 @@ struct Vectors {
 };
 
 // A block a run of `run` rows of one sample, NC chunks of 32 * VEC values a warp and row. n is a multiple of VEC. KEEP: the
-// vectors stay in registers from row to row and each row is loaded while the one before is worked on (otherwise a run is one
+// vectors stay in shared memory from row to row and each row is loaded while the one before is worked on (otherwise a run is one
 // row).
 template <int VEC, int NC, bool KEEP>
-__global__ void __launch_bounds__(512) k_gate_norm(const GateNormArgs a, int run)
+__global__ void __launch_bounds__(512, KEEP ? 2 : 1) k_gate_norm(const GateNormArgs a, int run)
 {
     __shared__ float red[2][5][16];
     grid_dep_wait();
@@ -344,13 +358,18 @@ __global__ void __launch_bounds__(512) k_gate_norm(const GateNormArgs a, int run
     const int n = a.n;
     const float inv_n = 1.0f / float(n);
     const Place<VEC, NC> at;
-    Vectors<VEC> kept[KEEP ? NC : 1];
+    extern __shared__ __align__(16) float kept[];  // KEEP: [gate, factor, shift][n], each thread its own places
+    float* mine = kept + at.first;
     if constexpr (KEEP)
 #pragma unroll
         for (int i = 0; i < NC; ++i)
             if (at.in(i, n)) {
-                kept[i].branch(a, sample, at.first + i * 32 * VEC);
-                kept[i].stream(a, sample, at.first + i * 32 * VEC);
+                Vectors<VEC> v;
+                v.branch(a, sample, at.first + i * 32 * VEC);
+                v.stream(a, sample, at.first + i * 32 * VEC);
+                store_row(mine + i * 32 * VEC, v.gate);
+                store_row(mine + n + i * 32 * VEC, v.factor);
+                store_row(mine + 2 * n + i * 32 * VEC, v.shift);
             }
     Raw<VEC> rx[NC], ry[NC];
     const auto load = [&](long row) {
@@ -376,8 +395,10 @@ __global__ void __launch_bounds__(512) k_gate_norm(const GateNormArgs a, int run
 #pragma unroll
             for (int i = 0; i < NC; ++i)
                 if (at.in(i, n)) {
-                    Vectors<VEC>& v = kept[KEEP ? i : 0];
-                    if constexpr (!KEEP)
+                    Vectors<VEC> v;
+                    if constexpr (KEEP)
+                        load_shared(mine + i * 32 * VEC, v.gate);
+                    else
                         v.branch(a, sample, at.first + i * 32 * VEC);
 #pragma unroll
                     for (int k = 0; k < VEC; ++k)
@@ -392,9 +413,13 @@ __global__ void __launch_bounds__(512) k_gate_norm(const GateNormArgs a, int run
 #pragma unroll
         for (int i = 0; i < NC; ++i)
             if (at.in(i, n)) {
-                Vectors<VEC>& v = kept[KEEP ? i : 0];
-                if constexpr (!KEEP)
+                Vectors<VEC> v;
+                if constexpr (KEEP) {
+                    load_shared(mine + n + i * 32 * VEC, v.factor);
+                    load_shared(mine + 2 * n + i * 32 * VEC, v.shift);
+                } else {
                     v.stream(a, sample, at.first + i * 32 * VEC);
+                }
 #pragma unroll
                 for (int k = 0; k < VEC; ++k)
                     x[i][k] = fmaf(x[i][k], v.factor[k], v.shift[k]);
@@ -446,8 +471,9 @@ __global__ void __launch_bounds__(512) k_quant_long(const QuantRowsArgs a)
 
 bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// How a row of `chunks` chunks is dealt out: NC chunks a warp (at most `most`) on up to 16 warps, with few idle chunk places;
-// among equals more warps, which shortens the block's way from its loads to its stores.
+// How a row of `chunks` chunks is dealt out: NC chunks a warp (at most `most`) on up to 16 warps, with few idle chunk places.
+// Among equals more warps, which shortens a block's way from its loads to its stores (8704 x 3072 to int8: 63 us on 12 warps
+// a row, 67 on 8).
 struct Deal {
     int nc, warps;
 };
@@ -466,11 +492,26 @@ template <int VEC, int NC, bool KEEP>
 cudaError_t launch_gate_norm(const GateNormArgs& a, int warps, cudaStream_t st)
 {
     const long samples = (a.rows + a.rows_per_sample - 1) / a.rows_per_sample;
-    // Runs as long as still leave one wave of blocks (24 warps an SM).
-    const long wave = long(num_sms()) * std::max(1, 24 / warps);
-    const int run = KEEP ? int(std::min(a.rows_per_sample, std::max(1L, (a.rows + wave - 1) / wave))) : 1;
+    const size_t smem = KEEP ? size_t(3) * a.n * sizeof(float) : 0;
+    if (smem > 48 * 1024) {
+        static std::atomic<uint64_t> devs{0};
+        const cudaError_t e = smem_limit_once(devs, k_gate_norm<VEC, NC, KEEP>, 3 * 6144 * int(sizeof(float)));
+        if (e != cudaSuccess)
+            return e;
+    }
+    // Runs as long as still leave one wave of resident blocks (two waves: 65 against 63 us at 8704 x 3072, three 69).
+    int run = 1;
+    if (KEEP && a.rows > 2L * num_sms()) {
+        int resident = 1;
+        const cudaError_t e =
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, k_gate_norm<VEC, NC, KEEP>, 32 * warps, smem);
+        if (e != cudaSuccess)
+            return e;
+        const long wave = long(num_sms()) * std::max(1, resident);
+        run = int(std::min(a.rows_per_sample, std::max(1L, (a.rows + wave - 1) / wave)));
+    }
     return launch_k(k_gate_norm<VEC, NC, KEEP>, dim3(unsigned(samples * ((a.rows_per_sample + run - 1) / run))), 32 * warps,
-                    0, st, a, run);
+                    smem, st, a, run);
 }
 
 template <typename XT, int VEC, int NC>

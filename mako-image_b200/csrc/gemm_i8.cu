@@ -15,6 +15,7 @@
 #include <cudaTypedefs.h>
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 namespace mkb {
 
@@ -225,7 +226,7 @@ template <int BN>
 struct SplitCfg {
     static constexpr int kABytes = 128 * kBK, kBBytes = BN * kBK, kStageBytes = kABytes + kBBytes;
     static constexpr int kStages = BN == 64 ? 8 : 6;
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + 256;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + 2 * BN * 4 + 256;
     static_assert(kSmem <= 227 * 1024);
     static_assert(kStages * kStageBytes >= 128 * BN * 4, "the partial sums reuse the stages");
 };
@@ -253,7 +254,8 @@ __global__ void __launch_bounds__(192, 1) k_i8_split(const __grid_constant__ I8P
     using C = SplitCfg<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kStages * C::kStageBytes);
+    float* vec = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);  // [w_scale, bias][BN]
+    uint64_t* full = reinterpret_cast<uint64_t*>(vec + 2 * BN);
     uint64_t* empty = full + C::kStages;
     uint64_t* acc_full = empty + C::kStages;
     uint64_t* drain = acc_full + 1;
@@ -338,6 +340,13 @@ __global__ void __launch_bounds__(192, 1) k_i8_split(const __grid_constant__ I8P
         __syncwarp();
         mbar_wait(drain, 0, a.status, kErrWaitDrain, nullptr);
     } else {
+        const int et = int(threadIdx.x) - 64;
+        for (int i = et; i < BN; i += 128) {  // while the main loop runs
+            const bool in = nb * BN + i < a.N;
+            vec[i] = in ? __ldg(a.w_scale + nb * BN + i) : 0.0f;
+            vec[BN + i] = in && a.bias ? __ldg(a.bias + nb * BN + i) : 0.0f;
+        }
+        named_barrier_sync<1, 128>();
         ok = mbar_wait(acc_full, 0, a.status, kErrWaitAccFull, abort_flag);
         tc_fence_after();
     }
@@ -369,26 +378,36 @@ __global__ void __launch_bounds__(192, 1) k_i8_split(const __grid_constant__ I8P
     if (warp >= 2 && ok) {
         const long row = long(mb) * 128 + r;
         const float sx = row < a.M ? __ldg(a.x_scale + row) : 0.0f;
-        for (int c = 0; c < cols; c += 8) {
-            const int col = nb * BN + part * cols + c;
-            if (col >= a.N)
-                break;
-            uint32_t t[8];
-            tmem_ld8(t_row + part * cols + c, t);
+        // W columns from tile column c on: this CTA's sum, the other parts' sums, the epilogue.
+        const auto finish = [&](auto width, int c) {
+            constexpr int W = decltype(width)::value;
+            const int tc = part * cols + c, col = nb * BN + tc;
+            uint32_t t[W];
+            if constexpr (W == 32)
+                tmem_ld32(t_row + tc, t);
+            else
+                tmem_ld8(t_row + tc, t);
             tmem_wait_ld();
-            float v[8];
+            float v[W];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < W; ++j) {
                 int s = int(t[j]);
                 for (int o = 0; o < S - 1; ++o)
                     s += sums[(o * cols + c + j) * 128 + r];
-                const bool in = col + j < a.N;
-                v[j] = fmaf(float(s) * sx, in ? __ldg(a.w_scale + col + j) : 0.0f,
-                            in && a.bias ? __ldg(a.bias + col + j) : 0.0f);
+                v[j] = fmaf(float(s) * sx, vec[tc + j], vec[BN + tc + j]);
             }
             act_out(v, a.act, a.out_f32);
             if (row < a.M)
                 store_row(a, row, col, v);
+        };
+        for (int c = 0; c < cols && nb * BN + part * cols + c < a.N;) {
+            if (cols - c >= 32) {
+                finish(std::integral_constant<int, 32>{}, c);
+                c += 32;
+            } else {
+                finish(std::integral_constant<int, 8>{}, c);
+                c += 8;
+            }
         }
     }
     tc_fence_before();
