@@ -472,17 +472,18 @@ __global__ void __launch_bounds__(512) k_quant_long(const QuantRowsArgs a)
 bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 // How a row of `chunks` chunks is dealt out: NC chunks a warp (at most `most`) on up to 16 warps, with few idle chunk places.
-// Among equals more warps, which shortens a block's way from its loads to its stores (8704 x 3072 to int8: 63 us on 12 warps
-// a row, 67 on 8).
+// Among equals the gated add takes more warps, whose barriers it waits for while the next row is on its way (8704 x 3072 to
+// int8: 63 us on 12 warps a row, 67 on 8), and plain quantising fewer (8192 x 3072: 15.5 us on 3 warps a row, 21 on 6 or 12).
 struct Deal {
     int nc, warps;
 };
-Deal deal(int chunks, int most)
+Deal deal(int chunks, int most, bool few_warps)
 {
     Deal best{0, 0};
     for (int nc = 1; nc <= most; ++nc) {
         const int warps = (chunks + nc - 1) / nc;
-        if (warps <= 16 && (!best.nc || warps * nc < best.warps * best.nc))
+        const int more = best.nc ? warps * nc - best.warps * best.nc : -1;
+        if (warps <= 16 && (more < 0 || (more == 0 && few_warps)))
             best = Deal{nc, warps};
     }
     return best;
@@ -538,7 +539,7 @@ cudaError_t gate_norm(const GateNormArgs& args, cudaStream_t st)
     cudaError_t e;
     if (vec) {
         const int chunks = (a.n + 127) / 128;
-        const Deal d = deal(chunks, chunks <= 48 ? 3 : 6);
+        const Deal d = deal(chunks, chunks <= 48 ? 3 : 6, false);
         e = d.nc == 1   ? launch_gate_norm<4, 1, true>(a, d.warps, st)
             : d.nc == 2 ? launch_gate_norm<4, 2, true>(a, d.warps, st)
             : d.nc == 3 ? launch_gate_norm<4, 3, true>(a, d.warps, st)
@@ -579,7 +580,7 @@ cudaError_t quantize_rows(const QuantRowsArgs& a, cudaStream_t st)
             e = chunks <= 128 ? launch_quant<__nv_bfloat16, 1, 8>(a, (chunks + 7) / 8, st)
                               : launch_quant<__nv_bfloat16, 1, 32>(a, (chunks + 31) / 32, st);
     } else if (a.x_f32) {
-        const Deal d = deal(chunks, chunks <= 64 ? 4 : 8);
+        const Deal d = deal(chunks, chunks <= 64 ? 4 : 8, true);
         e = d.nc == 1   ? launch_quant<float, 4, 1>(a, d.warps, st)
             : d.nc == 2 ? launch_quant<float, 4, 2>(a, d.warps, st)
             : d.nc == 3 ? launch_quant<float, 4, 3>(a, d.warps, st)
@@ -587,7 +588,7 @@ cudaError_t quantize_rows(const QuantRowsArgs& a, cudaStream_t st)
             : d.nc <= 6 ? launch_quant<float, 4, 6>(a, (chunks + 5) / 6, st)
                         : launch_quant<float, 4, 8>(a, (chunks + 7) / 8, st);
     } else {
-        const Deal d = deal(chunks, 4);
+        const Deal d = deal(chunks, 4, true);
         e = d.nc == 1   ? launch_quant<__nv_bfloat16, 8, 1>(a, d.warps, st)
             : d.nc == 2 ? launch_quant<__nv_bfloat16, 8, 2>(a, d.warps, st)
             : d.nc == 3 ? launch_quant<__nv_bfloat16, 8, 3>(a, d.warps, st)

@@ -1,8 +1,9 @@
 // The 8-bit integer projection (see gemm_i8.cuh): three kernels for three ranges of rows.
-//   k_i8_rows   up to 8 rows: the weights stream through the CUDA cores once (dp4a); HBM is the bound.
-//   k_i8_split  few output tiles: 128 x BN tiles on one SM each, the K axis cut over a cluster whose CTAs add their
-//               integer sums through distributed shared memory; latency is the bound.
-//   k_i8_pair   the rest: persistent 256 x BN tiles on CTA pairs (cta_group::2), the tensor pipe is the bound.
+//   k_i8_rows    one or two rows: the weights stream through the CUDA cores once (dp4a); HBM is the bound.
+//   k_i8_few     up to 256 rows: 128 rows of W are the MMA's M and the tokens its N (16 to 128), so that a stage is almost
+//                all weights and the outputs' columns lie along the lanes; K is cut over a cluster whose CTAs add their
+//                integer sums through distributed shared memory. Bound by HBM for wide W, else by latency.
+//   k_i8_pair    the rest: persistent 256 x BN tiles on CTA pairs (cta_group::2), the tensor pipe is the bound.
 // The sums are exact integers, so a row's result is the same bits whichever kernel and split computes it.
 #include "gemm_i8.cuh"
 #include "common.cuh"
@@ -123,7 +124,7 @@ __device__ __forceinline__ void store_row(const GemmI8Args& a, long row, int col
 
 // ------------------------------------------------------------------------------------------------ few rows
 
-constexpr int kRowsMax = 8;
+constexpr int kRowsMax = 2, kFewMax = 256;
 
 // MR rows of x against R rows of W a warp (WK = 1), or against R rows of W a block whose 8 warps share the K axis (WK =
 // 8, for matrices with too few rows of W to fill the GPU otherwise). Lanes take 16 bytes of K each.
@@ -218,21 +219,27 @@ __global__ void __launch_bounds__(256) k_i8_rows(const GemmI8Args a)
 struct I8Params {
     CUtensorMap tx, tw, ty;
     GemmI8Args a;
-    int splits;   // k_i8_split: CTAs of a cluster, each a part of K
+    int splits;   // k_i8_few: CTAs of a cluster, each a part of K
     int boxes;    // k_i8_pair: outputs leave as TMA boxes
 };
 
 template <int BN>
-struct SplitCfg {
-    static constexpr int kABytes = 128 * kBK, kBBytes = BN * kBK, kStageBytes = kABytes + kBBytes;
-    static constexpr int kStages = BN == 64 ? 8 : 6;
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + 2 * BN * 4 + 256;
+struct FewCfg {
+    static constexpr int kWBytes = 128 * kBK, kXBytes = BN * kBK, kStageBytes = kWBytes + kXBytes;
+    static constexpr int kStages = (200 * 1024) / kStageBytes;
+    static constexpr int kTmemCols = BN < 32 ? 32 : BN;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + BN * 4 + 256;
     static_assert(kSmem <= 227 * 1024);
     static_assert(kStages * kStageBytes >= 128 * BN * 4, "the partial sums reuse the stages");
 };
 
-// Columns [c0, c0 + 8) of this warp's rows.
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8])
+// Two (or eight) consecutive columns of this warp's lanes.
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[2])
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(taddr) : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[8])
 {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
@@ -245,17 +252,19 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v)
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-// One 128 x BN tile a cluster (blockIdx.x = tile * splits + part), K cut into `splits` runs of whole stages. After the
-// main loop CTA p holds the sums of its run; it hands columns [o * BN / splits, ...) to CTA o's shared memory for every
-// other o, and finishes its own columns with what the others brought.
+// One tile of 128 output columns x BN tokens a cluster (blockIdx.x = tile * splits + part), K cut into `splits` runs of whole
+// stages. Accumulator lane n holds output column n, its columns the tokens. After the main loop CTA p holds the sums of its
+// run; it hands the tokens [o * BN / splits, ...) to CTA o's shared memory for every other o, and finishes its own tokens with
+// what the others brought. The epilogue is written small: a launch runs it once or twice, and long straight code costs more
+// in instruction misses (7 us for 32 unrolled columns) than it saves.
 template <int BN>
-__global__ void __launch_bounds__(192, 1) k_i8_split(const __grid_constant__ I8Params P)
+__global__ void __launch_bounds__(192, 1) k_i8_few(const __grid_constant__ I8Params P)
 {
-    using C = SplitCfg<BN>;
+    using C = FewCfg<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float* vec = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);  // [w_scale, bias][BN]
-    uint64_t* full = reinterpret_cast<uint64_t*>(vec + 2 * BN);
+    float* sx = reinterpret_cast<float*>(smem + C::kStages * C::kStageBytes);  // [BN] the tokens' scales
+    uint64_t* full = reinterpret_cast<uint64_t*>(sx + BN);
     uint64_t* empty = full + C::kStages;
     uint64_t* acc_full = empty + C::kStages;
     uint64_t* drain = acc_full + 1;
@@ -264,7 +273,7 @@ __global__ void __launch_bounds__(192, 1) k_i8_split(const __grid_constant__ I8P
     const GemmI8Args& a = P.a;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int S = P.splits, part = S > 1 ? int(cluster_ctarank()) : 0, tile = blockIdx.x / S;
-    const int num_n = (a.N + BN - 1) / BN, mb = tile / num_n, nb = tile % num_n;
+    const int num_m = (a.M + BN - 1) / BN, mb = tile % num_m, nb = tile / num_m;
     const int num_k = (a.K + kBK - 1) / kBK, k_lo = int(long(num_k) * part / S), k_hi = int(long(num_k) * (part + 1) / S);
 
     if (threadIdx.x == 0) {
@@ -283,7 +292,7 @@ __global__ void __launch_bounds__(192, 1) k_i8_split(const __grid_constant__ I8P
     }
     grid_dep_wait();  // before TMEM allocation and the first global access
     if (warp == 1) {
-        tmem_alloc(tmem_slot, BN);
+        tmem_alloc(tmem_slot, C::kTmemCols);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -291,6 +300,8 @@ __global__ void __launch_bounds__(192, 1) k_i8_split(const __grid_constant__ I8P
     tc_fence_after();
     grid_dep_launch();
     const uint32_t tmem = *tmem_slot;
+    const int n = nb * 128 + (warp & 3) * 32 + lane;  // this epilogue thread's output column
+    float sw = 0.0f, bias = 0.0f;
     bool ok = true;
     if (warp == 0) {
         if (lane == 0) {
@@ -301,10 +312,10 @@ __global__ void __launch_bounds__(192, 1) k_i8_split(const __grid_constant__ I8P
                     ok = false;
                     break;
                 }
-                uint8_t* sa = smem + s * C::kStageBytes;
+                uint8_t* st = smem + s * C::kStageBytes;
                 mbar_arrive_expect_tx(&full[s], C::kStageBytes);
-                tma_load_2d(sa, &P.tx, &full[s], kb * kBK, mb * 128);
-                tma_load_2d(sa + C::kABytes, &P.tw, &full[s], kb * kBK, nb * BN);
+                tma_load_2d(st, &P.tw, &full[s], kb * kBK, nb * 128);
+                tma_load_2d(st + C::kWBytes, &P.tx, &full[s], kb * kBK, mb * BN);
             }
             if (!ok)  // let the loads already issued land before the CTA can exit
                 for (int j = std::max(0, it - C::kStages); j < it; ++j)
@@ -322,12 +333,12 @@ __global__ void __launch_bounds__(192, 1) k_i8_split(const __grid_constant__ I8P
                 break;
             }
             tc_fence_after();
-            const uint64_t da = desc_kmajor_sw128(smem_u32(smem + s * C::kStageBytes)),
-                           db = desc_kmajor_sw128(smem_u32(smem + s * C::kStageBytes + C::kABytes));
+            const uint64_t dw = desc_kmajor_sw128(smem_u32(smem + s * C::kStageBytes)),
+                           dx = desc_kmajor_sw128(smem_u32(smem + s * C::kStageBytes + C::kWBytes));
             if (elect_one_sync()) {
 #pragma unroll
                 for (int k = 0; k < kBK / 32; ++k)  // 32 bytes are 2 units of a descriptor's address
-                    mma_i8_ss(tmem, da + 2 * k, db + 2 * k, idesc, (it | k) != 0);
+                    mma_i8_ss(tmem, dw + 2 * k, dx + 2 * k, idesc, (it | k) != 0);
                 mma_commit(&empty[s]);
             }
             __syncwarp();
@@ -340,81 +351,95 @@ __global__ void __launch_bounds__(192, 1) k_i8_split(const __grid_constant__ I8P
         __syncwarp();
         mbar_wait(drain, 0, a.status, kErrWaitDrain, nullptr);
     } else {
-        const int et = int(threadIdx.x) - 64;
-        for (int i = et; i < BN; i += 128) {  // while the main loop runs
-            const bool in = nb * BN + i < a.N;
-            vec[i] = in ? __ldg(a.w_scale + nb * BN + i) : 0.0f;
-            vec[BN + i] = in && a.bias ? __ldg(a.bias + nb * BN + i) : 0.0f;
+        // While the main loop runs: the tokens' scales, this thread's column's scale and bias.
+        for (int i = int(threadIdx.x) - 64; i < BN; i += 128)
+            sx[i] = mb * BN + i < a.M ? __ldg(a.x_scale + mb * BN + i) : 0.0f;
+        if (n < a.N) {
+            sw = __ldg(a.w_scale + n);
+            bias = a.bias ? __ldg(a.bias + n) : 0.0f;
         }
         named_barrier_sync<1, 128>();
         ok = mbar_wait(acc_full, 0, a.status, kErrWaitAccFull, abort_flag);
         tc_fence_after();
     }
     __syncwarp();
-    const int q = warp & 3, r = q * 32 + lane;
-    const uint32_t t_row = tmem + (uint32_t(q * 32) << 16);
-    const int cols = BN / S;  // of this CTA, a multiple of 8
-    int* sums = reinterpret_cast<int*>(smem);  // [splits - 1][cols][128]
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t t_lane = tmem + (uint32_t((warp & 3) * 32) << 16);
+    const int mine = BN / S;  // tokens of this CTA, two at least
+    int* sums = reinterpret_cast<int*>(smem);  // [splits - 1][mine][128]
     if (S > 1) {
         __syncthreads();  // the producer and the MMA warp are past their last use of the stages
         cluster_sync_all();
         if (warp >= 2 && ok)
+#pragma unroll 1
             for (int o = 0; o < S; ++o) {
                 if (o == part)
                     continue;
-                const uint32_t slot = uint32_t(part < o ? part : part - 1);
-                const uint32_t dst = map_to_cta(smem_u32(sums) + (slot * cols * 128 + r) * 4, o);
-                for (int c = 0; c < cols; c += 8) {
-                    uint32_t v[8];
-                    tmem_ld8(t_row + o * cols + c, v);
+                const uint32_t dst = map_to_cta(smem_u32(sums) + ((part < o ? part : part - 1) * mine * 128 + r) * 4, o);
+                const auto send = [&](auto width, int c) {
+                    constexpr int W = decltype(width)::value;
+                    uint32_t v[W];
+                    tmem_ld(t_lane + o * mine + c, v);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
+                    for (int j = 0; j < W; ++j)
                         st_cluster(dst + (c + j) * 512, v[j]);
+                };
+                const int want = min(mine, a.M - mb * BN - o * mine);  // tokens that exist
+                if (mine >= 8) {
+#pragma unroll 1
+                    for (int c = 0; c < want; c += 8)
+                        send(std::integral_constant<int, 8>{}, c);
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < want; c += 2)
+                        send(std::integral_constant<int, 2>{}, c);
                 }
             }
         cluster_sync_all();
     }
     if (warp >= 2 && ok) {
-        const long row = long(mb) * 128 + r;
-        const float sx = row < a.M ? __ldg(a.x_scale + row) : 0.0f;
-        // W columns from tile column c on: this CTA's sum, the other parts' sums, the epilogue.
+        const int m0 = mb * BN + part * mine;
         const auto finish = [&](auto width, int c) {
             constexpr int W = decltype(width)::value;
-            const int tc = part * cols + c, col = nb * BN + tc;
-            uint32_t t[W];
-            if constexpr (W == 32)
-                tmem_ld32(t_row + tc, t);
-            else
-                tmem_ld8(t_row + tc, t);
+            uint32_t s[W];
+            tmem_ld(t_lane + part * mine + c, s);
             tmem_wait_ld();
+#pragma unroll 1
+            for (int o = 0; o < S - 1; ++o)
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    s[j] += uint32_t(sums[(o * mine + c + j) * 128 + r]);
             float v[W];
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                int s = int(t[j]);
-                for (int o = 0; o < S - 1; ++o)
-                    s += sums[(o * cols + c + j) * 128 + r];
-                v[j] = fmaf(float(s) * sx, vec[tc + j], vec[BN + tc + j]);
-            }
+            for (int j = 0; j < W; ++j)
+                v[j] = fmaf(float(int(s[j])) * sx[part * mine + c + j], sw, bias);
             act_out(v, a.act, a.out_f32);
-            if (row < a.M)
-                store_row(a, row, col, v);
+            if (n < a.N)
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+                    if (m0 + c + j < a.M) {
+                        if (a.out_f32)
+                            static_cast<float*>(a.y)[long(m0 + c + j) * a.ldy + n] = v[j];
+                        else
+                            static_cast<__nv_bfloat16*>(a.y)[long(m0 + c + j) * a.ldy + n] = __float2bfloat16(v[j]);
+                    }
         };
-        for (int c = 0; c < cols && nb * BN + part * cols + c < a.N;) {
-            if (cols - c >= 32) {
-                finish(std::integral_constant<int, 32>{}, c);
-                c += 32;
-            } else {
+        if (mine >= 8) {
+#pragma unroll 1
+            for (int c = 0; c < mine && m0 + c < a.M; c += 8)
                 finish(std::integral_constant<int, 8>{}, c);
-                c += 8;
-            }
+        } else {
+#pragma unroll 1
+            for (int c = 0; c < mine && m0 + c < a.M; c += 2)
+                finish(std::integral_constant<int, 2>{}, c);
         }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, BN);
+        tmem_dealloc(tmem, C::kTmemCols);
     }
 }
 
@@ -693,13 +718,18 @@ cudaError_t launch_rows(const GemmI8Args& a, cudaStream_t st)
 }
 
 template <int BN>
-cudaError_t launch_split(const I8Params& P, int tiles, cudaStream_t st)
+cudaError_t launch_few(I8Params& P, cudaStream_t st)
 {
     static std::atomic<uint64_t> devs{0};
-    const cudaError_t e = smem_limit_once(devs, k_i8_split<BN>, SplitCfg<BN>::kSmem);
+    const cudaError_t e = smem_limit_once(devs, k_i8_few<BN>, FewCfg<BN>::kSmem);
     if (e != cudaSuccess)
         return e;
-    return launch_k_cluster(k_i8_split<BN>, dim3(unsigned(tiles) * P.splits), P.splits, 192, SplitCfg<BN>::kSmem, st, P);
+    // K over as many CTAs as the SMs allow, two stages a part or more.
+    const int tiles = (P.a.M + BN - 1) / BN * ((P.a.N + 127) / 128), num_k = (P.a.K + kBK - 1) / kBK;
+    P.splits = 1;
+    while (P.splits < 8 && tiles * P.splits * 2 <= num_sms() && num_k >= 4 * P.splits)
+        P.splits *= 2;
+    return launch_k_cluster(k_i8_few<BN>, dim3(unsigned(tiles) * P.splits), P.splits, 192, FewCfg<BN>::kSmem, st, P);
 }
 
 template <int BN>
@@ -720,35 +750,28 @@ cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
     cudaError_t e;
     if (a.M <= kRowsMax) {
         e = a.M == 1   ? launch_rows<1>(a, st)
-            : a.M == 2 ? launch_rows<2>(a, st)
-            : a.M <= 4 ? launch_rows<4>(a, st)
-                       : launch_rows<8>(a, st);
+                       : launch_rows<2>(a, st);
     } else {
         I8Params P{};
         P.a = a;
-        const long sms = num_sms(), num_k = (a.K + kBK - 1) / kBK;
-        const auto tiles = [&](int rows, int bn) { return ((a.M + rows - 1L) / rows) * ((a.N + bn - 1L) / bn); };
-        // Single-SM tiles when they fit one round (or one row of tiles is all there is), cut along K as far as the SMs and whole stages allow (at least four
-        // stages a part: below that the exchange of the sums costs more than the loads it saves).
-        const bool split = tiles(128, 64) <= sms || a.M <= 128;
-        const int sbn = tiles(128, 64) <= sms ? 64 : 128;
-        if (split) {
-            P.splits = 1;
-            while (P.splits < 8 && tiles(128, sbn) * P.splits * 2 <= sms && num_k >= 8 * P.splits)
-                P.splits *= 2;
-        }
-        // Pair tiles of 256 or 128 columns: whichever has the shorter last-round cost.
-        const long slots = sms / 2;
-        const int pbn = (tiles(256, 256) + slots - 1) / slots * 2 <= (tiles(256, 128) + slots - 1) / slots ? 256 : 128;
-        const int rows = 128, cols = split ? sbn : pbn / 2;
+        const bool few = a.M <= kFewMax;
+        const int few_bn = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+        // Pair tiles of 256 or 128 columns: whichever has the shorter rounds, 256 among equals (half the shared-memory traffic
+        // of x a product: 512 x 9216 x 3072 in one round of 256 15.0 us, in two of 128 17.3).
+        const long slots = num_sms() / 2;
+        const auto rounds = [&](int bn) { return (((a.M + 255L) / 256) * ((a.N + bn - 1L) / bn) + slots - 1) / slots; };
+        const int bn = rounds(256) * 2 <= rounds(128) ? 256 : 128;
         const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-        if (!encode_2d(&P.tx, u8, a.x, a.K, a.M, a.ldx, kBK, rows) ||
-            !encode_2d(&P.tw, u8, a.w, a.K, a.N, a.ldw, kBK, cols)) {
+        if (!encode_2d(&P.tx, u8, a.x, a.K, a.M, a.ldx, kBK, few ? few_bn : 128) ||
+            !encode_2d(&P.tw, u8, a.w, a.K, a.N, a.ldw, kBK, few ? 128 : bn / 2)) {
             *err = "proj_i8: tensor map encoding failed";
             return cudaErrorInvalidValue;
         }
-        if (split) {
-            e = sbn == 64 ? launch_split<64>(P, int(tiles(128, 64)), st) : launch_split<128>(P, int(tiles(128, 128)), st);
+        if (few) {
+            e = few_bn == 16   ? launch_few<16>(P, st)
+                : few_bn == 32 ? launch_few<32>(P, st)
+                : few_bn == 64 ? launch_few<64>(P, st)
+                               : launch_few<128>(P, st);
         } else {
             const int size = a.out_f32 ? 4 : 2;
             P.boxes = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.ldy * size) % 16 == 0;
@@ -757,7 +780,8 @@ cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
                 *err = "proj_i8: tensor map encoding failed";
                 return cudaErrorInvalidValue;
             }
-            e = pbn == 256 ? launch_pair<256>(P, int(tiles(256, 256)), st) : launch_pair<128>(P, int(tiles(256, 128)), st);
+            const int tiles = (a.M + 255) / 256 * ((a.N + bn - 1) / bn);
+            e = bn == 256 ? launch_pair<256>(P, tiles, st) : launch_pair<128>(P, tiles, st);
         }
     }
     if (e != cudaSuccess)
