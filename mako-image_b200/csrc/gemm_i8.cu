@@ -1,8 +1,8 @@
 // The 8-bit integer projection (see gemm_i8.cuh): three kernels for three ranges of rows.
 //   k_i8_rows    one or two rows: the weights stream through the CUDA cores once (dp4a); HBM is the bound.
-//   k_i8_few     up to 256 rows: 128 rows of W are the MMA's M and the tokens its N (16 to 128), so that a stage is almost
-//                all weights and the outputs' columns lie along the lanes; K is cut over a cluster whose CTAs add their
-//                integer sums through distributed shared memory. Bound by HBM for wide W, else by latency.
+//   k_i8_few     few rows: 128 rows of W are the MMA's M and the tokens its N (16 to 64), so that a stage is mostly weights
+//                and the outputs' columns lie along the lanes; K is cut over a cluster whose CTAs add their integer sums
+//                through distributed shared memory. Bound by HBM for wide W, else by latency.
 //   k_i8_pair    the rest: persistent 256 x BN tiles on CTA pairs (cta_group::2), the tensor pipe is the bound.
 // The sums are exact integers, so a row's result is the same bits whichever kernel and split computes it.
 #include "gemm_i8.cuh"
@@ -124,7 +124,7 @@ __device__ __forceinline__ void store_row(const GemmI8Args& a, long row, int col
 
 // ------------------------------------------------------------------------------------------------ few rows
 
-constexpr int kRowsMax = 2, kFewMax = 256;
+constexpr int kRowsMax = 2;
 
 // MR rows of x against R rows of W a warp (WK = 1), or against R rows of W a block whose 8 warps share the K axis (WK =
 // 8, for matrices with too few rows of W to fill the GPU otherwise). Lanes take 16 bytes of K each.
@@ -754,8 +754,13 @@ cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
     } else {
         I8Params P{};
         P.a = a;
-        const bool few = a.M <= kFewMax;
-        const int few_bn = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+        // k_i8_few's tokens a tile: the fewest that leave no more than a tile for each SM (W comes out of L2 again for each
+        // tile, but K is cut less and an epilogue is short). Where that takes more than 32 of them, over 64 rows, the pair
+        // kernel is faster: 256 x 3072 x 3072 12.6 against 10.6 us; 128 rows 9.9 against 10.3, 77 x 1280 x 1280 4.7 against 6.8.
+        int few_bn = 16;
+        while (few_bn < 64 && (a.M + few_bn - 1L) / few_bn * ((a.N + 127L) / 128) > num_sms())
+            few_bn *= 2;
+        const bool few = a.M <= 64 || few_bn <= 32;
         // Pair tiles of 256 or 128 columns: whichever has the shorter rounds, 256 among equals (half the shared-memory traffic
         // of x a product: 512 x 9216 x 3072 in one round of 256 15.0 us, in two of 128 17.3).
         const long slots = num_sms() / 2;
@@ -770,8 +775,7 @@ cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
         if (few) {
             e = few_bn == 16   ? launch_few<16>(P, st)
                 : few_bn == 32 ? launch_few<32>(P, st)
-                : few_bn == 64 ? launch_few<64>(P, st)
-                               : launch_few<128>(P, st);
+                               : launch_few<64>(P, st);
         } else {
             const int size = a.out_f32 ? 4 : 2;
             P.boxes = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.ldy * size) % 16 == 0;
