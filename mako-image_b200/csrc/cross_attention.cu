@@ -715,9 +715,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
 
 // ------------------------------------------------------------------------------------------------ few query rows
 
-constexpr int kFewRows = 8;    // query rows that share a key head
+constexpr int kFewRows = 4;    // query rows that share a key head
 constexpr int kFewWarps = 8;
-constexpr int kFewDepth = 4;   // K and V rows a lane has in flight, each
+// K and V rows a lane takes a round, each, and the rounds in flight: 64 KB a CTA, three CTAs an SM (96 KB: 27 against 22 us at
+// 2 x 24 heads of 128 over 4096 keys). Several query rows leave registers for two rows a round (two rows: 23 against 29 us).
+template <int R>
+struct FewCfg {
+    static constexpr int kDepth = R == 1 ? 4 : 2, kRounds = 8 / kDepth;
+};
+constexpr int kFewSmem = kFewWarps * 8 * 2 * 32 * 16;  // a warp's rounds: [round][K, V][depth][lane] of 16 bytes
+
+// 16 bytes to shared memory behind the thread's back; zeros where `on` is false (nothing is read).
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool on)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0)
+                 : "memory");
+}
 
 __device__ __forceinline__ void unpack8(uint4 u, float (&f)[8])
 {
@@ -731,12 +744,14 @@ __device__ __forceinline__ void unpack8(uint4 u, float (&f)[8])
 
 // A few query rows of the heads that share a key head: with so few, K and V pass the CUDA cores once and HBM is the bound. A
 // cluster takes one (sample, key head), each CTA a run of its keys; D / 8 lanes take a key, 8 values each, so that a warp's
-// load is whole rows. Each warp keeps its own running maximum, sum and outputs; the warps' parts meet in shared memory, the
-// CTAs' in the first CTA's.
+// load is whole rows. Each lane copies what it will use itself into shared memory ahead of its use (in registers alone too
+// little is in flight where there are few CTAs: 28 against 17 us at 8 heads of 128 over 8192 keys). Each warp keeps its own
+// running maximum, sum and outputs; the warps' parts meet in shared memory, the CTAs' in the first CTA's.
 template <int D, int R>
 __global__ void __launch_bounds__(32 * kFewWarps) k_cross_few(const CrossArgs a, int splits)
 {
     constexpr int kLanes = D / 8, kKeys = 32 / kLanes;  // lanes a key, keys a load
+    constexpr int kFewDepth = FewCfg<R>::kDepth, kFewRounds = FewCfg<R>::kRounds;
     __shared__ float po[kFewWarps][R][D];
     __shared__ float pm[kFewWarps][R], pl[kFewWarps][R];
     grid_dep_wait();
@@ -765,19 +780,59 @@ __global__ void __launch_bounds__(32 * kFewWarps) k_cross_few(const CrossArgs a,
     const __nv_bfloat16* kb = a.k + b * a.sk.sample + hk * a.sk.head + dim;
     const __nv_bfloat16* vb = a.v + b * a.sv.sample + hk * a.sv.head + dim;
     const uint8_t* mask = a.key_mask ? a.key_mask + b * a.mask_stride : nullptr;
-    for (int j0 = lo + warp * kKeys; j0 < hi; j0 += kFewWarps * kKeys * kFewDepth) {
+    extern __shared__ __align__(16) uint4 few_ring[];
+    uint4* ring = few_ring + warp * (kFewRounds * 2 * kFewDepth * 32) + lane;
+    constexpr int kRound = kFewWarps * kKeys * kFewDepth;  // keys a round of the CTA
+    const int first = lo + warp * kKeys + lane / kLanes;   // this lane's first key
+    // Which of a round's keys are visible, a bit each.
+    const auto look = [&](int j0) {
+        uint32_t see = 0;
+#pragma unroll
+        for (int u = 0; u < kFewDepth; ++u) {
+            const int j = j0 + u * kFewWarps * kKeys;
+            if (j < hi && (!mask || __ldg(mask + j) != 0))
+                see |= 1u << u;
+        }
+        return see;
+    };
+    const auto fetch = [&](int slot, int j0, uint32_t see) {
+        uint4* dst = ring + slot * (2 * kFewDepth * 32);
+#pragma unroll
+        for (int u = 0; u < kFewDepth; ++u) {
+            const bool on = (see >> u) & 1;
+            const long j = on ? j0 + u * kFewWarps * kKeys : 0;
+            copy16(dst + u * 32, kb + j * a.sk.row, on);
+            copy16(dst + (kFewDepth + u) * 32, vb + j * a.sv.row, on);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // sees: the rounds in flight, four bits each, the next to come lowest; ahead: of the round to be fetched next, looked up
+    // a round early.
+    uint32_t sees = 0;
+#pragma unroll
+    for (int i = 0; i < kFewRounds - 1; ++i) {
+        const uint32_t see = look(first + i * kRound);
+        sees |= see << (4 * i);
+        fetch(i, first + i * kRound, see);
+    }
+    uint32_t ahead = look(first + (kFewRounds - 1) * kRound);
+    int slot = 0;
+    for (int j0 = first; j0 - lane / kLanes < hi; j0 += kRound) {
+        const int next = j0 + (kFewRounds - 1) * kRound;
+        fetch(slot == 0 ? kFewRounds - 1 : slot - 1, next, ahead);
+        sees |= ahead << (4 * (kFewRounds - 1));
+        ahead = look(next + kRound);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kFewRounds - 1) : "memory");
         uint4 ku[kFewDepth], vu[kFewDepth];
         bool see[kFewDepth];
 #pragma unroll
         for (int u = 0; u < kFewDepth; ++u) {
-            const int j = j0 + u * kFewWarps * kKeys + lane / kLanes;
-            see[u] = j < hi && (!mask || __ldg(mask + j) != 0);
-            ku[u] = vu[u] = make_uint4(0, 0, 0, 0);  // a hidden key is not read
-            if (see[u]) {
-                ku[u] = __ldg(reinterpret_cast<const uint4*>(kb + j * a.sk.row));
-                vu[u] = __ldg(reinterpret_cast<const uint4*>(vb + j * a.sv.row));
-            }
+            see[u] = (sees >> u) & 1;
+            ku[u] = ring[(slot * 2 * kFewDepth + u) * 32];
+            vu[u] = ring[(slot * 2 * kFewDepth + kFewDepth + u) * 32];
         }
+        sees >>= 4;
+        slot = slot == kFewRounds - 1 ? 0 : slot + 1;
         float s[kFewDepth][R];
 #pragma unroll
         for (int u = 0; u < kFewDepth; ++u) {
@@ -983,10 +1038,15 @@ cudaError_t launch(const CrossParams& P, cudaStream_t st)
 template <int D, int R>
 cudaError_t launch_few(const CrossArgs& a, cudaStream_t st)
 {
-    // Keys over as many CTAs as keep four on each SM, 128 keys each or more.
+    // The keys over as many CTAs as leave four for each SM, 128 keys each or more (the size that divides the CTAs most evenly
+    // over the SMs instead, 6 for 8 at 48 key heads, was slower: 23.6 against 22.4 us).
     const int pairs = a.B * a.Hkv;
     const int splits = std::max(1, std::min({kMaxSplits, kFewWarps, 4 * num_sms() / pairs, a.Lk / 128}));
-    return launch_k_cluster(k_cross_few<D, R>, dim3(pairs * splits), splits, 32 * kFewWarps, 0, st, a, splits);
+    static std::atomic<uint64_t> devs{0};
+    const cudaError_t e = smem_limit_once(devs, k_cross_few<D, R>, kFewSmem);
+    if (e != cudaSuccess)
+        return e;
+    return launch_k_cluster(k_cross_few<D, R>, dim3(pairs * splits), splits, 32 * kFewWarps, kFewSmem, st, a, splits);
 }
 
 template <int D>
@@ -995,8 +1055,7 @@ cudaError_t launch_few(const CrossArgs& a, cudaStream_t st)
     const int rows = a.H / a.Hkv * a.Lq;
     return rows == 1   ? launch_few<D, 1>(a, st)
            : rows == 2 ? launch_few<D, 2>(a, st)
-           : rows <= 4 ? launch_few<D, 4>(a, st)
-                       : launch_few<D, 8>(a, st);
+                       : launch_few<D, 4>(a, st);
 }
 
 }  // namespace
