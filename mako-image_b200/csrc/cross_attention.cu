@@ -13,7 +13,8 @@
 //              staged in the Q tile that made them and leave as TMA stores (a thread storing its row directly touches 32
 //              lines an instruction)
 // Where the items leave most of the GPU idle and the keys are many, SPLIT runs one item a cluster, whose CTAs take a run of
-// the key steps each and put the parts together through distributed shared memory: no workspace, no second launch.
+// the key steps each and put the parts together through distributed shared memory: no workspace, no second launch. An item of a
+// single query tile gives it to both softmax groups there, who take the steps in turn as two parts.
 // Only ceil(visible / 16) * 16 keys of the last tile are multiplied and exponentiated (77 keys cost 80, not 128).
 // TMEM columns: S_A [0, 128), S_B [128, 256), O_A [256, 384), O_B [384, 512); P takes the first half of its S.
 #include "cross_attention.cuh"
@@ -396,9 +397,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             constexpr std::integral_constant<int, 0> kA;
             constexpr std::integral_constant<int, 1> kB;
             // S_t = Q_t K^T; Q is waited for at an item's first step.
-            const auto scores = [&](auto tile, bool first, bool last, uint64_t dk, uint32_t idesc) {
+            const auto scores = [&](auto tile, bool first, bool last, uint64_t dk, uint32_t idesc, bool shared_q = false) {
                 constexpr int t = decltype(tile)::value;
-                const uint32_t qi = QB * t + nq[t] % QB;
+                const uint32_t qi = shared_q ? 0 : QB * t + nq[t] % QB;
                 const uint64_t dq = dq0 + qi * kUnit;
                 if (first && !wait(&q_full[qi], nq[t] / QB))
                     return false;
@@ -436,6 +437,38 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             };
             Walk<SPLIT> w, x;
             w.first(P);
+            if (SPLIT && w.more(P) && w.it.tiles == 1) {
+                // One query tile: step g, of tile g % 2, is S_t as soon as its P of two steps before is spent.
+                const int steps = w.it.hi - w.it.lo;
+                const auto width = [&](int g) { return min(kTile, (w.it.n - (w.it.lo + g) * kTile + 15) & ~15); };
+                const auto free_slot = [&](uint64_t* bar) {
+                    if (elect_one_sync())
+                        mma_commit(bar);
+                    __syncwarp();
+                };
+                const auto score = [&](auto tile, int g) {
+                    const uint32_t s = 2 * g % NS;
+                    if (!wait(&k_full[g % kSteps], g / kSteps) ||
+                        !scores(tile, g < 2, false, dk0 + s * kUnit, idesc_s0 | uint32_t(width(g) >> 3) << 17, true))
+                        return false;
+                    free_slot(&kv_empty[s]);
+                    return true;
+                };
+                const auto output = [&](auto tile, int g) {
+                    const uint32_t s = (2 * g + 1) % NS;
+                    if (!wait(&v_full[g % kSteps], g / kSteps) ||
+                        !outputs(tile, g < 2, g + 2 >= steps, dv0 + s * kUnit, width(g)))
+                        return false;
+                    free_slot(&kv_empty[s]);
+                    if (a.key_mask)
+                        free_slot(&h_empty[g % kHideSteps]);
+                    return g + 2 >= steps || score(tile, g + 2);
+                };
+                ok = score(kA, 0) && (steps < 2 || score(kB, 1));
+                for (int g = 0; g < steps && ok; g += 2)
+                    ok = output(kA, g) && (g + 1 >= steps || output(kB, g + 1));
+                w.it.item = P.items;  // done
+            }
             if (w.more(P)) {
                 const uint32_t idesc = idesc_s0 | uint32_t(w.width() >> 3) << 17;
                 ok = wait(&k_full[0], 0) && scores(kA, true, w.last(), dk0, idesc) &&
@@ -515,11 +548,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
         for (; it.more(P) && ok; it = nx) {
             nx = it;
             nx.next(P);
-            if (t >= it.tiles) {
+            const bool both = SPLIT && it.tiles == 1;  // both groups on one tile, its steps in turn
+            if (t >= it.tiles && !both) {
                 step += it.hi - it.lo;
                 continue;
             }
-            const int row0 = it.q0() + t * kTile + w32;  // of the warp
+            const int row0 = it.q0() + (both ? 0 : t * kTile) + w32;  // of the warp
+            if (both)
+                step = t;
             if (it.n == 0) {  // no keys: zeros, a row's 16-byte pieces side by side
                 constexpr int per = D / 8;
                 for (int i = lane; i < 32 * per; i += 32) {
@@ -531,7 +567,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 continue;
             }
             float m = -INFINITY, l = 0.0f;
-            for (int j = it.lo; j < it.hi; ++j, ++step) {
+            const int stride = both ? 2 : 1, begin = it.lo + (both ? t : 0);
+            for (int j = begin; j < it.hi; j += stride, step += stride) {
                 if (!mbar_wait(&s_full[t], ns & 1, a.status, kErrAttnWait, abort_flag)) {
                     ok = false;
                     break;
@@ -552,10 +589,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                     tail = 32;  // the bounds know of it
                 }
                 switch (min(4, (valid + 31) >> 5)) {
-                case 1: softmax_step<D, 1>(ts, to, tail, masked, bound, a.scale_log2, j == it.lo, m, l); break;
-                case 2: softmax_step<D, 2>(ts, to, tail, masked, bound, a.scale_log2, j == it.lo, m, l); break;
-                case 3: softmax_step<D, 3>(ts, to, tail, masked, bound, a.scale_log2, j == it.lo, m, l); break;
-                default: softmax_step<D, 4>(ts, to, tail, masked, bound, a.scale_log2, j == it.lo, m, l); break;
+                case 1: softmax_step<D, 1>(ts, to, tail, masked, bound, a.scale_log2, j == begin, m, l); break;
+                case 2: softmax_step<D, 2>(ts, to, tail, masked, bound, a.scale_log2, j == begin, m, l); break;
+                case 3: softmax_step<D, 3>(ts, to, tail, masked, bound, a.scale_log2, j == begin, m, l); break;
+                default: softmax_step<D, 4>(ts, to, tail, masked, bound, a.scale_log2, j == begin, m, l); break;
                 }
                 if (masked || (valid < kTile && it.n < a.Lk)) {
                     // Rows of V that are multiplied (those up to valid, in sixteens) and belong to hidden keys: both tiles'
@@ -576,13 +613,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 }
                 tc_fence_before();
                 mbar_arrive(&p_full[t]);
-                if (j == it.lo && no > 0 && lane == 0) {  // the last item's rows are out by now: its Q tile is free
+                if (j == begin && no > 0 && lane == 0) {  // the last item's rows are out by now: its Q tile is free
                     bulk_wait_read<0>();
                     mbar_arrive(&q_empty[QB * t + (no - 1) % QB]);
                 }
                 __syncwarp();
             }
-            if (!ok || (it.lo < it.hi && !mbar_wait(&o_full[t], no & 1, a.status, kErrAttnWait, abort_flag))) {
+            if (!ok || (begin < it.hi && !mbar_wait(&o_full[t], no & 1, a.status, kErrAttnWait, abort_flag))) {
                 ok = false;
                 break;
             }
@@ -591,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 part_m = m;
                 part_l = l;
                 part_here = true;
-                part_any = it.lo < it.hi;
+                part_any = begin < it.hi;
                 break;
             }
             // The item's scores are all made, so its Q tile takes the output rows on their way out.
@@ -630,18 +667,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
     }
 
     if constexpr (SPLIT) {
-        // Each CTA holds, for every row, its part's maximum m, sum l and O. With M the largest m, the row's result is
-        // sum O 2^(m - M) / sum l 2^(m - M). The tiles' valid rows are dealt out over the CTAs; every CTA sends its scaled
-        // rows to their owners, and those add and write them. The stages' memory takes the parts: all products that read it
-        // are done (o_full) before the first cluster barrier.
+        // Each CTA holds, for every row, its part's maximum m, sum l and O (two parts where both groups shared a tile). With M
+        // the largest m, the row's result is sum O 2^(m - M) / sum l 2^(m - M). The tiles' valid rows are dealt out over the
+        // CTAs; every CTA sends its scaled rows to their owners, and those add and write them. The stages' memory takes the
+        // parts: all products that read it are done (o_full) before the first cluster barrier.
         const int S = P.splits, me = int(cluster_ctarank());
-        const int t = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
+        const int t = max((warp - 4) >> 2, 0), r = (warp & 3) * 32 + lane;
         Items<true> it;
         it.first(P);
-        const int rows = min(kTile, a.Lq - it.q0() - max(t, 0) * kTile);  // of tile t
-        const int per = (kTile + S - 1) / S;                               // owned rows at most
-        float* parts = reinterpret_cast<float*>(smem) + max(t, 0) * (S * per * D);  // [S][per][D]
-        float* ml = reinterpret_cast<float*>(smem) + 2 * (S * per * D);    // [tiles][S][kTile][2]
+        const bool both = it.tiles == 1;
+        const int q0 = it.q0() + (both ? 0 : t * kTile), rows = min(kTile, a.Lq - q0);
+        const int per = (kTile + S - 1) / S;                             // owned rows at most
+        float* parts = reinterpret_cast<float*>(smem);                    // [tiles][S][per][D]
+        float* ml = reinterpret_cast<float*>(smem) + 2 * (S * per * D);  // [tiles][S][kTile][2]
+        // The parts of this group's rows: S of its own tile, or the 2 S of both.
+        const int from = both ? 0 : t * S, to_part = both ? 2 * S : from + S;
         __syncwarp();
         __syncthreads();
         cluster_sync_all();
@@ -654,11 +694,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
         cluster_sync_all();
         if (part_here && __any_sync(0xffffffffu, r < rows)) {
             float M = -INFINITY, L = 0.0f;
-            for (int o = 0; o < S && r < rows; ++o)
-                M = fmaxf(M, ml[((t * S + o) * kTile + r) * 2]);
+            for (int o = from; o < to_part && r < rows; ++o)
+                M = fmaxf(M, ml[(o * kTile + r) * 2]);
             const auto weight = [&](float m) { return m == -INFINITY ? 0.0f : ex2(m - M); };
-            for (int o = 0; o < S && r < rows; ++o) {
-                const float* e = ml + ((t * S + o) * kTile + r) * 2;
+            for (int o = from; o < to_part && r < rows; ++o) {
+                const float* e = ml + (o * kTile + r) * 2;
                 L += e[1] * weight(e[0]);
             }
             // A part without a visible key adds nothing (its O may never have been written); NaN parts stay NaN.
@@ -668,16 +708,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             while (owner + 1 < S && rows * (owner + 1) / S <= r)
                 ++owner;
             const int lr = r - rows * owner / S;
-            const uint32_t dst = map_to_cta(smem_u32(parts + (me * per + lr) * D), owner);
+            const uint32_t dst = map_to_cta(smem_u32(parts + ((t * S + me) * per + lr) * D), owner);
             const uint32_t to = tmem + (uint32_t((warp & 3) * 32) << 16) + 256 + t * 128;
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                uint32_t v[32];
-                tmem_ld32(to + c, v);
+            for (int c = 0; c < D; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(to + c, v);
                 tmem_wait_ld();
                 if (r < rows) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
+                    for (int i = 0; i < 16; i += 4)
                         st_cluster_f32x4(dst + (c + i) * 4,
                                          add ? make_float4(__uint_as_float(v[i]) * f, __uint_as_float(v[i + 1]) * f,
                                                            __uint_as_float(v[i + 2]) * f, __uint_as_float(v[i + 3]) * f)
@@ -690,16 +730,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
         if (part_here) {
             const int first = rows * me / S, count = rows * (me + 1) / S - first;
             __nv_bfloat16* out = a.out + it.b * a.so.sample + it.h * a.so.head;
-            for (int i = r; i < count * (D / 8); i += kTile) {
+            for (int i = r + (both ? t * kTile : 0); i < count * (D / 8); i += both ? 2 * kTile : kTile) {
                 const int lr = i / (D / 8), c = i % (D / 8) * 8;
                 float4 x = make_float4(0, 0, 0, 0), y = x;
-                for (int o = 0; o < S; ++o) {
+#pragma unroll 1
+                for (int o = from; o < to_part; ++o) {
                     const float4* e = reinterpret_cast<const float4*>(parts + (o * per + lr) * D + c);
                     const float4 u = e[0], v = e[1];
                     x = make_float4(x.x + u.x, x.y + u.y, x.z + u.z, x.w + u.w);
                     y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
                 }
-                *reinterpret_cast<uint4*>(out + long(it.q0() + t * kTile + first + lr) * a.so.row + c) =
+                *reinterpret_cast<uint4*>(out + long(q0 + first + lr) * a.so.row + c) =
                     make_uint4(pack_bf16x2(x.x, x.y), pack_bf16x2(x.z, x.w), pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
             }
         }
@@ -1020,6 +1061,48 @@ cudaError_t setup()
     return smem_limit_once(devs, k_cross<D, SPLIT>, Cfg<D, SPLIT>::kSmem);
 }
 
+// Clusters of `size` CTAs of k_cross<D, true> that the current device runs at once (they have to fit its GPCs), kept for
+// devices 0..63 once asked.
+template <int D>
+int clusters_at_once(int size)
+{
+    static std::atomic<int> known[64][kMaxSplits + 1];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess)
+        return 0;
+    const bool keep = dev >= 0 && dev < 64;
+    if (keep && known[dev][size].load(std::memory_order_relaxed))
+        return known[dev][size].load(std::memory_order_relaxed);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg<D, true>::kSmem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = size;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (setup<D, true>() != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, k_cross<D, true>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    if (keep)
+        known[dev][size].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+// CTAs an item: as many as run at once for all items, with two key steps each or more; 1 where that is not even two.
+template <int D>
+int splits_of(int items, int steps)
+{
+    for (int s = std::min({kMaxSplits, num_sms() / items, steps / 2}); s > 1; --s)
+        if (clusters_at_once<D>(s) >= items)
+            return s;
+    return 1;
+}
+
 template <int D>
 cudaError_t launch(const CrossParams& P, cudaStream_t st)
 {
@@ -1073,8 +1156,8 @@ cudaError_t cross_attention(const CrossArgs& a, const char** err, cudaStream_t s
     P.a = a;
     P.blocks = (a.Lq + 2 * kTile - 1) / (2 * kTile);
     P.items = a.B * a.H * P.blocks;
-    // Clusters where at least two CTAs an item fit the GPU at once and each gets two key steps or more.
-    P.splits = std::max(1, std::min({kMaxSplits, num_sms() / P.items, (a.Lk + kTile - 1) / kTile / 2}));
+    const int steps = (a.Lk + kTile - 1) / kTile;
+    P.splits = a.d == 64 ? splits_of<64>(P.items, steps) : splits_of<128>(P.items, steps);
     const void* k = a.Lk ? a.k : a.q;  // no keys: the maps are not used
     const void* v = a.Lk ? a.v : a.q;
     if (!encode_heads(&P.tq, a.q, a.sq, a.Lq, a.H, a.B, a.d, kTile, &P.q_head, &P.q_sample) ||
