@@ -4,14 +4,14 @@
 // k_cross: keys are few and queries many, so the work is a stream of query tiles past small sets of keys: persistent CTAs walk
 // items of (sample, head, 256 query rows) as two 128-row tiles A and B, and every stage runs ahead into the next item, so
 // that one item's loads, another's products and a third's stores overlap. Twelve warps:
-//   warp 0     TMA: Q tiles (two buffers for each of A and B), K and V tiles of 128 keys in one ring
+//   warp 0     TMA: Q tiles in one ring, K and V tiles of 128 keys in another
 //   warp 1     MMA: S = Q K^T, then O += P V with P in tensor memory, for A and B in turn (a warp for each of A and B, whose
 //              products then mix on the tensor pipe, was slower: 603 against 455 us at 2 x 24 x 4096 x 4096 x 128)
 //   warp 2     with a mask: a bound for each key's score, -inf for a hidden one, ahead of the softmax
 //   warps 4-7  softmax of tile A, 8-11 of tile B: a thread a row, the running maximum and sum of one pass; where a step has
-//              hidden keys each thread also clears its row of V if that is one (0 * NaN would spread); the output rows are
-//              staged in the Q tile that made them and leave as TMA stores (a thread storing its row directly touches 32
-//              lines an instruction)
+//              hidden keys each thread also clears its row of V if that is one (0 * NaN would spread); each warp stages its
+//              output rows in 4 KB of its own, 64 columns at a time, and sends them off as TMA stores (a thread storing its
+//              row directly touches 32 lines an instruction)
 // Where the items leave most of the GPU idle and the keys are many, SPLIT runs one item a cluster, whose CTAs take a run of
 // the key steps each and put the parts together through distributed shared memory: no workspace, no second launch. An item of a
 // single query tile gives it to both softmax groups there, who take the steps in turn as two parts.
@@ -48,13 +48,15 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units: O is rescaled only whe
 template <int D, bool SPLIT>
 struct Cfg {
     static constexpr int kTileBytes = (D / 64) * kPanel;
-    static constexpr int kQ = SPLIT ? 1 : 2;  // Q buffers of each tile: with a single item nothing is fetched ahead
-    static constexpr int kSlots = D == 64 ? (SPLIT ? 10 : 8) : (SPLIT ? 5 : 3);  // K and V tiles
-    static constexpr int kSmem = 1024 + (2 * kQ + kSlots) * kTileBytes + 512 + kHideSteps * (kTile * 4 + 16);
+    // Q tiles (two at work and, unless the item is the only one, the next on their way), K and V tiles, the output stage.
+    static constexpr int kQ = SPLIT ? 2 : D == 64 ? 5 : 3;
+    static constexpr int kSlots = SPLIT ? (D == 64 ? 10 : 5) : (D == 64 ? 7 : 3);
+    static constexpr int kStage = SPLIT ? 0 : 2 * kPanel;
+    static constexpr int kSmem = 1024 + (kQ + kSlots) * kTileBytes + kStage + 512 + kHideSteps * (kTile * 4 + 16);
     static_assert(kSmem <= 227 * 1024);
     static_assert((kSlots + 1) / 2 <= kSteps);
     // SPLIT: two tiles' parts and (m, l) pairs for up to 8 CTAs (S * ceil(128 / S) <= 133 rows for S <= 8) fit the stages.
-    static_assert(2 * 133 * D * 4 + 2 * 8 * kTile * 8 <= (2 * kQ + kSlots) * kTileBytes);
+    static_assert(2 * 133 * D * 4 + 2 * 8 * kTile * 8 <= (kQ + kSlots) * kTileBytes);
 };
 
 struct CrossParams {
@@ -267,18 +269,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
     constexpr int TB = C::kTileBytes, NS = C::kSlots;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    constexpr uint32_t QB = C::kQ;
-    uint8_t* sQ = smem;                 // [2 tiles][QB]
-    uint8_t* sKV = smem + 2 * QB * TB;  // [NS]
-    float* bounds = reinterpret_cast<float*>(smem + (2 * QB + NS) * TB);  // [kHideSteps][kTile]
+    constexpr uint32_t NQ = C::kQ;
+    uint8_t* sQ = smem;             // [NQ]
+    uint8_t* sKV = smem + NQ * TB;  // [NS]
+    uint8_t* sO = sKV + NS * TB;    // [tiles][kPanel]
+    float* bounds = reinterpret_cast<float*>(sO + C::kStage);  // [kHideSteps][kTile]
     volatile uint32_t* maskeds = reinterpret_cast<volatile uint32_t*>(bounds + kHideSteps * kTile);
     uint64_t* bars = reinterpret_cast<uint64_t*>(bounds + kHideSteps * (kTile + 4));
     // SPLIT: the rows' parts overlay the stages, this CTA's own result of a row stays in its softmax thread until then.
     float part_m = -INFINITY, part_l = 0.0f;
     bool part_here = false, part_any = false;
-    uint64_t* q_full = bars;             // [2 tiles][QB]
-    uint64_t* q_empty = q_full + 4;      // [2 tiles][QB]
-    uint64_t* kv_empty = q_empty + 4;    // [NS]
+    uint64_t* q_full = bars;             // [NQ]
+    uint64_t* q_empty = q_full + NQ;     // [NQ]
+    uint64_t* kv_empty = q_empty + NQ;   // [NS]
     // By key step, not by slot: where K and V take turns in a slot, threads that follow only the V tiles would miss phases
     // of the slot's barrier.
     uint64_t* k_full = kv_empty + NS;    // [kSteps]
@@ -295,9 +298,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < int(NQ); ++i) {
             mbar_init(&q_full[i], 1);
-            mbar_init(&q_empty[i], 4);  // the warps whose output rows have left the tile
+            mbar_init(&q_empty[i], 1);
         }
         for (int i = 0; i < NS; ++i)
             mbar_init(&kv_empty[i], 1);
@@ -340,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
     if (warp == 0) {
         if (lane == 0) {
             Walk<SPLIT> w;
-            uint32_t seq = 0, nq0 = 0, nq1 = 0;  // K and V tiles, Q tiles of A and of B loaded
+            uint32_t seq = 0, nq = 0;  // K and V tiles, Q tiles loaded
             bool ok = true;
             const auto load = [&](uint8_t* dst, const CUtensorMap* m, uint64_t* bar, int row, int h, int b) {
                 mbar_arrive_expect_tx(bar, TB);
@@ -351,12 +354,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             for (w.first(P); w.more(P) && ok; w.next(P)) {
                 const int hk = w.it.h / (a.H / a.Hkv);
                 for (int t = 0; w.start() && t < w.it.tiles && ok; ++t) {
-                    const uint32_t n = t ? nq1++ : nq0++, i = QB * t + n % QB;
-                    ok = mbar_wait(&q_empty[i], ((n / QB) & 1) ^ 1, a.status, kErrAttnWait, abort_flag);
-                    if (ok)
-                        load(sQ + i * TB, &P.tq, &q_full[i], w.it.q0() + t * kTile, w.it.h * P.q_head, w.it.b * P.q_sample);
-                    else
-                        --(t ? nq1 : nq0);
+                    const uint32_t s = nq % NQ;
+                    ok = mbar_wait(&q_empty[s], ((nq / NQ) & 1) ^ 1, a.status, kErrAttnWait, abort_flag);
+                    if (ok) {
+                        load(sQ + s * TB, &P.tq, &q_full[s], w.it.q0() + t * kTile, w.it.h * P.q_head,
+                             w.it.b * P.q_sample);
+                        ++nq;
+                    }
                 }
                 for (int kv = 0; kv < 2 && ok; ++kv) {
                     const uint32_t s = seq % NS;
@@ -372,11 +376,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 }
             }
             if (!ok) {  // let the loads already issued land before the CTA can exit
-                for (int t = 0; t < 2; ++t) {
-                    const uint32_t n = t ? nq1 : nq0;
-                    for (uint32_t i = n > QB ? n - QB : 0; i < n; ++i)
-                        mbar_wait(&q_full[QB * t + i % QB], (i / QB) & 1, a.status, kErrWaitDrain, nullptr);
-                }
+                for (uint32_t i = nq > NQ ? nq - NQ : 0; i < nq; ++i)
+                    mbar_wait(&q_full[i % NQ], (i / NQ) & 1, a.status, kErrWaitDrain, nullptr);
                 for (uint32_t i = seq > NS ? seq - NS : 0; i < seq; ++i)
                     mbar_wait(&(i & 1 ? v_full : k_full)[(i >> 1) % kSteps], ((i >> 1) / kSteps) & 1, a.status,
                               kErrWaitDrain, nullptr);
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             const uint64_t dq0 = desc_kmajor_sw128(smem_u32(sQ)), dk0 = desc_kmajor_sw128(smem_u32(sKV)),
                            dv0 = desc_mnmajor_sw128(smem_u32(sKV), kPanel, 1024);  // in units of 16 bytes
             constexpr uint32_t kUnit = TB >> 4;
-            uint32_t step = 0, nq[2] = {0, 0}, np[2] = {0, 0};  // key steps; Q and P tiles taken of A and B
+            uint32_t step = 0, nq = 0, np[2] = {0, 0};  // key steps; Q tile of the item's A; P tiles taken of A and B
             bool ok = true;
             const auto wait = [&](uint64_t* bar, uint32_t phase) {
                 return bool(__all_sync(0xffffffffu, mbar_wait(bar, phase & 1, a.status, kErrAttnWait, abort_flag)));
@@ -399,9 +400,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             // S_t = Q_t K^T; Q is waited for at an item's first step.
             const auto scores = [&](auto tile, bool first, bool last, uint64_t dk, uint32_t idesc, bool shared_q = false) {
                 constexpr int t = decltype(tile)::value;
-                const uint32_t qi = shared_q ? 0 : QB * t + nq[t] % QB;
+                const uint32_t n = shared_q ? 0 : nq + t, qi = n % NQ;
                 const uint64_t dq = dq0 + qi * kUnit;
-                if (first && !wait(&q_full[qi], nq[t] / QB))
+                if (first && !wait(&q_full[qi], n / NQ))
                     return false;
                 tc_fence_after();
                 if (elect_one_sync()) {
@@ -411,9 +412,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                         mma_bf16_ss(tmem + t * 128, dq + off, dk + off, idesc, k > 0);
                     }
                     mma_commit(&s_full[t]);
+                    if (last)
+                        mma_commit(&q_empty[qi]);
                 }
                 __syncwarp();
-                nq[t] += last;
                 return true;
             };
             // O_t += P_t V.
@@ -488,6 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 const uint32_t sv = (2 * step + 1) % NS, sk = (2 * step + 2) % NS;
                 const uint64_t dv = dv0 + sv * kUnit, dk = dk0 + sk * kUnit;
                 const uint32_t idesc = idesc_s0 | uint32_t(x.width() >> 3) << 17;
+                if (last)
+                    nq += w.it.tiles;  // the next scores are the next item's
                 const auto next_k = [&] { return wait(&k_full[(step + 1) % kSteps], (step + 1) / kSteps); };
                 ok = wait(&v_full[step % kSteps], step / kSteps) &&
                      outputs(kA, first, last, dv, width) && (!more || (next_k() && scores(kA, xfirst, xlast, dk, idesc))) &&
@@ -613,11 +617,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 }
                 tc_fence_before();
                 mbar_arrive(&p_full[t]);
-                if (j == begin && no > 0 && lane == 0) {  // the last item's rows are out by now: its Q tile is free
-                    bulk_wait_read<0>();
-                    mbar_arrive(&q_empty[QB * t + (no - 1) % QB]);
-                }
-                __syncwarp();
             }
             if (!ok || (begin < it.hi && !mbar_wait(&o_full[t], no & 1, a.status, kErrAttnWait, abort_flag))) {
                 ok = false;
@@ -631,36 +630,35 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 part_any = begin < it.hi;
                 break;
             }
-            // The item's scores are all made, so its Q tile takes the output rows on their way out.
-            uint8_t* stage = sQ + (QB * t + no % QB) * TB;
             ++no;
+            uint8_t* stage = sO + t * kPanel + w32 * 128;
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld32(to + c * 32, o);
+            for (int p = 0; p < D / 64; ++p) {
+                uint32_t o[64];
+                tmem_ld32(to + p * 64, *reinterpret_cast<uint32_t(*)[32]>(&o[0]));
+                tmem_ld32(to + p * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(&o[32]));
                 tmem_wait_ld();
-                uint8_t* dst = stage + (c >> 1) * kPanel + r * 128;
+                if (lane == 0)
+                    bulk_wait_read<0>();  // the warp's last store has read the stage
+                __syncwarp();
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<uint4*>(dst + ((((c & 1) * 4 + i) ^ (r & 7)) << 4)) = make_uint4(
+                for (int i = 0; i < 8; ++i)
+                    *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(
                         pack_bf16x2(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv),
                         pack_bf16x2(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv),
                         pack_bf16x2(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv),
                         pack_bf16x2(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv));
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    if (row0 < a.Lq)
+                        tma_store_4d(&P.to, stage, p * 64, row0, it.h * P.o_head, it.b * P.o_sample);
+                    bulk_commit();
+                }
+                __syncwarp();
             }
             tc_fence_before();  // O has been read before the P that lets the next item's product overwrite it
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                if (row0 < a.Lq)
-#pragma unroll
-                    for (int p = 0; p < D / 64; ++p)
-                        tma_store_4d(&P.to, stage + p * kPanel + w32 * 128, p * 64, row0, it.h * P.o_head,
-                                     it.b * P.o_sample);
-                bulk_commit();
-            }
-            __syncwarp();
         }
         if (lane == 0)
             bulk_wait_all();  // the last rows are written before the CTA and its shared memory go
@@ -1145,7 +1143,10 @@ cudaError_t launch_few(const CrossArgs& a, cudaStream_t st)
 
 cudaError_t cross_attention(const CrossArgs& a, const char** err, cudaStream_t st)
 {
-    if (long(a.H / a.Hkv) * a.Lq <= kFewRows) {
+    // The CUDA cores keep up with HBM for one or two rows; up to four they still win where the keys are few (four rows over 4096
+    // keys of 48 heads: 46 against 29 us).
+    const long few = long(a.H / a.Hkv) * a.Lq;
+    if (few <= 2 || (few <= kFewRows && a.Lk <= 512)) {
         const cudaError_t e = a.d == 64 ? launch_few<64>(a, st) : launch_few<128>(a, st);
         if (e != cudaSuccess)
             return e;
