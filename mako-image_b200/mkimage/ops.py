@@ -212,30 +212,40 @@ NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 OUT_NONE, OUT_BF16, OUT_F32, OUT_I8 = 0, 1, 2, 3
 
 
+# torch and the two calls every launch needs of it, looked up once: a call of these operators costs the host about as much as
+# its launch, so their checks are written for few steps.
+torch = None
+_current_device = _raw_stream = None
+
+
+def _load():
+    global torch, _current_device, _raw_stream
+    import torch as t
+
+    torch, _current_device, _raw_stream = t, t._C._cuda_getDevice, t._C._cuda_getCurrentRawStream
+    return t
+
+
 def _fail(what):
     raise MkbError(1, what)
 
 
-def _device_of(name, *tensors):
-    """The one CUDA device that the given tensors live on."""
-    dev = tensors[0].get_device()
+def _same_device(name, dev, *tensors):
+    """The given tensors live on CUDA device `dev`."""
     if dev < 0:
         _fail(f"{name}: tensors must be CUDA tensors")
     for t in tensors:
         if t is not None and t.get_device() != dev:
             _fail(f"{name}: a tensor is on {t.device}, not on cuda:{dev}")
-    return dev
 
 
 def _launch(fn, dev, *args):
     """fn(*args, stream) on the tensors' device and its current stream, whatever device is current."""
-    import torch
-
-    if torch._C._cuda_getDevice() == dev:
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if _current_device() == dev:
+        code = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+            code = fn(*args, _raw_stream(dev))
     if code:
         check(code)
 
@@ -250,68 +260,72 @@ def _row_stride(t, n):
     return s if s >= n else n if t.shape[0] <= 1 else s
 
 
-def _rows_i8(rows, n, dev):
-    import torch
-
-    return torch.empty_strided((rows, n), (-(-n // 16) * 16, 1), device=dev, dtype=torch.int8)
-
-
 def _vector(t, n, f32, what):
-    if t is not None and (t.dtype != f32 or t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1)):
+    if t.dtype is not f32 or t.shape != (n,) or (n > 1 and not t.is_contiguous()):
         _fail(what)
 
 
 def quantize_rows(x, q=None, scale=None):
     """(q, scale): rows of x [rows][n] (bf16 or fp32) as int8 with an fp32 step max|row| / 127 each, so that q * scale
     is x to half a step (see mkb_quantize_rows). q's rows are 16 bytes aligned, as proj_i8 wants them."""
-    import torch
-
-    dtype = x.dtype
-    if x.dim() != 2 or (dtype != torch.bfloat16 and dtype != torch.float32):
+    t = torch or _load()
+    f32 = x.dtype is t.float32
+    if x.dim() != 2 or not (f32 or x.dtype is t.bfloat16):
         _fail("quantize_rows: x must be 2-D bf16 or fp32")
     rows, n = x.shape
-    if n == 0 or (n > 1 and x.stride(1) != 1):
+    ldx, step = x.stride()
+    if n == 0 or (step != 1 and n > 1):
         _fail("quantize_rows: the values of a row must be contiguous, one at least")
+    dev = x.get_device()
+    _same_device("quantize_rows", dev, q, scale)
     if q is None:
-        q = _rows_i8(rows, n, x.device)
-    elif q.shape != x.shape or q.dtype != torch.int8 or (n > 1 and q.stride(1) != 1):
-        _fail("quantize_rows: q must be int8 rows of x's shape")
-    if scale is None:
-        scale = torch.empty(rows, device=x.device, dtype=torch.float32)
+        ldq = (n + 15) & ~15
+        q = t.empty_strided((rows, n), (ldq, 1), device=x.device, dtype=t.int8)
     else:
-        _vector(scale, rows, torch.float32, "quantize_rows: scale must be contiguous fp32 [rows]")
-    dev = _device_of("quantize_rows", x, q, scale)
-    _launch(lib.mkb_quantize_rows, dev, x.data_ptr(), _row_stride(x, n), dtype == torch.float32, q.data_ptr(),
-            _row_stride(q, n), scale.data_ptr(), rows, n)
+        if q.shape != x.shape or q.dtype is not t.int8 or (n > 1 and q.stride(1) != 1):
+            _fail("quantize_rows: q must be int8 rows of x's shape")
+        ldq = _row_stride(q, n)
+    if scale is None:
+        scale = t.empty(rows, device=x.device, dtype=t.float32)
+    else:
+        _vector(scale, rows, t.float32, "quantize_rows: scale must be contiguous fp32 [rows]")
+    _launch(lib.mkb_quantize_rows, dev, x.data_ptr(), ldx if rows > 1 else n, f32, q.data_ptr(), ldq, scale.data_ptr(),
+            rows, n)
     return q, scale
 
 
 def proj_i8(x, x_scale, w, w_scale, bias=None, act=ACT_NONE, out=None, out_f32=False):
     """y = act(x_scale[:, None] * w_scale * (x @ w.T) + bias): x [M][K] and w [N][K] int8 with rows 16 bytes aligned
     (quantize_rows makes such rows), scales fp32, exact integer sums (see mkb_proj_i8)."""
-    import torch
-
-    f32 = torch.float32
-    if x.dtype != torch.int8 or w.dtype != torch.int8 or x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+    t = torch or _load()
+    f32 = t.float32
+    if x.dtype is not t.int8 or w.dtype is not t.int8 or x.dim() != 2 or w.dim() != 2:
         _fail("proj_i8: x [M][K] and w [N][K] must be int8")
     M, K = x.shape
-    N = w.shape[0]
-    if out is None:
-        out = torch.empty(M, N, device=x.device, dtype=f32 if out_f32 else torch.bfloat16)
-    else:
-        out_f32 = out.dtype == f32
-        if out.shape != (M, N) or (not out_f32 and out.dtype != torch.bfloat16) or (N > 1 and out.stride(1) != 1):
-            _fail("proj_i8: out must be [M][N] fp32 or bf16 with contiguous rows")
-    if K > 1 and (x.stride(1) != 1 or w.stride(1) != 1):
+    N, Kw = w.shape
+    if K != Kw:
+        _fail("proj_i8: x [M][K] and w [N][K] must have rows of one length")
+    ldx, sx = x.stride()
+    ldw, sw = w.stride()
+    if K > 1 and (sx != 1 or sw != 1):
         _fail("proj_i8: the values of a row must be contiguous")
-    _vector(x_scale, M, f32, "proj_i8: x_scale must be contiguous fp32 [M]")
-    _vector(w_scale, N, f32, "proj_i8: w_scale must be contiguous fp32 [N]")
-    _vector(bias, N, f32, "proj_i8: bias must be contiguous fp32 [N]")
-    dev = _device_of("proj_i8", x, x_scale, w, w_scale, bias, out)
-    ldx = x.stride(0) if M > 1 else -(-K // 16) * 16
-    ldw = w.stride(0) if N > 1 else -(-K // 16) * 16
-    _launch(lib.mkb_proj_i8, dev, x.data_ptr(), ldx, x_scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(),
-            _ptr(bias), out.data_ptr(), _row_stride(out, N), M, N, K, act, out_f32)
+    if x_scale.dtype is not f32 or w_scale.dtype is not f32 or x_scale.shape != (M,) or w_scale.shape != (N,) or \
+            not (x_scale.is_contiguous() and w_scale.is_contiguous()):
+        _fail("proj_i8: the scales must be contiguous fp32 vectors, one value a row of x or w")
+    if bias is not None:
+        _vector(bias, N, f32, "proj_i8: bias must be contiguous fp32 [N]")
+    dev = x.get_device()
+    _same_device("proj_i8", dev, x_scale, w, w_scale, bias, out)
+    if out is None:
+        out = t.empty((M, N), device=x.device, dtype=f32 if out_f32 else t.bfloat16)
+        ldy = N
+    else:
+        out_f32 = out.dtype is f32
+        if out.shape != (M, N) or not (out_f32 or out.dtype is t.bfloat16) or (N > 1 and out.stride(1) != 1):
+            _fail("proj_i8: out must be [M][N] fp32 or bf16 with contiguous rows")
+        ldy = _row_stride(out, N)
+    _launch(lib.mkb_proj_i8, dev, x.data_ptr(), ldx if M > 1 else (K + 15) & ~15, x_scale.data_ptr(), w.data_ptr(),
+            ldw if N > 1 else (K + 15) & ~15, w_scale.data_ptr(), _ptr(bias), out.data_ptr(), ldy, M, N, K, act, out_f32)
     return out
 
 
@@ -325,31 +339,29 @@ def gate_add_norm(x, y=None, y_norm=NORM_NONE, y_weight=None, gate=None, tanh_ga
 
     x [rows][n] fp32, y bf16 or fp32; gate, scale, shift [samples][n] (or [n]) of the sample row // rows_per_sample.
     Returns out as out_type says: bf16, fp32, (int8 rows, steps) or None."""
-    import torch
-
-    f32 = torch.float32
-    if x.dim() != 2 or x.dtype != f32:
+    t = torch or _load()
+    f32 = t.float32
+    if x.dim() != 2 or x.dtype is not f32:
         _fail("gate_add_norm: x must be 2-D fp32")
-    rows, n = x.shape
+    shape = x.shape
+    rows, n = shape
     rps = rows_per_sample or max(rows, 1)
     samples = -(-rows // rps)
 
-    def rows_of(t, dtype):
-        if t.shape != x.shape or t.dtype != dtype or (n > 1 and t.stride(1) != 1):
+    def rows_of(a, dtype):
+        ld, step = a.stride() if a.dim() == 2 else (0, 0)
+        if a.shape != shape or a.dtype is not dtype or (step != 1 and n > 1):
             _fail("gate_add_norm: x, x_out, y and out must be [rows][n] of their types with contiguous rows")
-        return _row_stride(t, n)
+        return ld if rows > 1 else max(ld, n)
 
-    def per_sample(t):
-        if t is None:
-            return 0
-        if t.dtype != f32 or t.shape[-1] != n or (n > 1 and t.stride(-1) != 1):
+    def per_sample(a):
+        if a.dtype is not f32 or a.shape[-1] != n or (n > 1 and a.stride(-1) != 1) or \
+                not (a.dim() == 1 or (a.dim() == 2 and a.shape[0] in (1, samples))):
             _fail("gate_add_norm: gate, scale and shift must be fp32 [n] or [samples][n]")
-        if t.dim() == 1:
-            return 0
-        if t.dim() != 2 or (t.shape[0] != samples and t.shape[0] != 1):
-            _fail("gate_add_norm: gate, scale and shift must be fp32 [n] or [samples][n]")
-        return t.stride(0) if t.shape[0] > 1 else 0
+        return a.stride(0) if a.dim() == 2 and a.shape[0] > 1 else 0
 
+    dev = x.get_device()
+    _same_device("gate_add_norm", dev, y, y_weight, gate, x_weight, scale, shift, x_out, out, out_scale)
     ldx = rows_of(x, f32)
     if x_out is None:
         x_out, ldxo = x, ldx
@@ -357,37 +369,41 @@ def gate_add_norm(x, y=None, y_norm=NORM_NONE, y_weight=None, gate=None, tanh_ga
         ldxo = rows_of(x_out, f32)
     ldy, y_f32 = 0, False
     if y is not None:
-        y_f32 = y.dtype == f32
-        ldy = rows_of(y, f32 if y_f32 else torch.bfloat16)
+        y_f32 = y.dtype is f32
+        ldy = rows_of(y, f32 if y_f32 else t.bfloat16)
     if out_type == OUT_NONE:
         if out is not None:
             _fail("gate_add_norm: out without an out_type")
         x_norm, ldo = NORM_NONE, 0
     else:
-        dtype = torch.bfloat16 if out_type == OUT_BF16 else f32 if out_type == OUT_F32 else torch.int8
+        dtype = t.bfloat16 if out_type == OUT_BF16 else f32 if out_type == OUT_F32 else t.int8
         if out is not None:
             ldo = rows_of(out, dtype)
         elif out_type == OUT_I8:
-            out = _rows_i8(rows, n, x.device)
-            ldo = -(-n // 16) * 16
+            ldo = (n + 15) & ~15
+            out = t.empty_strided(shape, (ldo, 1), device=x.device, dtype=dtype)
         else:
-            out = torch.empty(rows, n, device=x.device, dtype=dtype)
             ldo = n
+            out = t.empty(shape, device=x.device, dtype=dtype)
     if out_type == OUT_I8:
         if out_scale is None:
-            out_scale = torch.empty(rows, device=x.device, dtype=f32)
+            out_scale = t.empty(rows, device=x.device, dtype=f32)
         else:
             _vector(out_scale, rows, f32, "gate_add_norm: out_scale must be contiguous fp32 [rows]")
     elif out_scale is not None:
         _fail("gate_add_norm: out_scale goes with 8-bit outputs alone")
-    _vector(y_weight, n, f32, "gate_add_norm: weights must be contiguous fp32 [n]")
-    _vector(x_weight, n, f32, "gate_add_norm: weights must be contiguous fp32 [n]")
-    gate_stride, mod_stride, shift_stride = per_sample(gate), per_sample(scale), per_sample(shift)
-    if scale is None:
-        mod_stride = shift_stride
-    elif shift is not None and shift_stride != mod_stride and samples > 1:
-        _fail("gate_add_norm: scale and shift must have the same strides")
-    dev = _device_of("gate_add_norm", x, y, y_weight, gate, x_weight, scale, shift, x_out, out, out_scale)
+    if y_weight is not None:
+        _vector(y_weight, n, f32, "gate_add_norm: weights must be contiguous fp32 [n]")
+    if x_weight is not None:
+        _vector(x_weight, n, f32, "gate_add_norm: weights must be contiguous fp32 [n]")
+    gate_stride = 0 if gate is None else per_sample(gate)
+    mod_stride = 0 if scale is None else per_sample(scale)
+    if shift is not None:
+        shift_stride = per_sample(shift)
+        if scale is None:
+            mod_stride = shift_stride
+        elif shift_stride != mod_stride and samples > 1:
+            _fail("gate_add_norm: scale and shift must have the same strides")
     _launch(lib.mkb_gate_add_norm, dev, x.data_ptr(), ldx, x_out.data_ptr(), ldxo, _ptr(y), ldy, y_f32, y_norm,
             _ptr(y_weight), _ptr(gate), gate_stride, tanh_gate, x_norm, _ptr(x_weight), _ptr(scale), _ptr(shift),
             mod_stride, rps, eps, _ptr(out), ldo, out_type, _ptr(out_scale), rows, n)
@@ -399,17 +415,19 @@ def cross_attention(q, k, v, key_len=None, key_mask=None, scale=None, out=None):
     contiguous heads: permuted token-major projections as well as head-major ones), over each sample's first key_len[b]
     keys that key_mask [B][Lk] (bool) leaves (see mkb_cross_attention). Returns out [B][Lq][H * d] (given: any
     [B][Lq][H][d] or [B][Lq][H * d] bf16)."""
-    import torch
-
-    bf16 = torch.bfloat16
+    t = torch or _load()
+    bf16 = t.bfloat16
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
         _fail("cross_attention: q must be [B][H][Lq][d], k and v [B][Hkv][Lk][d]")
     B, H, Lq, d = q.shape
     Bk, Hkv, Lk, dk = k.shape
     if Bk != B or dk != d:
         _fail("cross_attention: q must be [B][H][Lq][d], k and v [B][Hkv][Lk][d]")
+    dev = q.get_device()
+    _same_device("cross_attention", dev, k, v, out, key_len, key_mask)
+    o_last = 1
     if out is None:
-        out = torch.empty(B, Lq, H * d, device=q.device, dtype=bf16)
+        out = t.empty((B, Lq, H * d), device=q.device, dtype=bf16)
         o_row, o_head, o_sample = H * d, d, Lq * H * d
     elif out.shape == (B, Lq, H * d):
         o_sample, o_row, o_last = out.stride()
@@ -421,20 +439,18 @@ def cross_attention(q, k, v, key_len=None, key_mask=None, scale=None, out=None):
     q_sample, q_head, q_row, q_last = q.stride()
     k_sample, k_head, k_row, k_last = k.stride()
     v_sample, v_head, v_row, v_last = v.stride()
-    for t in (q, k, v, out):
-        if t.dtype != bf16 or t.stride(-1) != 1:
-            _fail("cross_attention: tensors must be bf16 with contiguous heads")
-    if key_len is not None and (key_len.dtype != torch.int32 or key_len.shape != (B,) or (B > 1 and key_len.stride(0) != 1)):
+    if not (q_last == k_last == v_last == o_last == 1) or not (q.dtype is bf16 and k.dtype is bf16 and v.dtype is bf16 and
+                                                              out.dtype is bf16):
+        _fail("cross_attention: tensors must be bf16 with contiguous heads")
+    if key_len is not None and (key_len.dtype is not t.int32 or key_len.shape != (B,) or not key_len.is_contiguous()):
         _fail("cross_attention: key_len must be contiguous int32 [B]")
     mask_stride = 0
     if key_mask is not None:
-        if key_mask.shape != (B, Lk) or key_mask.dtype not in (torch.bool, torch.uint8) or \
-                (Lk > 1 and key_mask.stride(1) != 1):
+        if key_mask.shape != (B, Lk) or key_mask.dtype not in (t.bool, t.uint8) or (Lk > 1 and key_mask.stride(1) != 1):
             _fail("cross_attention: key_mask must be bool [B][Lk]")
         mask_stride = key_mask.stride(0)
     if scale is not None and not scale > 0:
         _fail("cross_attention: the scale must be positive")
-    dev = _device_of("cross_attention", q, k, v, out, key_len, key_mask)
     _launch(lib.mkb_cross_attention, dev, q.data_ptr(), q_row, q_head, q_sample, k.data_ptr(), k_row, k_head, k_sample,
             v.data_ptr(), v_row, v_head, v_sample, out.data_ptr(), o_row, o_head, o_sample, B, H, Hkv, Lq, Lk, d,
             _ptr(key_len), _ptr(key_mask), mask_stride, scale or 0.0)
