@@ -447,9 +447,9 @@ template <int BN>
 struct PairCfg {
     static constexpr int kABytes = 128 * kBK, kBBytes = BN / 2 * kBK, kStageBytes = kABytes + kBBytes;
     static constexpr int kBox = 32 * 128;  // a warp's box: 32 rows of 128 bytes
-    static constexpr int kStages = BN == 256 ? 5 : 7;
+    static constexpr int kStages = BN == 256 ? 6 : 8;
     static constexpr int kVec = 2 * 2 * BN * 4;  // w_scale and bias of two tiles
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + 8 * kBox + kVec + 256;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + 4 * kBox + kVec + 256;
     static constexpr int kTmemCols = 2 * BN;
     static_assert(kSmem <= 227 * 1024);
 };
@@ -473,8 +473,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(co
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* boxes = smem + C::kStages * C::kStageBytes;
-    float* vec = reinterpret_cast<float*>(boxes + 8 * C::kBox);  // [2][w_scale, bias][BN]
-    uint64_t* full = reinterpret_cast<uint64_t*>(boxes + 8 * C::kBox + C::kVec);
+    float* vec = reinterpret_cast<float*>(boxes + 4 * C::kBox);  // [2][w_scale, bias][BN]
+    uint64_t* full = reinterpret_cast<uint64_t*>(boxes + 4 * C::kBox + C::kVec);
     uint64_t* empty = full + C::kStages;
     uint64_t* acc_full = empty + C::kStages;
     uint64_t* acc_empty = acc_full + 2;
@@ -581,8 +581,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(co
     } else {
         const int q = warp & 3, et = int(threadIdx.x) - 64;
         const uint32_t acc_empty0 = map_to_cta(smem_u32(&acc_empty[0]), 0);
-        uint8_t* box = boxes + (warp - 2) * 2 * C::kBox;
-        uint32_t lt = 0, nbox = 0;
+        uint8_t* box = boxes + (warp - 2) * C::kBox;
+        uint32_t lt = 0;
         for (int tile = pair; tile < num_tiles; tile += npairs, ++lt) {
             int mb, nb;
             tile_of(tile, num_m, num_n, mb, nb);
@@ -627,10 +627,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(co
                 }
                 // A box holds 128 bytes of each row: 32 fp32 columns, or two rounds of 32 bf16 ones.
                 const int half = a.out_f32 ? 0 : (c >> 5) & 1;
-                uint8_t* bx = box + (nbox & 1) * C::kBox + lane * 128;
+                uint8_t* bx = box + lane * 128;
                 if (half == 0) {
                     if (lane == 0)
-                        bulk_wait_read<1>();  // the store before last has read this box
+                        bulk_wait_read<0>();  // the last store has read the box
                     __syncwarp();
                 }
                 if (a.out_f32) {
@@ -650,10 +650,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(co
                     __syncwarp();
                     if (lane == 0) {
                         if (row0 < a.M)
-                            tma_store_2d(&P.ty, box + (nbox & 1) * C::kBox, a.out_f32 ? n0 + c : n0 + c - 32 * half, row0);
+                            tma_store_2d(&P.ty, box, a.out_f32 ? n0 + c : n0 + c - 32 * half, row0);
                         bulk_commit();
                     }
-                    ++nbox;
                 }
             }
             tc_fence_before();
