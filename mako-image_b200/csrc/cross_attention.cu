@@ -1141,8 +1141,13 @@ cudaError_t launch_few(const CrossArgs& a, cudaStream_t st)
 
 }  // namespace
 
-cudaError_t cross_attention(const CrossArgs& a, const char** err, cudaStream_t st)
+cudaError_t cross_attention(const CrossArgs& args, const char** err, cudaStream_t st)
 {
+    CrossArgs a = args;
+    if (a.Lk == 0) {  // no key is read; addresses are still made
+        a.k = a.v = a.q;
+        a.sk = a.sv = HeadStrides{a.d, 0, 0};
+    }
     // The CUDA cores keep up with HBM for one or two rows; up to four they still win where the keys are few (four rows over 4096
     // keys of 48 heads: 46 against 29 us).
     const long few = long(a.H / a.Hkv) * a.Lq;
@@ -1159,11 +1164,9 @@ cudaError_t cross_attention(const CrossArgs& a, const char** err, cudaStream_t s
     P.items = a.B * a.H * P.blocks;
     const int steps = (a.Lk + kTile - 1) / kTile;
     P.splits = a.d == 64 ? splits_of<64>(P.items, steps) : splits_of<128>(P.items, steps);
-    const void* k = a.Lk ? a.k : a.q;  // no keys: the maps are not used
-    const void* v = a.Lk ? a.v : a.q;
     if (!encode_heads(&P.tq, a.q, a.sq, a.Lq, a.H, a.B, a.d, kTile, &P.q_head, &P.q_sample) ||
-        !encode_heads(&P.tk, k, a.sk, a.Lk, a.Hkv, a.B, a.d, kTile, &P.kv_head_k, &P.kv_sample_k) ||
-        !encode_heads(&P.tv, v, a.sv, a.Lk, a.Hkv, a.B, a.d, kTile, &P.kv_head_v, &P.kv_sample_v) ||
+        !encode_heads(&P.tk, a.k, a.sk, a.Lk, a.Hkv, a.B, a.d, kTile, &P.kv_head_k, &P.kv_sample_k) ||
+        !encode_heads(&P.tv, a.v, a.sv, a.Lk, a.Hkv, a.B, a.d, kTile, &P.kv_head_v, &P.kv_sample_v) ||
         !encode_heads(&P.to, a.out, a.so, a.Lq, a.H, a.B, a.d, 32, &P.o_head, &P.o_sample)) {
         *err = "cross_attention: tensor map encoding failed";
         return cudaErrorInvalidValue;

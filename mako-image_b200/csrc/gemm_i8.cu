@@ -486,7 +486,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(co
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
     const int pair = blockIdx.x / 2, npairs = gridDim.x / 2;
-    const int num_m = (a.M + 255) / 256, num_n = (a.N + BN - 1) / BN, num_k = (a.K + kBK - 1) / kBK;
+    const int num_m = int((a.M + 255L) / 256), num_n = int((a.N + BN - 1L) / BN), num_k = (a.K + kBK - 1) / kBK;
     const int num_tiles = num_m * num_n;
 
     if (threadIdx.x == 0) {
@@ -783,7 +783,7 @@ cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
                 *err = "proj_i8: tensor map encoding failed";
                 return cudaErrorInvalidValue;
             }
-            const int tiles = (a.M + 255) / 256 * ((a.N + bn - 1) / bn);
+            const int tiles = int((a.M + 255L) / 256 * ((a.N + bn - 1L) / bn));
             e = bn == 256 ? launch_pair<256>(P, tiles, st) : launch_pair<128>(P, tiles, st);
         }
     }

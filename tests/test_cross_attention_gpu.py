@@ -65,7 +65,9 @@ def _check(q, k, v, key_len=None, key_mask=None, scale=None, out=None):
 @pytest.mark.parametrize("B,H,Hkv,Lq,Lk", [
     (1, 1, 1, 1, 1), (1, 2, 2, 1, 77), (2, 3, 3, 5, 16), (2, 4, 2, 127, 77), (1, 3, 1, 128, 128), (2, 2, 1, 129, 129),
     (1, 2, 2, 256, 300), (1, 2, 2, 257, 512), (3, 4, 4, 300, 31), (2, 10, 10, 1000, 77), (1, 4, 1, 700, 1000),
-    (1, 1, 1, 1, 4096), (2, 4, 4, 1, 5000), (1, 8, 2, 3, 2049), (1, 2, 2, 64, 3333), (4, 24, 24, 260, 130)])
+    (1, 1, 1, 1, 4096), (2, 4, 4, 1, 5000), (1, 8, 2, 3, 2049), (1, 2, 2, 64, 3333), (4, 24, 24, 260, 130),
+    (2, 8, 4, 1, 700), (2, 3, 1, 1, 300), (1, 3, 3, 128, 8000), (1, 3, 3, 256, 8000), (2, 3, 3, 255, 257), (3, 20, 20, 1100, 77),
+    (2, 12, 12, 800, 600)])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("layout", ["head", "token"])
 def test_full_keys(cuda, B, H, Hkv, Lq, Lk, d, layout):
@@ -75,7 +77,8 @@ def test_full_keys(cuda, B, H, Hkv, Lq, Lk, d, layout):
     _check(_heads(cuda, g, B, H, Lq, d, layout, 1.5), _heads(cuda, g, B, Hkv, Lk, d, layout), _heads(cuda, g, B, Hkv, Lk, d, layout))
 
 
-@pytest.mark.parametrize("Lq,Lk", [(1, 200), (40, 77), (257, 333), (600, 512), (2, 3000)])
+@pytest.mark.parametrize("Lq,Lk", [(1, 200), (40, 77), (257, 333), (600, 512), (1, 3000), (2, 3000), (100, 2500), (200, 2500),
+                                   (1300, 300)])
 @pytest.mark.parametrize("d", [64, 128])
 def test_key_lengths_and_masks(cuda, Lq, Lk, d):
     """Each sample its own keys: none, one, all; holes, a first tile without keys, the last key alone."""
@@ -104,7 +107,7 @@ def test_key_lengths_and_masks(cuda, Lq, Lk, d):
 
 
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("Lq,Lk", [(1, 300), (200, 77), (520, 400)])
+@pytest.mark.parametrize("Lq,Lk", [(1, 300), (200, 77), (520, 400), (1, 4000), (3, 200), (60, 1700), (180, 1700)])
 def test_nothing_hidden_reaches_the_result(cuda, d, Lq, Lk):
     """NaN and infinities in masked and cut-off keys and values, and behind them in memory, change no bit."""
     import torch

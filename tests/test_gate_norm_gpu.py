@@ -66,7 +66,9 @@ def _check(ops, c, per, y_norm, x_norm, tanh, mod, out_type, eps=1e-6, in_place=
     got = ops.gate_add_norm(x_in, c["y"], y_norm=y_norm, y_weight=c["yw"] if y_norm else None, gate=c["gate"],
                             tanh_gate=tanh, x_norm=x_norm, x_weight=c["xw"], scale=c["scale"] if mod else None,
                             shift=c["shift"] if mod else None, rows_per_sample=per, eps=eps, x_out=x_out,
-                            out_type=out_type)
+                            out_type=out_type) if out_type != ops.OUT_NONE else ops.gate_add_norm(
+        x_in, c["y"], y_norm=y_norm, y_weight=c["yw"] if y_norm else None, gate=c["gate"], tanh_gate=tanh,
+        rows_per_sample=per, eps=eps, x_out=x_out, out_type=out_type)
     x_got = (x_in if in_place else x_out).to(D)
     if not in_place:
         assert torch.equal(c["x"], x0)
@@ -112,6 +114,22 @@ def test_gate_add_norm(cuda, rows, n, y_norm, x_norm, out):
     c = _case(cuda, rows, n, rows * n, y_f32=n % 2 == 1, vec_samples=-(-rows // per))
     kind = dict(bf16=ops.OUT_BF16, f32=ops.OUT_F32, i8=ops.OUT_I8)[out]
     _check(ops, c, per, y_norm, x_norm, tanh=(y_norm == 1), mod=(out != "f32"), out_type=kind)
+
+
+@pytest.mark.parametrize("rows,n,samples", [(1000, 640, 3), (2100, 3072, 2), (900, 1283, 7), (5000, 96, 1), (700, 6144, 2),
+                                             (400, 6400, 2), (301, 4099, 301), (800, 12288, 5)])
+@pytest.mark.parametrize("out", ["bf16", "i8", "none"])
+def test_runs_of_rows(cuda, rows, n, samples, out):
+    """Rows enough that a block walks several of one sample, with short last runs and samples; in place as well. Outputs
+    with no norm at all take one barrier a row or none."""
+    import mkimage
+
+    ops = mkimage.ops
+    per = -(-rows // samples)
+    c = _case(cuda, rows, n, rows + n, False, -(-rows // per))
+    kind = dict(bf16=ops.OUT_BF16, i8=ops.OUT_I8, none=ops.OUT_NONE)[out]
+    for y_norm, x_norm in ((1, 1), (0, 2), (0, 0)):
+        _check(ops, c, per, y_norm, x_norm, tanh=y_norm == 1, mod=True, out_type=kind, in_place=y_norm == 1)
 
 
 def test_in_place_no_output_and_no_branch(cuda):
