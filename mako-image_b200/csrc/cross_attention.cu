@@ -66,6 +66,7 @@ struct CrossParams {
     int q_head, q_sample, kv_head_k, kv_sample_k, kv_head_v, kv_sample_v, o_head, o_sample;
     int items, blocks;  // work items, query blocks of 256 rows
     int splits;         // SPLIT: CTAs of a cluster
+    int in_step;        // every item gives both softmax groups work
 };
 
 __device__ __forceinline__ float ex2(float x)
@@ -262,7 +263,8 @@ __device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, float4 v)
 
 constexpr int kMaxSplits = 8;
 
-template <int D, bool SPLIT>
+// HIDE: with key lengths or a mask (the code for them, even where it is not run, costs a plain call 4 to 8%).
+template <int D, bool SPLIT, bool HIDE>
 __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ CrossParams P)
 {
     using C = Cfg<D, SPLIT>;
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                         !outputs(tile, g < 2, g + 2 >= steps, dv0 + s * kUnit, width(g)))
                         return false;
                     free_slot(&kv_empty[s]);
-                    if (a.key_mask)
+                    if (HIDE && a.key_mask)
                         free_slot(&h_empty[g % kHideSteps]);
                     return g + 2 >= steps || score(tile, g + 2);
                 };
@@ -499,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 if (!ok)
                     break;
                 if (elect_one_sync()) {
-                    if (a.key_mask)  // the step's weights are made, so its bounds have been read
+                    if (HIDE && a.key_mask)  // the step's weights are made, so its bounds have been read
                         mma_commit(&h_empty[step % kHideSteps]);
                     mma_commit(&kv_empty[sv]);
                     if (more)
@@ -513,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             mbar_wait(drain, 0, a.status, kErrWaitDrain, nullptr);
         }
     } else if (warp == 2) {
-        if (a.key_mask) {
+        if (HIDE && a.key_mask) {
             Walk<SPLIT> w;
             uint32_t step = 0;
             for (w.first(P); w.more(P); w.next(P), ++step) {
@@ -573,38 +575,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             float m = -INFINITY, l = 0.0f;
             const int stride = both ? 2 : 1, begin = it.lo + (both ? t : 0);
             for (int j = begin; j < it.hi; j += stride, step += stride) {
-                if (!mbar_wait(&s_full[t], ns & 1, a.status, kErrAttnWait, abort_flag)) {
-                    ok = false;
-                    break;
-                }
-                ++ns;
-                tc_fence_after();
                 const int valid = it.n - j * kTile;
                 int tail = valid >= kTile || valid % 32 == 0 ? 32 : valid % 32;
                 uint32_t masked = 0;
                 const float* bound = bounds + step % kHideSteps * kTile;
-                if (a.key_mask) {  // after the scores: a tile that skipped items may be phases ahead of the bounds until then
-                    const uint32_t s = step % kHideSteps;
-                    if (!mbar_wait(&h_full[s], (step / kHideSteps) & 1, a.status, kErrAttnWait, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
-                    masked = maskeds[s];
-                    tail = 32;  // the bounds know of it
-                }
-                switch (min(4, (valid + 31) >> 5)) {
-                case 1: softmax_step<D, 1>(ts, to, tail, masked, bound, a.scale_log2, j == begin, m, l); break;
-                case 2: softmax_step<D, 2>(ts, to, tail, masked, bound, a.scale_log2, j == begin, m, l); break;
-                case 3: softmax_step<D, 3>(ts, to, tail, masked, bound, a.scale_log2, j == begin, m, l); break;
-                default: softmax_step<D, 4>(ts, to, tail, masked, bound, a.scale_log2, j == begin, m, l); break;
-                }
-                if (masked || (valid < kTile && it.n < a.Lk)) {
-                    // Rows of V that are multiplied (those up to valid, in sixteens) and belong to hidden keys: both tiles'
-                    // threads clear them, whichever comes first. V stays until both tiles' products have read it.
-                    if (!mbar_wait(&v_full[step % kSteps], (step / kSteps) & 1, a.status, kErrAttnWait, abort_flag)) {
-                        ok = false;
-                        break;
-                    }
+                uint64_t* v_here = &v_full[step % kSteps];
+                const uint32_t v_phase = (step / kSteps) & 1;
+                // Rows of V that are multiplied (those up to valid, in sixteens) and belong to hidden keys: both tiles' threads
+                // clear them, whichever comes first. V stays until both tiles' products have read it.
+                const auto clear = [&] {
                     if (r < ((valid + 15) & ~15) && (a.key_mask ? bound[r] < 0.0f : r >= valid)) {
                         uint8_t* row = sKV + (2 * step + 1) % NS * TB + r * 128;
 #pragma unroll
@@ -614,6 +593,50 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                                 *reinterpret_cast<uint4*>(row + p * kPanel + ((i ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
                     }
                     fence_proxy_async_smem();
+                };
+                const auto look = [&] {  // the mask's word on this step
+                    if (!HIDE || !a.key_mask)
+                        return true;
+                    const uint32_t s = step % kHideSteps;
+                    if (!mbar_wait(&h_full[s], (step / kHideSteps) & 1, a.status, kErrAttnWait, abort_flag))
+                        return false;
+                    masked = maskeds[s];
+                    tail = 32;  // the bounds know of it
+                    return true;
+                };
+                // While the scores are on their way, as far as the mask and V are there. Not where this group may have skipped
+                // items: until its scores have come it could then take an older phase of a barrier for its own.
+                bool cleared = false;
+                if (HIDE && P.in_step) {
+                    ok = look();
+                    if (ok && (masked || (valid < kTile && it.n < a.Lk)) &&
+                        __all_sync(0xffffffffu, mbar_try_wait(smem_u32(v_here), v_phase))) {
+                        clear();
+                        cleared = true;
+                    }
+                }
+                if (!ok || !mbar_wait(&s_full[t], ns & 1, a.status, kErrAttnWait, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                ++ns;
+                tc_fence_after();
+                if (HIDE && !P.in_step && !look()) {
+                    ok = false;
+                    break;
+                }
+                switch (min(4, (valid + 31) >> 5)) {
+                case 1: softmax_step<D, 1>(ts, to, tail, masked, bound, a.scale_log2, j == begin, m, l); break;
+                case 2: softmax_step<D, 2>(ts, to, tail, masked, bound, a.scale_log2, j == begin, m, l); break;
+                case 3: softmax_step<D, 3>(ts, to, tail, masked, bound, a.scale_log2, j == begin, m, l); break;
+                default: softmax_step<D, 4>(ts, to, tail, masked, bound, a.scale_log2, j == begin, m, l); break;
+                }
+                if (HIDE && !cleared && (masked || (valid < kTile && it.n < a.Lk))) {
+                    if (!mbar_wait(v_here, v_phase, a.status, kErrAttnWait, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    clear();
                 }
                 tc_fence_before();
                 mbar_arrive(&p_full[t]);
@@ -1042,12 +1065,12 @@ bool encode_heads(CUtensorMap* m, const void* p, const HeadStrides& s, int rows,
 
 // A one-time check that the compiled register count holds the warpgroups' split (otherwise the softmax groups' increase
 // could never be granted), and the shared memory limit on each device.
-template <int D, bool SPLIT>
+template <int D, bool SPLIT, bool HIDE>
 cudaError_t setup()
 {
     static const cudaError_t regs = [] {
         cudaFuncAttributes fa{};
-        const cudaError_t e = cudaFuncGetAttributes(&fa, k_cross<D, SPLIT>);
+        const cudaError_t e = cudaFuncGetAttributes(&fa, k_cross<D, SPLIT, HIDE>);
         if (e != cudaSuccess)
             return e;
         return fa.numRegs * kThreads < 128 * kRegsCtl + 256 * kRegsSoftmax ? cudaErrorInvalidConfiguration
@@ -1056,10 +1079,10 @@ cudaError_t setup()
     if (regs != cudaSuccess)
         return regs;
     static std::atomic<uint64_t> devs{0};
-    return smem_limit_once(devs, k_cross<D, SPLIT>, Cfg<D, SPLIT>::kSmem);
+    return smem_limit_once(devs, k_cross<D, SPLIT, HIDE>, Cfg<D, SPLIT>::kSmem);
 }
 
-// Clusters of `size` CTAs of k_cross<D, true> that the current device runs at once (they have to fit its GPCs), kept for
+// Clusters of `size` CTAs of the split kernel that the current device runs at once (they have to fit its GPCs), kept for
 // devices 0..63 once asked.
 template <int D>
 int clusters_at_once(int size)
@@ -1082,7 +1105,8 @@ int clusters_at_once(int size)
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (setup<D, true>() != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, k_cross<D, true>, &cfg) != cudaSuccess) {
+    if (setup<D, true, true>() != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k_cross<D, true, true>, &cfg) != cudaSuccess) {
         cudaGetLastError();
         return 0;
     }
@@ -1101,19 +1125,19 @@ int splits_of(int items, int steps)
     return 1;
 }
 
-template <int D>
+template <int D, bool HIDE>
 cudaError_t launch(const CrossParams& P, cudaStream_t st)
 {
     if (P.splits > 1) {
-        const cudaError_t e = setup<D, true>();
+        const cudaError_t e = setup<D, true, HIDE>();
         return e != cudaSuccess ? e
-                                : launch_k_cluster(k_cross<D, true>, dim3(P.items * P.splits), P.splits, kThreads,
+                                : launch_k_cluster(k_cross<D, true, HIDE>, dim3(P.items * P.splits), P.splits, kThreads,
                                                    Cfg<D, true>::kSmem, st, P);
     }
-    const cudaError_t e = setup<D, false>();
-    return e != cudaSuccess
-               ? e
-               : launch_k(k_cross<D, false>, dim3(std::min(P.items, num_sms())), kThreads, Cfg<D, false>::kSmem, st, P);
+    const cudaError_t e = setup<D, false, HIDE>();
+    return e != cudaSuccess ? e
+                            : launch_k(k_cross<D, false, HIDE>, dim3(std::min(P.items, num_sms())), kThreads,
+                                       Cfg<D, false>::kSmem, st, P);
 }
 
 template <int D, int R>
@@ -1162,6 +1186,7 @@ cudaError_t cross_attention(const CrossArgs& args, const char** err, cudaStream_
     P.a = a;
     P.blocks = (a.Lq + 2 * kTile - 1) / (2 * kTile);
     P.items = a.B * a.H * P.blocks;
+    P.in_step = a.Lq > kTile && (a.Lq - 1) % (2 * kTile) >= kTile;
     const int steps = (a.Lk + kTile - 1) / kTile;
     P.splits = a.d == 64 ? splits_of<64>(P.items, steps) : splits_of<128>(P.items, steps);
     if (!encode_heads(&P.tq, a.q, a.sq, a.Lq, a.H, a.B, a.d, kTile, &P.q_head, &P.q_sample) ||
@@ -1171,7 +1196,9 @@ cudaError_t cross_attention(const CrossArgs& args, const char** err, cudaStream_
         *err = "cross_attention: tensor map encoding failed";
         return cudaErrorInvalidValue;
     }
-    const cudaError_t e = a.d == 64 ? launch<64>(P, st) : launch<128>(P, st);
+    const bool hide = a.key_len || a.key_mask;
+    const cudaError_t e = a.d == 64 ? (hide ? launch<64, true>(P, st) : launch<64, false>(P, st))
+                                    : (hide ? launch<128, true>(P, st) : launch<128, false>(P, st));
     if (e != cudaSuccess)
         return e;
     count_launch();
