@@ -263,8 +263,9 @@ __device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, float4 v)
 
 constexpr int kMaxSplits = 8;
 
-// HIDE: with key lengths or a mask (the code for them, even where it is not run, costs a plain call 4 to 8%).
-template <int D, bool SPLIT, bool HIDE>
+// HIDE: which keys may be hidden (the code for a mask, even where it is not run, costs a plain call 4 to 8%).
+enum Hide : int { kHideNone = 0, kHideLengths = 1, kHideMask = 2 };
+template <int D, bool SPLIT, int HIDE>
 __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ CrossParams P)
 {
     using C = Cfg<D, SPLIT>;
@@ -464,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                         !outputs(tile, g < 2, g + 2 >= steps, dv0 + s * kUnit, width(g)))
                         return false;
                     free_slot(&kv_empty[s]);
-                    if (HIDE && a.key_mask)
+                    if (HIDE == kHideMask)
                         free_slot(&h_empty[g % kHideSteps]);
                     return g + 2 >= steps || score(tile, g + 2);
                 };
@@ -501,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 if (!ok)
                     break;
                 if (elect_one_sync()) {
-                    if (HIDE && a.key_mask)  // the step's weights are made, so its bounds have been read
+                    if (HIDE == kHideMask)  // the step's weights are made, so its bounds have been read
                         mma_commit(&h_empty[step % kHideSteps]);
                     mma_commit(&kv_empty[sv]);
                     if (more)
@@ -515,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
             mbar_wait(drain, 0, a.status, kErrWaitDrain, nullptr);
         }
     } else if (warp == 2) {
-        if (HIDE && a.key_mask) {
+        if (HIDE == kHideMask) {
             Walk<SPLIT> w;
             uint32_t step = 0;
             for (w.first(P); w.more(P); w.next(P), ++step) {
@@ -584,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 // Rows of V that are multiplied (those up to valid, in sixteens) and belong to hidden keys: both tiles' threads
                 // clear them, whichever comes first. V stays until both tiles' products have read it.
                 const auto clear = [&] {
-                    if (r < ((valid + 15) & ~15) && (a.key_mask ? bound[r] < 0.0f : r >= valid)) {
+                    if (r < ((valid + 15) & ~15) && (HIDE == kHideMask ? bound[r] < 0.0f : r >= valid)) {
                         uint8_t* row = sKV + (2 * step + 1) % NS * TB + r * 128;
 #pragma unroll
                         for (int p = 0; p < D / 64; ++p)
@@ -595,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                     fence_proxy_async_smem();
                 };
                 const auto look = [&] {  // the mask's word on this step
-                    if (!HIDE || !a.key_mask)
+                    if (HIDE != kHideMask)
                         return true;
                     const uint32_t s = step % kHideSteps;
                     if (!mbar_wait(&h_full[s], (step / kHideSteps) & 1, a.status, kErrAttnWait, abort_flag))
@@ -607,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 // While the scores are on their way, as far as the mask and V are there. Not where this group may have skipped
                 // items: until its scores have come it could then take an older phase of a barrier for its own.
                 bool cleared = false;
-                if (HIDE && P.in_step) {
+                if (HIDE == kHideMask && P.in_step) {
                     ok = look();
                     if (ok && (masked || (valid < kTile && it.n < a.Lk)) &&
                         __all_sync(0xffffffffu, mbar_try_wait(smem_u32(v_here), v_phase))) {
@@ -621,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
                 }
                 ++ns;
                 tc_fence_after();
-                if (HIDE && !P.in_step && !look()) {
+                if (HIDE == kHideMask && !P.in_step && !look()) {
                     ok = false;
                     break;
                 }
@@ -1065,7 +1066,7 @@ bool encode_heads(CUtensorMap* m, const void* p, const HeadStrides& s, int rows,
 
 // A one-time check that the compiled register count holds the warpgroups' split (otherwise the softmax groups' increase
 // could never be granted), and the shared memory limit on each device.
-template <int D, bool SPLIT, bool HIDE>
+template <int D, bool SPLIT, int HIDE>
 cudaError_t setup()
 {
     static const cudaError_t regs = [] {
@@ -1105,8 +1106,8 @@ int clusters_at_once(int size)
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     int n = 0;
-    if (setup<D, true, true>() != cudaSuccess ||
-        cudaOccupancyMaxActiveClusters(&n, k_cross<D, true, true>, &cfg) != cudaSuccess) {
+    if (setup<D, true, kHideMask>() != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k_cross<D, true, kHideMask>, &cfg) != cudaSuccess) {
         cudaGetLastError();
         return 0;
     }
@@ -1125,7 +1126,7 @@ int splits_of(int items, int steps)
     return 1;
 }
 
-template <int D, bool HIDE>
+template <int D, int HIDE>
 cudaError_t launch(const CrossParams& P, cudaStream_t st)
 {
     if (P.splits > 1) {
@@ -1138,6 +1139,14 @@ cudaError_t launch(const CrossParams& P, cudaStream_t st)
     return e != cudaSuccess ? e
                             : launch_k(k_cross<D, false, HIDE>, dim3(std::min(P.items, num_sms())), kThreads,
                                        Cfg<D, false>::kSmem, st, P);
+}
+
+template <int D>
+cudaError_t launch(const CrossParams& P, cudaStream_t st)
+{
+    return P.a.key_mask  ? launch<D, kHideMask>(P, st)
+           : P.a.key_len ? launch<D, kHideLengths>(P, st)
+                         : launch<D, kHideNone>(P, st);
 }
 
 template <int D, int R>
@@ -1196,9 +1205,7 @@ cudaError_t cross_attention(const CrossArgs& args, const char** err, cudaStream_
         *err = "cross_attention: tensor map encoding failed";
         return cudaErrorInvalidValue;
     }
-    const bool hide = a.key_len || a.key_mask;
-    const cudaError_t e = a.d == 64 ? (hide ? launch<64, true>(P, st) : launch<64, false>(P, st))
-                                    : (hide ? launch<128, true>(P, st) : launch<128, false>(P, st));
+    const cudaError_t e = a.d == 64 ? launch<64>(P, st) : launch<128>(P, st);
     if (e != cudaSuccess)
         return e;
     count_launch();
