@@ -345,8 +345,9 @@ struct Vectors {
 // A block a run of `run` rows of one sample, NC chunks of 32 * VEC values a warp and row. n is a multiple of VEC. KEEP: the
 // vectors stay in shared memory from row to row and each row is loaded while the one before is worked on (otherwise a run is one
 // row).
-template <int VEC, int NC, bool KEEP>
-__global__ void __launch_bounds__(512, KEEP ? 2 : 1) k_gate_norm(const GateNormArgs a, int run)
+// T: threads at most; up to 256 leave 85 registers each for three blocks an SM, the widest rows take an SM's for one block.
+template <int VEC, int NC, bool KEEP, int T>
+__global__ void __launch_bounds__(T, KEEP && NC * VEC <= 12 ? (T == 256 ? 3 : 2) : 1) k_gate_norm(const GateNormArgs a, int run)
 {
     __shared__ float red[2][5][16];
     grid_dep_wait();
@@ -472,8 +473,9 @@ __global__ void __launch_bounds__(512) k_quant_long(const QuantRowsArgs a)
 bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 // How a row of `chunks` chunks is dealt out: NC chunks a warp (at most `most`) on up to 16 warps, with few idle chunk places.
-// Among equals the gated add takes more warps, whose barriers it waits for while the next row is on its way (8704 x 3072 to
-// int8: 63 us on 12 warps a row, 67 on 8), and plain quantising fewer (8192 x 3072: 15.5 us on 3 warps a row, 21 on 6 or 12).
+// Among equals fewer warps where there are many rows (8704 x 3072 to int8: 60 us on 8 warps a row, 63 on 12; plain quantising
+// 8192 x 3072: 15.5 us on 3 warps a row, 21 on 6 or 12), more where there are few, as that shortens a block's way from its
+// loads to its stores (154 x 1280: 2.6 us on 10 warps a row, 3.2 on 5).
 struct Deal {
     int nc, warps;
 };
@@ -489,14 +491,14 @@ Deal deal(int chunks, int most, bool few_warps)
     return best;
 }
 
-template <int VEC, int NC, bool KEEP>
-cudaError_t launch_gate_norm(const GateNormArgs& a, int warps, cudaStream_t st)
+template <int VEC, int NC, bool KEEP, int T>
+cudaError_t launch_gate_norm_of(const GateNormArgs& a, int warps, cudaStream_t st)
 {
     const long samples = (a.rows + a.rows_per_sample - 1) / a.rows_per_sample;
     const size_t smem = KEEP ? size_t(3) * a.n * sizeof(float) : 0;
     if (smem > 48 * 1024) {
         static std::atomic<uint64_t> devs{0};
-        const cudaError_t e = smem_limit_once(devs, k_gate_norm<VEC, NC, KEEP>, 3 * 6144 * int(sizeof(float)));
+        const cudaError_t e = smem_limit_once(devs, k_gate_norm<VEC, NC, KEEP, T>, 3 * kGateNormMaxWidth * int(sizeof(float)));
         if (e != cudaSuccess)
             return e;
     }
@@ -505,14 +507,23 @@ cudaError_t launch_gate_norm(const GateNormArgs& a, int warps, cudaStream_t st)
     if (KEEP && a.rows > 2L * num_sms()) {
         int resident = 1;
         const cudaError_t e =
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, k_gate_norm<VEC, NC, KEEP>, 32 * warps, smem);
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, k_gate_norm<VEC, NC, KEEP, T>, 32 * warps, smem);
         if (e != cudaSuccess)
             return e;
         const long wave = long(num_sms()) * std::max(1, resident);
         run = int(std::min(a.rows_per_sample, std::max(1L, (a.rows + wave - 1) / wave)));
     }
-    return launch_k(k_gate_norm<VEC, NC, KEEP>, dim3(unsigned(samples * ((a.rows_per_sample + run - 1) / run))), 32 * warps,
+    return launch_k(k_gate_norm<VEC, NC, KEEP, T>, dim3(unsigned(samples * ((a.rows_per_sample + run - 1) / run))), 32 * warps,
                     smem, st, a, run);
+}
+
+template <int VEC, int NC, bool KEEP>
+cudaError_t launch_gate_norm(const GateNormArgs& a, int warps, cudaStream_t st)
+{
+    if constexpr (KEEP && NC * VEC <= 12)
+        if (warps <= 8)
+            return launch_gate_norm_of<VEC, NC, KEEP, 256>(a, warps, st);
+    return launch_gate_norm_of<VEC, NC, KEEP, 512>(a, warps, st);
 }
 
 template <typename XT, int VEC, int NC>
@@ -539,13 +550,13 @@ cudaError_t gate_norm(const GateNormArgs& args, cudaStream_t st)
     cudaError_t e;
     if (vec) {
         const int chunks = (a.n + 127) / 128;
-        const Deal d = deal(chunks, chunks <= 48 ? 3 : 6, false);
+        const Deal d = deal(chunks, chunks <= 48 ? 3 : 6, a.rows > 2L * num_sms());
         e = d.nc == 1   ? launch_gate_norm<4, 1, true>(a, d.warps, st)
             : d.nc == 2 ? launch_gate_norm<4, 2, true>(a, d.warps, st)
             : d.nc == 3 ? launch_gate_norm<4, 3, true>(a, d.warps, st)
-            : d.nc == 4 ? launch_gate_norm<4, 4, false>(a, d.warps, st)
-            : d.nc == 5 ? launch_gate_norm<4, 5, false>(a, d.warps, st)
-                        : launch_gate_norm<4, 6, false>(a, d.warps, st);
+            : d.nc == 4 ? launch_gate_norm<4, 4, true>(a, d.warps, st)
+            : d.nc == 5 ? launch_gate_norm<4, 5, true>(a, d.warps, st)
+                        : launch_gate_norm<4, 6, true>(a, d.warps, st);
     } else {
         const int chunks = (a.n + 31) / 32;
         if (chunks <= 64)
