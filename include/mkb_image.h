@@ -199,8 +199,9 @@ mkb_status mkb_quantize_rows(const void* x, long ldx, int x_f32, int8_t* q, long
 
 /* y[m][n] = act(x_scale[m] * w_scale[n] * sum_k x[m][k] w[n][k] + bias[n]): mkb_proj on 8-bit integers, with the scale of
  * each token (mkb_quantize_rows of the activations) and of each output channel (mkb_quantize_rows of the weight's rows).
- * The sums are exact 32-bit integers (K <= 131071). x and w are 16-byte aligned with ldx and ldw multiples of 16 (K itself
- * may be any: what lies between K and the row's end is not read as data); y is bf16 (out_f32 = 0) or fp32, any ldy >= N. */
+ * The sums are exact 32-bit integers (K <= 131071; M and N up to 2^30, and no more 128 x 128 tiles than that). x and w are
+ * 16-byte aligned with ldx and ldw multiples of 16 (K itself may be any: what lies between K and the row's end is not read
+ * as data); y is bf16 (out_f32 = 0) or fp32, any ldy >= N. */
 mkb_status mkb_proj_i8(const int8_t* x, long ldx, const float* x_scale, const int8_t* w, long ldw, const float* w_scale,
                        const float* bias, void* y, long ldy, int M, int N, int K, int act, int out_f32, void* stream);
 

@@ -440,8 +440,8 @@ mkb_status mkb_proj_i8(const int8_t* x, long ldx, const float* x_scale, const in
         return fail(MKB_ERR_INVALID, "proj_i8: unknown activation");
     if (M < 0 || N <= 0 || K <= 0 || K > kI8MaxK)
         return fail(MKB_ERR_INVALID, "proj_i8: need M >= 0, N > 0 and 0 < K <= 131071 (exact 32-bit sums)");
-    if (double((M + 127L) / 128) * double((N + 127L) / 128) > double(1 << 30))
-        return fail(MKB_ERR_INVALID, "proj_i8: more than 2^30 output tiles of 128 x 128");
+    if (M > (1 << 30) || N > (1 << 30) || double((M + 127L) / 128) * double((N + 127L) / 128) > double(1 << 30))
+        return fail(MKB_ERR_INVALID, "proj_i8: need M, N <= 2^30 and no more than 2^30 output tiles of 128 x 128");
     if (ldx < K || ldw < K || ldy < N || (ldx & 15) || (ldw & 15))
         return fail(MKB_ERR_INVALID, "proj_i8: need ldx, ldw >= K and multiples of 16, ldy >= N");
     if (M == 0)

@@ -39,7 +39,8 @@ PROJ = dict(x=P, ldx=64, xs=P, w=P, ldw=64, ws=P, bias=None, y=P, ldy=32, M=4, N
     (dict(K=131072, ldx=131072, ldw=131072), "131071"), (dict(N=0), "N > 0"), (dict(M=-1), "M >= 0"),
     (dict(ldx=72), "16"), (dict(ldw=40), "16"), (dict(ldx=48), "ldx"), (dict(ldy=31), "ldy"), (dict(x=P + 8), "alignment"),
     (dict(w=P + 8), "alignment"), (dict(y=P + 1), "alignment"), (dict(y=P + 2, f32=1), "alignment"),
-    (dict(bias=P + 1), "alignment"), (dict(M=(1 << 31) - 1, N=1 << 20, ldy=1 << 20), "2^30 output tiles")])
+    (dict(bias=P + 1), "alignment"), (dict(M=(1 << 31) - 1, N=1 << 20, ldy=1 << 20), "2^30 output tiles"),
+    (dict(M=1, N=(1 << 31) - 1, ldy=1 << 31), "N <= 2^30"), (dict(M=(1 << 31) - 1), "N <= 2^30")])
 def test_proj_i8_refuses(change, word):
     _refused(mkimage.lib.mkb_proj_i8, _with(PROJ, **change), word)
 
