@@ -88,40 +88,6 @@ __device__ __forceinline__ void act_out(float (&v)[N], int act, bool f32)
         act_all<true>(v, act);
 }
 
-// N consecutive columns of a row, as far as they exist, in the widest stores the address allows.
-template <int N>
-__device__ __forceinline__ void store_row(const GemmI8Args& a, long row, int col, const float (&v)[N])
-{
-    const int n = min(N, a.N - col);
-    if (a.out_f32) {
-        float* p = static_cast<float*>(a.y) + row * a.ldy + col;
-        if (n == N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-#pragma unroll
-            for (int j = 0; j < N; j += 4)
-                *reinterpret_cast<float4*>(p + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (j < n)
-                    p[j] = v[j];
-        }
-    } else {
-        __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.y) + row * a.ldy + col;
-        if (n == N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-#pragma unroll
-            for (int j = 0; j < N; j += 8)
-                *reinterpret_cast<uint4*>(p + j) =
-                    make_uint4(pack_bf16x2(v[j], v[j + 1]), pack_bf16x2(v[j + 2], v[j + 3]),
-                               pack_bf16x2(v[j + 4], v[j + 5]), pack_bf16x2(v[j + 6], v[j + 7]));
-        } else {
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-                if (j < n)
-                    p[j] = __float2bfloat16(v[j]);
-        }
-    }
-}
-
 // ------------------------------------------------------------------------------------------------ few rows
 
 constexpr int kRowsMax = 2;
@@ -447,11 +413,12 @@ template <int BN>
 struct PairCfg {
     static constexpr int kABytes = 128 * kBK, kBBytes = BN / 2 * kBK, kStageBytes = kABytes + kBBytes;
     static constexpr int kBox = 32 * 128;  // a warp's box: 32 rows of 128 bytes
-    static constexpr int kStages = BN == 256 ? 6 : 8;
+    static constexpr int kStages = BN == 256 ? 6 : BN > 128 ? 7 : 8;
+    static constexpr int kBf16Cols = BN % 64 == 0 ? 64 : 32;  // bf16 columns of a box: 32 where a tile is no multiple of 64
     static constexpr int kVec = 2 * 2 * BN * 4;  // w_scale and bias of two tiles
     static constexpr int kSmem = 1024 + kStages * kStageBytes + 4 * kBox + kVec + 256;
-    static constexpr int kTmemCols = 2 * BN;
-    static_assert(kSmem <= 227 * 1024);
+    static constexpr int kTmemCols = BN > 128 ? 512 : 256;  // two accumulators, a power of two
+    static_assert(kStageBytes % 1024 == 0 && kSmem <= 227 * 1024);
 };
 
 // Tiles in groups of 8 along M, so that concurrent tiles share panels of x and W in L2.
@@ -461,6 +428,27 @@ __device__ __forceinline__ void tile_of(int tile, int num_m, int num_n, int& mb,
     const int gsize = min(num_m - first, 8), t = tile - group * per_group;
     mb = first + t % gsize;
     nb = t / gsize;
+}
+
+// A warp's 32 x 32 values, staged as fp32 in rows of swizzled 16-byte pieces, to rows of any alignment: a lane a column, a row
+// at a time. The values come back 16 at a time ahead of their stores: the compiler keeps a load behind a store that might be to
+// the same place (one at a time 22.5 us at 2300 x 2100 x 2048 to bf16, 8 17.8, 16 17.6, 32 21.0).
+template <typename T>
+__device__ __forceinline__ void store_box(T* p, long ldy, const uint8_t* box, int rows, int cols, int lane)
+{
+    const uint8_t* from = box + (lane & 3) * 4;
+    p += lane;
+#pragma unroll 1
+    for (int i = 0; i < 32; i += 16, p += 16 * ldy) {
+        float x[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+            x[k] = *reinterpret_cast<const float*>(from + (i + k) * 128 + (((lane >> 2) ^ (k & 7)) << 4));
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+            if (i + k < rows && lane < cols)
+                p[k * ldy] = T(x[k]);
+    }
 }
 
 // Persistent CTA pairs. Warp 0 of each CTA loads its 128 rows of x and its half of the W tile by TMA, the leader's warp 1
@@ -621,13 +609,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(co
                 }
                 act_out(v, a.act, a.out_f32);
                 if (!P.boxes) {
-                    if (row < a.M)
-                        store_row(a, row, n0 + c, v);
+                    // Rows that TMA cannot address: through the box as fp32 and out along the rows (a thread storing its own
+                    // row: 45 against 17.6 us at 2300 x 2100 x 2048 to bf16, 81 against 21.5 at 8000 x 777 x 1000).
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                            make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    __syncwarp();
+                    const long to = row0 * a.ldy + n0 + c;
+                    const int rows = a.M - row0, cols = a.N - n0 - c;
+                    if (a.out_f32)
+                        store_box(static_cast<float*>(a.y) + to, a.ldy, box, rows, cols, lane);
+                    else
+                        store_box(static_cast<__nv_bfloat16*>(a.y) + to, a.ldy, box, rows, cols, lane);
                     continue;
                 }
-                // A box holds 128 bytes of each row: 32 fp32 columns, or two rounds of 32 bf16 ones.
-                const int half = a.out_f32 ? 0 : (c >> 5) & 1;
-                uint8_t* bx = box + lane * 128;
+                // A box holds 128 bytes of each row: 32 fp32 columns, or two rounds of 32 bf16 ones; or 64 bytes, one round.
+                constexpr bool kTwo = C::kBf16Cols == 64;
+                const int half = a.out_f32 || !kTwo ? 0 : (c >> 5) & 1;
+                uint8_t* bx = box + lane * (kTwo || a.out_f32 ? 128 : 64);
                 if (half == 0) {
                     if (lane == 0)
                         bulk_wait_read<0>();  // the last store has read the box
@@ -641,11 +642,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(co
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        *reinterpret_cast<uint4*>(bx + (((4 * half + j) ^ (lane & 7)) << 4)) =
+                        *reinterpret_cast<uint4*>(bx + (((4 * half + j) ^ (kTwo ? lane & 7 : (lane >> 1) & 3)) << 4)) =
                             make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
                                        pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
                 }
-                if (a.out_f32 || half == 1 || n0 + c + 32 >= a.N) {
+                if (a.out_f32 || !kTwo || half == 1 || n0 + c + 32 >= a.N) {
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
@@ -691,7 +692,7 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn()
 }
 
 bool encode_2d(CUtensorMap* m, CUtensorMapDataType type, const void* p, long inner, long outer, long row_bytes,
-               int box_inner, int box_outer)
+               int box_inner, int box_outer, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B)
 {
     auto fn = encode_fn();
     const cuuint64_t dims[2] = {cuuint64_t(inner), cuuint64_t(outer)};
@@ -699,7 +700,7 @@ bool encode_2d(CUtensorMap* m, CUtensorMapDataType type, const void* p, long inn
     const cuuint32_t box[2] = {cuuint32_t(box_inner), cuuint32_t(box_outer)};
     const cuuint32_t es[2] = {1, 1};
     return fn && fn(m, type, 2, const_cast<void*>(p), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -732,8 +733,18 @@ cudaError_t launch_few(I8Params& P, cudaStream_t st)
 }
 
 template <int BN>
-cudaError_t launch_pair(const I8Params& P, int tiles, cudaStream_t st)
+cudaError_t launch_pair(I8Params& P, const char** err, cudaStream_t st)
 {
+    const GemmI8Args& a = P.a;
+    const int size = a.out_f32 ? 4 : 2, cols = a.out_f32 ? 32 : PairCfg<BN>::kBf16Cols;
+    P.boxes = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.ldy * size) % 16 == 0;
+    if (P.boxes && !encode_2d(&P.ty, a.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.N,
+                              a.M, a.ldy * size, cols, 32,
+                              cols * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B)) {
+        *err = "proj_i8: tensor map encoding failed";
+        return cudaErrorInvalidValue;
+    }
+    const int tiles = int((a.M + 255L) / 256 * ((a.N + BN - 1L) / BN));
     static std::atomic<uint64_t> devs{0};
     const cudaError_t e = smem_limit_once(devs, k_i8_pair<BN>, PairCfg<BN>::kSmem);
     if (e != cudaSuccess)
@@ -760,11 +771,18 @@ cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
         while (few_bn < 64 && (a.M + few_bn - 1L) / few_bn * ((a.N + 127L) / 128) > num_sms())
             few_bn *= 2;
         const bool few = a.M <= 64 || few_bn <= 32;
-        // Pair tiles of 256 or 128 columns: whichever has the shorter rounds, 256 among equals (half the shared-memory traffic
-        // of x a product: 512 x 9216 x 3072 in one round of 256 15.0 us, in two of 128 17.3).
+        // Pair tiles of 256, 192, 160 or 128 columns: a round of tiles takes about as long as its columns and 128 more (its rows
+        // of x, the way in and out), so the width whose rounds take least, the widest among equals. In us, 256, 192, 160, 128
+        // columns: 4097 x 1280 x 5120 31.5, 26.2, 25.3, 32.7; 700 x 8192 x 1024 14.7, 12.8, 15.6, 14.7; 512 x 9216 x 3072
+        // 15.3, 18.3, 17.6, 17.1; 1000 x 1536 x 1536 10.2, 8.7, 8.2, 7.8.
         const long slots = num_sms() / 2;
-        const auto rounds = [&](int bn) { return (((a.M + 255L) / 256) * ((a.N + bn - 1L) / bn) + slots - 1) / slots; };
-        const int bn = rounds(256) * 2 <= rounds(128) ? 256 : 128;
+        const auto cost = [&](int bn) {
+            return (((a.M + 255L) / 256) * ((a.N + bn - 1L) / bn) + slots - 1) / slots * (bn + 128);
+        };
+        int bn = 256;
+        for (const int width : {192, 160, 128})
+            if (cost(width) < cost(bn))
+                bn = width;
         const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
         if (!encode_2d(&P.tx, u8, a.x, a.K, a.M, a.ldx, kBK, few ? few_bn : 128) ||
             !encode_2d(&P.tw, u8, a.w, a.K, a.N, a.ldw, kBK, few ? 128 : bn / 2)) {
@@ -776,15 +794,10 @@ cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
                 : few_bn == 32 ? launch_few<32>(P, st)
                                : launch_few<64>(P, st);
         } else {
-            const int size = a.out_f32 ? 4 : 2;
-            P.boxes = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.ldy * size) % 16 == 0;
-            if (P.boxes && !encode_2d(&P.ty, a.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                                      a.y, a.N, a.M, a.ldy * size, 128 / size, 32)) {
-                *err = "proj_i8: tensor map encoding failed";
-                return cudaErrorInvalidValue;
-            }
-            const int tiles = int((a.M + 255L) / 256 * ((a.N + bn - 1L) / bn));
-            e = bn == 256 ? launch_pair<256>(P, tiles, st) : launch_pair<128>(P, tiles, st);
+            e = bn == 256   ? launch_pair<256>(P, err, st)
+                : bn == 192 ? launch_pair<192>(P, err, st)
+                : bn == 160 ? launch_pair<160>(P, err, st)
+                            : launch_pair<128>(P, err, st);
         }
     }
     if (e != cudaSuccess)

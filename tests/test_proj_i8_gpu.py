@@ -111,6 +111,25 @@ def test_largest_sums_are_exact(cuda, M):
     assert bool((out == float(128 * 128 * K)).all())
 
 
+# Tiles of 160, 160, 192, 192, 128 and 256 columns on 148 SMs, whole and cut.
+@pytest.mark.parametrize("M,N", [(2000, 2560), (2000, 2467), (700, 8192), (705, 8101), (1030, 1500), (8000, 777)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_widths_of_tiles(cuda, M, N, f32):
+    """Outputs that TMA can address and ones that it cannot, inside a buffer whose other values stay."""
+    import torch
+    import mkimage
+
+    x, xs, w, ws, b = _case(cuda, M, N, 300, M + N)
+    for off, ld in ((0, (N + 63) // 32 * 32), (3, N + 8 - N % 2)):
+        buf = torch.full((M + 2, ld), 5.0, dtype=torch.float32 if f32 else torch.bfloat16, device=cuda)
+        out = buf[1:M + 1, off:off + N]
+        mkimage.ops.proj_i8(x, xs, w, ws, bias=b, out=out)
+        _check(out, x, xs, w, ws, b, 0)
+        assert bool((buf[0] == 5).all() and (buf[M + 1] == 5).all() and (buf[:, :off] == 5).all() and
+                    (buf[:, off + N:] == 5).all())
+    assert mkimage.ops.check_kernels() == 0
+
+
 @pytest.mark.parametrize("M", [2, 30, 200, 2000])
 def test_guards_and_strided_output(cuda, M):
     """Only [M][N] of a wider, longer output is written, at an unaligned place as well."""
