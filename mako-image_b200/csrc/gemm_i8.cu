@@ -38,12 +38,12 @@ __device__ __forceinline__ float act1(float v, int act)
             asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(u));
             return 0.5f * v * (1.0f + t);
         }
-        return v / (1.0f + __expf(-2.0f * u));
+        return __fdividef(v, 1.0f + __expf(-2.0f * u));
     }
     if (act == kActSilu)
-        return v / (1.0f + __expf(-v));
+        return __fdividef(v, 1.0f + __expf(-v));
     if (act == kActQuickGelu)
-        return v / (1.0f + __expf(-1.702f * v));
+        return __fdividef(v, 1.0f + __expf(-1.702f * v));
     if (act == kActGeluErf)
         return 0.5f * v * (1.0f + erff(v * 0.7071067811865476f));
     return v;
@@ -409,14 +409,16 @@ __global__ void __launch_bounds__(192, 1) k_i8_few(const __grid_constant__ I8Par
     }
 }
 
+constexpr int kEpiWarps = 8;
+constexpr int kPairThreads = 32 * (2 + kEpiWarps);
+
 template <int BN>
 struct PairCfg {
     static constexpr int kABytes = 128 * kBK, kBBytes = BN / 2 * kBK, kStageBytes = kABytes + kBBytes;
-    static constexpr int kBox = 32 * 128;  // a warp's box: 32 rows of 128 bytes
+    static constexpr int kBox = 32 * 64;  // a warp's box: 32 rows of 64 bytes
     static constexpr int kStages = BN == 256 ? 6 : BN > 128 ? 7 : 8;
-    static constexpr int kBf16Cols = BN % 64 == 0 ? 64 : 32;  // bf16 columns of a box: 32 where a tile is no multiple of 64
     static constexpr int kVec = 2 * 2 * BN * 4;  // w_scale and bias of two tiles
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + 4 * kBox + kVec + 256;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kEpiWarps * kBox + kVec + 256;
     static constexpr int kTmemCols = BN > 128 ? 512 : 256;  // two accumulators, a power of two
     static_assert(kStageBytes % 1024 == 0 && kSmem <= 227 * 1024);
 };
@@ -430,39 +432,43 @@ __device__ __forceinline__ void tile_of(int tile, int num_m, int num_n, int& mb,
     nb = t / gsize;
 }
 
-// A warp's 32 x 32 values, staged as fp32 in rows of swizzled 16-byte pieces, to rows of any alignment: a lane a column, a row
-// at a time. The values come back 16 at a time ahead of their stores: the compiler keeps a load behind a store that might be to
-// the same place (one at a time 22.5 us at 2300 x 2100 x 2048 to bf16, 8 17.8, 16 17.6, 32 21.0).
+// A warp's box, 32 rows of 64 bytes in pieces of 16 that are exchanged by the row (as TMA's 64-byte swizzle has them), to rows
+// of any alignment: a lane a column, a row or two at a time. The values come back 16 at a time ahead of their stores: the
+// compiler keeps a load behind a store that might be to the same place (one at a time 22.5 us at 2300 x 2100 x 2048 to bf16).
+__device__ __forceinline__ int box_piece(int row, int piece) { return row * 64 + ((piece ^ ((row >> 1) & 3)) << 4); }
+
 template <typename T>
 __device__ __forceinline__ void store_box(T* p, long ldy, const uint8_t* box, int rows, int cols, int lane)
 {
-    const uint8_t* from = box + (lane & 3) * 4;
-    p += lane;
+    constexpr int kCols = 64 / sizeof(T), kRows = 32 / kCols, kPiece = 16 / sizeof(T);
+    const int col = lane % kCols, row = lane / kCols;
+    p += row * ldy + col;
 #pragma unroll 1
-    for (int i = 0; i < 32; i += 16, p += 16 * ldy) {
-        float x[16];
+    for (int i = 0; i < 32; i += 16 * kRows, p += 16 * kRows * ldy) {
+        T x[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-            x[k] = *reinterpret_cast<const float*>(from + (i + k) * 128 + (((lane >> 2) ^ (k & 7)) << 4));
+            x[k] = *reinterpret_cast<const T*>(box + box_piece(i + k * kRows + row, col / kPiece) + col % kPiece * sizeof(T));
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-            if (i + k < rows && lane < cols)
-                p[k * ldy] = T(x[k]);
+            if (i + k * kRows + row < rows && col < cols)
+                p[k * kRows * ldy] = x[k];
     }
 }
 
 // Persistent CTA pairs. Warp 0 of each CTA loads its 128 rows of x and its half of the W tile by TMA, the leader's warp 1
-// issues 256 x BN x 32 MMAs into one of two accumulators, warps 2-5 of both CTAs drain the other: a thread a row, 32
-// columns at a time, through a 4 KB box a warp that leaves as a TMA store.
+// issues 256 x BN x 32 MMAs into one of two accumulators, warps 2-9 of both CTAs drain the other: a thread a row, 32 columns at
+// a time and every second 32 each, through a 2 KB box a warp that leaves as TMA stores. With four such warps and boxes of 4 KB
+// the epilogue was what the tensor pipe waited for (8192 x 12288 x 3072 with GELU 218 us, with eight 205).
 template <int BN>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(const __grid_constant__ I8Params P)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i8_pair(const __grid_constant__ I8Params P)
 {
     using C = PairCfg<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* boxes = smem + C::kStages * C::kStageBytes;
-    float* vec = reinterpret_cast<float*>(boxes + 4 * C::kBox);  // [2][w_scale, bias][BN]
-    uint64_t* full = reinterpret_cast<uint64_t*>(boxes + 4 * C::kBox + C::kVec);
+    float* vec = reinterpret_cast<float*>(boxes + kEpiWarps * C::kBox);  // [2][w_scale, bias][BN]
+    uint64_t* full = reinterpret_cast<uint64_t*>(boxes + kEpiWarps * C::kBox + C::kVec);
     uint64_t* empty = full + C::kStages;
     uint64_t* acc_full = empty + C::kStages;
     uint64_t* acc_empty = acc_full + 2;
@@ -484,7 +490,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(co
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], 2 * 128);  // the epilogue threads of both CTAs (leader's barrier)
+            mbar_init(&acc_empty[i], 2 * 32 * kEpiWarps);  // the epilogue threads of both CTAs (leader's barrier)
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -578,20 +584,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(co
             const int n0 = nb * BN, row0 = mb * 256 + int(rank) * 128 + q * 32, row = row0 + lane;
             // The tile's column vectors, into the copy that the tile before last read.
             float* sw = vec + acc * 2 * BN;
-            for (int i = et; i < BN; i += 128) {
+            for (int i = et; i < BN; i += 32 * kEpiWarps) {
                 const bool in = n0 + i < a.N;
                 sw[i] = in ? __ldg(a.w_scale + n0 + i) : 0.0f;
                 sw[BN + i] = in && a.bias ? __ldg(a.bias + n0 + i) : 0.0f;
             }
             const float sx = row < a.M ? __ldg(a.x_scale + row) : 0.0f;
             const bool got = mbar_wait(&acc_full[acc], acc_ph, a.status, kErrWaitAccFull, abort_flag);
-            // Also publishes the vectors; the four warps leave together or not at all.
-            if (named_barrier_or<1, 128>(!got))
+            // Also publishes the vectors; the warps leave together or not at all.
+            if (named_barrier_or<1, 32 * kEpiWarps>(!got))
                 break;
             tc_fence_after();
             const uint32_t t_row = tmem + (uint32_t(q * 32) << 16) + acc * BN;
 #pragma unroll 1
-            for (int c = 0; c < BN; c += 32) {
+            for (int c = 32 * ((warp - 2) >> 2); c < BN; c += 64) {
                 if (n0 + c >= a.N)
                     break;
                 uint32_t t[32];
@@ -608,52 +614,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1) k_i8_pair(co
                     v[j + 3] = fmaf(float(int(t[j + 3])) * sx, s.w, b.w);
                 }
                 act_out(v, a.act, a.out_f32);
-                if (!P.boxes) {
-                    // Rows that TMA cannot address: through the box as fp32 and out along the rows (a thread storing its own
-                    // row: 45 against 17.6 us at 2300 x 2100 x 2048 to bf16, 81 against 21.5 at 8000 x 777 x 1000).
-                    __syncwarp();
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        *reinterpret_cast<float4*>(box + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                            make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                    __syncwarp();
-                    const long to = row0 * a.ldy + n0 + c;
-                    const int rows = a.M - row0, cols = a.N - n0 - c;
-                    if (a.out_f32)
-                        store_box(static_cast<float*>(a.y) + to, a.ldy, box, rows, cols, lane);
-                    else
-                        store_box(static_cast<__nv_bfloat16*>(a.y) + to, a.ldy, box, rows, cols, lane);
-                    continue;
-                }
-                // A box holds 128 bytes of each row: 32 fp32 columns, or two rounds of 32 bf16 ones; or 64 bytes, one round.
-                constexpr bool kTwo = C::kBf16Cols == 64;
-                const int half = a.out_f32 || !kTwo ? 0 : (c >> 5) & 1;
-                uint8_t* bx = box + lane * (kTwo || a.out_f32 ? 128 : 64);
-                if (half == 0) {
+                // Through the box to columns from `col`: as a TMA store, or along rows that TMA cannot address (a thread storing
+                // its own row: 45 against 16 us at 2300 x 2100 x 2048 to bf16, 81 against 19 at 8000 x 777 x 1000) and the last
+                // columns (a cut box would write zeros as far as a piece of 16 bytes goes).
+                const auto send = [&](const uint4 (&w)[4], int col, auto* y) {
                     if (lane == 0)
                         bulk_wait_read<0>();  // the last store has read the box
                     __syncwarp();
-                }
-                if (a.out_f32) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        *reinterpret_cast<float4*>(bx + ((j ^ (lane & 7)) << 4)) =
-                            make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        *reinterpret_cast<uint4*>(bx + (((4 * half + j) ^ (kTwo ? lane & 7 : (lane >> 1) & 3)) << 4)) =
-                            make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
-                                       pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
-                }
-                if (a.out_f32 || !kTwo || half == 1 || n0 + c + 32 >= a.N) {
+                        *reinterpret_cast<uint4*>(box + box_piece(lane, j)) = w[j];
+                    if (!P.boxes || col + int(64 / sizeof(*y)) > a.N) {
+                        __syncwarp();
+                        store_box(y + row0 * a.ldy + col, a.ldy, box, a.M - row0, a.N - col, lane);
+                        return;
+                    }
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
                         if (row0 < a.M)
-                            tma_store_2d(&P.ty, box, a.out_f32 ? n0 + c : n0 + c - 32 * half, row0);
+                            tma_store_2d(&P.ty, box, col, row0);
                         bulk_commit();
                     }
+                };
+                if (a.out_f32) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint4 w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float* f = v + 16 * h + 4 * j;
+                            w[j] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                                              __float_as_uint(f[3]));
+                        }
+                        send(w, n0 + c + 16 * h, static_cast<float*>(a.y));
+                    }
+                } else {
+                    uint4 w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        w[j] = make_uint4(pack_bf16x2(v[8 * j], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                                          pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+                    send(w, n0 + c, static_cast<__nv_bfloat16*>(a.y));
                 }
             }
             tc_fence_before();
@@ -736,11 +738,10 @@ template <int BN>
 cudaError_t launch_pair(I8Params& P, const char** err, cudaStream_t st)
 {
     const GemmI8Args& a = P.a;
-    const int size = a.out_f32 ? 4 : 2, cols = a.out_f32 ? 32 : PairCfg<BN>::kBf16Cols;
+    const int size = a.out_f32 ? 4 : 2;
     P.boxes = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.ldy * size) % 16 == 0;
     if (P.boxes && !encode_2d(&P.ty, a.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.N,
-                              a.M, a.ldy * size, cols, 32,
-                              cols * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B)) {
+                              a.M, a.ldy * size, 64 / size, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
         *err = "proj_i8: tensor map encoding failed";
         return cudaErrorInvalidValue;
     }
@@ -750,7 +751,7 @@ cudaError_t launch_pair(I8Params& P, const char** err, cudaStream_t st)
     if (e != cudaSuccess)
         return e;
     const int pairs = std::min(tiles, num_sms() / 2);
-    return launch_k(k_i8_pair<BN>, dim3(2 * pairs), 192, PairCfg<BN>::kSmem, st, P);
+    return launch_k(k_i8_pair<BN>, dim3(2 * pairs), kPairThreads, PairCfg<BN>::kSmem, st, P);
 }
 
 }  // namespace
