@@ -767,15 +767,15 @@ cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
         P.a = a;
         // k_i8_few's tokens a tile: the fewest that leave no more than a tile for each SM (W comes out of L2 again for each
         // tile, but K is cut less and an epilogue is short). Where that takes more than 32 of them, over 64 rows, the pair
-        // kernel is faster: 256 x 3072 x 3072 12.6 against 10.6 us; 128 rows 9.9 against 10.3, 77 x 1280 x 1280 4.7 against 6.8.
+        // kernel is faster: 256 x 3072 x 3072 12.6 against 10.3 us; 200 x 1280 x 1280 5.4 against 6.8, 77 rows 4.7 against 6.4.
         int few_bn = 16;
         while (few_bn < 64 && (a.M + few_bn - 1L) / few_bn * ((a.N + 127L) / 128) > num_sms())
             few_bn *= 2;
         const bool few = a.M <= 64 || few_bn <= 32;
         // Pair tiles of 256, 192, 160 or 128 columns: a round of tiles takes about as long as its columns and 128 more (its rows
         // of x, the way in and out), so the width whose rounds take least, the widest among equals. In us, 256, 192, 160, 128
-        // columns: 4097 x 1280 x 5120 31.5, 26.2, 25.3, 32.7; 700 x 8192 x 1024 14.7, 12.8, 15.6, 14.7; 512 x 9216 x 3072
-        // 15.3, 18.3, 17.6, 17.1; 1000 x 1536 x 1536 10.2, 8.7, 8.2, 7.8.
+        // columns: 4097 x 1280 x 5120 31.1, 26.6, 25.5, 32.8; 700 x 8192 x 1024 13.0, 11.7, 14.5, 13.9; 512 x 9216 x 3072
+        // 14.4, 17.8, 17.3, 16.7; 1000 x 1536 x 1536 9.6, 8.4, 8.2, 7.8.
         const long slots = num_sms() / 2;
         const auto cost = [&](int bn) {
             return (((a.M + 255L) / 256) * ((a.N + bn - 1L) / bn) + slots - 1) / slots * (bn + 128);

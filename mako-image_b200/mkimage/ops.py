@@ -213,7 +213,8 @@ OUT_NONE, OUT_BF16, OUT_F32, OUT_I8 = 0, 1, 2, 3
 
 
 # torch and the two calls every launch needs of it, looked up once: a call of these operators costs the host about as much as
-# its launch, so their checks are written for few steps (and outputs made by empty_strided: 1.8 us, empty takes 2.5).
+# its launch, so their checks are written for few steps (and outputs made by empty_strided: 1.8 us, empty takes 2.5). A call for
+# another device than the current one is made again with that device current; launches go to the device's current stream.
 torch = None
 _current_device = _raw_stream = None
 
@@ -237,21 +238,6 @@ def _same_device(name, dev, *tensors):
     for t in tensors:
         if t is not None and t.get_device() != dev:
             _fail(f"{name}: a tensor is on {t.device}, not on cuda:{dev}")
-
-
-def _launch(fn, dev, *args):
-    """fn(*args, stream) on the tensors' device and its current stream, whatever device is current."""
-    if _current_device() == dev:
-        code = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            code = fn(*args, _raw_stream(dev))
-    if code:
-        check(code)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
 
 
 def _row_stride(t, n):
@@ -278,6 +264,9 @@ def quantize_rows(x, q=None, scale=None):
         _fail("quantize_rows: the values of a row must be contiguous, one at least")
     dev = x.get_device()
     _same_device("quantize_rows", dev, q, scale)
+    if _current_device() != dev:
+        with t.cuda.device(dev):
+            return quantize_rows(x, q, scale)
     if q is None:
         ldq = (n + 15) & ~15
         q = t.empty_strided((rows, n), (ldq, 1), device=x.device, dtype=t.int8)
@@ -289,8 +278,10 @@ def quantize_rows(x, q=None, scale=None):
         scale = t.empty_strided((rows,), (1,), device=x.device, dtype=t.float32)
     else:
         _vector(scale, rows, t.float32, "quantize_rows: scale must be contiguous fp32 [rows]")
-    _launch(lib.mkb_quantize_rows, dev, x.data_ptr(), ldx if rows > 1 else n, f32, q.data_ptr(), ldq, scale.data_ptr(),
-            rows, n)
+    code = lib.mkb_quantize_rows(x.data_ptr(), ldx if rows > 1 else n, f32, q.data_ptr(), ldq, scale.data_ptr(), rows, n,
+                                 _raw_stream(dev))
+    if code:
+        check(code)
     return q, scale
 
 
@@ -316,6 +307,9 @@ def proj_i8(x, x_scale, w, w_scale, bias=None, act=ACT_NONE, out=None, out_f32=F
         _vector(bias, N, f32, "proj_i8: bias must be contiguous fp32 [N]")
     dev = x.get_device()
     _same_device("proj_i8", dev, x_scale, w, w_scale, bias, out)
+    if _current_device() != dev:
+        with t.cuda.device(dev):
+            return proj_i8(x, x_scale, w, w_scale, bias, act, out, out_f32)
     if out is None:
         out = t.empty_strided((M, N), (N, 1), device=x.device, dtype=f32 if out_f32 else t.bfloat16)
         ldy = N
@@ -324,8 +318,11 @@ def proj_i8(x, x_scale, w, w_scale, bias=None, act=ACT_NONE, out=None, out_f32=F
         if out.shape != (M, N) or not (out_f32 or out.dtype is t.bfloat16) or (N > 1 and out.stride(1) != 1):
             _fail("proj_i8: out must be [M][N] fp32 or bf16 with contiguous rows")
         ldy = _row_stride(out, N)
-    _launch(lib.mkb_proj_i8, dev, x.data_ptr(), ldx if M > 1 else (K + 15) & ~15, x_scale.data_ptr(), w.data_ptr(),
-            ldw if N > 1 else (K + 15) & ~15, w_scale.data_ptr(), _ptr(bias), out.data_ptr(), ldy, M, N, K, act, out_f32)
+    code = lib.mkb_proj_i8(x.data_ptr(), ldx if M > 1 else (K + 15) & ~15, x_scale.data_ptr(), w.data_ptr(),
+                           ldw if N > 1 else (K + 15) & ~15, w_scale.data_ptr(), None if bias is None else bias.data_ptr(),
+                           out.data_ptr(), ldy, M, N, K, act, out_f32, _raw_stream(dev))
+    if code:
+        check(code)
     return out
 
 
@@ -364,6 +361,10 @@ def gate_add_norm(x, y=None, y_norm=NORM_NONE, y_weight=None, gate=None, tanh_ga
 
     dev = x.get_device()
     _same_device("gate_add_norm", dev, y, y_weight, gate, x_weight, scale, shift, x_out, out, out_scale)
+    if _current_device() != dev:
+        with t.cuda.device(dev):
+            return gate_add_norm(x, y, y_norm, y_weight, gate, tanh_gate, x_norm, x_weight, scale, shift, rows_per_sample, eps,
+                                 x_out, out, out_scale, out_type)
     ldx = rows_of(x, f32)
     if x_out is None:
         x_out, ldxo = x, ldx
@@ -403,9 +404,14 @@ def gate_add_norm(x, y=None, y_norm=NORM_NONE, y_weight=None, gate=None, tanh_ga
             mod_stride = shift_stride
         elif shift_stride != mod_stride and samples > 1:
             _fail("gate_add_norm: scale and shift must have the same strides")
-    _launch(lib.mkb_gate_add_norm, dev, x.data_ptr(), ldx, x_out.data_ptr(), ldxo, _ptr(y), ldy, y_f32, y_norm,
-            _ptr(y_weight), _ptr(gate), gate_stride, tanh_gate, x_norm, _ptr(x_weight), _ptr(scale), _ptr(shift),
-            mod_stride, rps, eps, _ptr(out), ldo, out_type, _ptr(out_scale), rows, n)
+    code = lib.mkb_gate_add_norm(
+        x.data_ptr(), ldx, x_out.data_ptr(), ldxo, None if y is None else y.data_ptr(), ldy, y_f32, y_norm,
+        None if y_weight is None else y_weight.data_ptr(), None if gate is None else gate.data_ptr(), gate_stride, tanh_gate,
+        x_norm, None if x_weight is None else x_weight.data_ptr(), None if scale is None else scale.data_ptr(),
+        None if shift is None else shift.data_ptr(), mod_stride, rps, eps, None if out is None else out.data_ptr(), ldo,
+        out_type, None if out_scale is None else out_scale.data_ptr(), rows, n, _raw_stream(dev))
+    if code:
+        check(code)
     return (out, out_scale) if out_type == OUT_I8 else out
 
 
@@ -424,6 +430,9 @@ def cross_attention(q, k, v, key_len=None, key_mask=None, scale=None, out=None):
         _fail("cross_attention: q must be [B][H][Lq][d], k and v [B][Hkv][Lk][d]")
     dev = q.get_device()
     _same_device("cross_attention", dev, k, v, out, key_len, key_mask)
+    if _current_device() != dev:
+        with t.cuda.device(dev):
+            return cross_attention(q, k, v, key_len, key_mask, scale, out)
     o_last = 1
     if out is None:
         o_row, o_head, o_sample = H * d, d, Lq * H * d
@@ -450,7 +459,10 @@ def cross_attention(q, k, v, key_len=None, key_mask=None, scale=None, out=None):
         mask_stride = key_mask.stride(0)
     if scale is not None and not scale > 0:
         _fail("cross_attention: the scale must be positive")
-    _launch(lib.mkb_cross_attention, dev, q.data_ptr(), q_row, q_head, q_sample, k.data_ptr(), k_row, k_head, k_sample,
-            v.data_ptr(), v_row, v_head, v_sample, out.data_ptr(), o_row, o_head, o_sample, B, H, Hkv, Lq, Lk, d,
-            _ptr(key_len), _ptr(key_mask), mask_stride, scale or 0.0)
+    code = lib.mkb_cross_attention(
+        q.data_ptr(), q_row, q_head, q_sample, k.data_ptr(), k_row, k_head, k_sample, v.data_ptr(), v_row, v_head, v_sample,
+        out.data_ptr(), o_row, o_head, o_sample, B, H, Hkv, Lq, Lk, d, None if key_len is None else key_len.data_ptr(),
+        None if key_mask is None else key_mask.data_ptr(), mask_stride, scale or 0.0, _raw_stream(dev))
+    if code:
+        check(code)
     return out

@@ -193,3 +193,32 @@ def test_another_device_than_the_current_one(cuda):
         assert torch.equal(_run(p, b), h) and torch.equal(a, b)
     with pytest.raises(mkimage.MkbError):
         mkimage.ops.quantize_rows(x, scale=torch.empty(300, device="cuda:0"))
+
+
+def test_a_call_for_another_device_is_made_again_there(cuda, monkeypatch):
+    """With the current device reported as another one at first, each operator runs once more under the tensors' device and
+    gives what it gives otherwise."""
+    import torch
+    import mkimage
+
+    ops = mkimage.ops
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(20, 64, generator=g).to(cuda)
+    y = torch.randn(20, 64, generator=g).to(cuda).to(torch.bfloat16)
+    q = torch.randn(2, 3, 20, 64, generator=g).to(cuda).to(torch.bfloat16)
+    lens = torch.tensor([20, 7], dtype=torch.int32, device=cuda)
+
+    def all_of_them():
+        i8, step = ops.quantize_rows(x)
+        x_out = torch.empty_like(x)
+        n8, n_step = ops.gate_add_norm(x, y, y_norm=ops.NORM_RMS, gate=x[:1], x_norm=ops.NORM_LAYER, scale=x[:1], shift=x[:1],
+                                       x_out=x_out, out_type=ops.OUT_I8)
+        return [i8, step, x_out, n8, n_step, ops.proj_i8(i8, step, n8, n_step, bias=step, out_f32=True),
+                ops.cross_attention(q, q, q, key_len=lens, scale=0.2)]
+
+    want = all_of_them()
+    real, calls = ops._current_device, []
+    monkeypatch.setattr(ops, "_current_device", lambda: calls.append(1) or (real() if len(calls) % 2 == 0 else real() + 1))
+    got = all_of_them()
+    assert len(calls) == 8
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
