@@ -1152,10 +1152,11 @@ cudaError_t launch(const CrossParams& P, cudaStream_t st)
 template <int D, int R>
 cudaError_t launch_few(const CrossArgs& a, cudaStream_t st)
 {
-    // The keys over as many CTAs as leave four for each SM, 128 keys each or more (the size that divides the CTAs most evenly
-    // over the SMs instead, 6 for 8 at 48 key heads, was slower: 23.6 against 22.4 us).
+    // The keys over as many CTAs as the SMs hold at once, three each, 128 keys a CTA or more (four an SM leave a second wave:
+    // 128 key heads of 4096 keys 61 against 51 us; the size that divides the CTAs most evenly over the SMs instead, 6 for 8 at
+    // 48 key heads, was slower: 23.6 against 22.4 us).
     const int pairs = a.B * a.Hkv;
-    const int splits = std::max(1, std::min({kMaxSplits, kFewWarps, 4 * num_sms() / pairs, a.Lk / 128}));
+    const int splits = std::max(1, std::min({kMaxSplits, kFewWarps, 3 * num_sms() / pairs, a.Lk / 128}));
     static std::atomic<uint64_t> devs{0};
     const cudaError_t e = smem_limit_once(devs, k_cross_few<D, R>, kFewSmem);
     if (e != cudaSuccess)
