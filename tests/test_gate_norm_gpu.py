@@ -224,6 +224,26 @@ def test_quantize_rows_is_exact(cuda, rows, n, f32):
     assert q.stride(0) % 16 == 0
 
 
+@pytest.mark.parametrize("rows,n", [(9000, 640), (5000, 333), (3001, 8192), (2500, 5120), (1500, 5001)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_quantize_many_rows(cuda, rows, n, f32):
+    """More rows than blocks that run at once, strided, a NaN among them; what lies between the rows stays."""
+    import torch
+    import mkimage
+
+    g = torch.Generator().manual_seed(rows + n)
+    x = torch.randn(rows, n + 8, generator=g)
+    x = (x * torch.rand(rows, 1, generator=g)).to(cuda).to(torch.float32 if f32 else torch.bfloat16)[:, :n]
+    x[rows // 2, 3] = float("nan")
+    buf = torch.full((rows, (n + 31) // 16 * 16), 99, dtype=torch.int8, device=cuda)
+    step = torch.empty(rows, device=cuda)
+    mkimage.ops.quantize_rows(x, buf[:, :n], step)
+    fine = torch.arange(rows, device=cuda) != rows // 2
+    rq, rstep = _quant64(x[fine])
+    assert torch.equal(step[fine], rstep) and torch.equal(buf[:, :n][fine], rq) and bool((buf[:, n:] == 99).all())
+    assert bool(torch.isnan(step[rows // 2])) and int(buf[rows // 2, :n].abs().max()) == 0
+
+
 def test_quantize_rows_borders(cuda):
     """Quotients on and next to a border of two whole numbers, rows of zeros, tiny rows, infinities and NaN."""
     import torch
