@@ -67,6 +67,19 @@ __device__ __forceinline__ void load_vec(const float* p, float (&v)[VEC])
     }
 }
 
+// Columns c .. c + VEC - 1 of n, 0 outside them.
+template <int VEC, bool ODD>
+__device__ __forceinline__ void load_cols(const float* p, int c, int n, float (&v)[VEC])
+{
+    if constexpr (ODD) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+            v[k] = unsigned(c + k) < unsigned(n) ? __ldg(p + c + k) : 0.0f;
+    } else {
+        load_vec(p + c, v);
+    }
+}
+
 template <int VEC>
 __device__ __forceinline__ void load_shared(const float* p, float (&v)[VEC])
 {
@@ -124,6 +137,12 @@ struct Raw {
         for (int k = 0; k < VEC; ++k)
             u[k] = 0;
     }
+    // Value k alone, into words that were zero.
+    __device__ __forceinline__ void load_one(const float* p, int k) { u[k] = __ldcs(reinterpret_cast<const uint32_t*>(p) + k); }
+    __device__ __forceinline__ void load_one(const __nv_bfloat16* p, int k)
+    {
+        u[k >> 1] |= uint32_t(__ldcs(reinterpret_cast<const unsigned short*>(p) + k)) << (16 * (k & 1));
+    }
     __device__ __forceinline__ void values(bool f32, float (&v)[VEC]) const
     {
         if constexpr (VEC == 8) {
@@ -174,16 +193,25 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* p, const float (&v)[VEC
 }
 
 // A row's chunks of 32 * VEC values: NC to a warp, one after another, so that a thread's places in the row are constants apart.
-template <int VEC, int NC>
+// ODD: the row starts `skip` values after a vector's border, so the first and the last vector may be cut; `first` then counts
+// from the row's start and may be negative.
+template <int VEC, int NC, bool ODD = false>
 struct Place {
     int first;  // the thread's first value
-    __device__ __forceinline__ Place() : first(int(threadIdx.x >> 5) * NC * 32 * VEC + int(threadIdx.x & 31) * VEC) {}
-    __device__ __forceinline__ bool in(int i, int n) const { return first + i * 32 * VEC < n; }
+    __device__ __forceinline__ explicit Place(int skip = 0)
+        : first(int(threadIdx.x >> 5) * NC * 32 * VEC + int(threadIdx.x & 31) * VEC - skip)
+    {
+    }
+    __device__ __forceinline__ int at(int i) const { return first + i * 32 * VEC; }
+    // Any of vector i in the row; all of it; value k of it.
+    __device__ __forceinline__ bool in(int i, int n) const { return at(i) < n; }
+    __device__ __forceinline__ bool all(int i, int n) const { return !ODD || (at(i) >= 0 && at(i) + VEC <= n); }
+    __device__ __forceinline__ bool has(int i, int k, int n) const { return !ODD || unsigned(at(i) + k) < unsigned(n); }
 };
 
 // Standardises the row held in v (values past the row are 0 on entry and stay so).
-template <int VEC, int NC>
-__device__ __forceinline__ void normalise(float (&v)[NC][VEC], const Place<VEC, NC>& at, int kind, int n, float inv_n,
+template <int VEC, int NC, bool ODD>
+__device__ __forceinline__ void normalise(float (&v)[NC][VEC], const Place<VEC, NC, ODD>& at, int kind, int n, float inv_n,
                                           float eps, float* red)
 {
     if (kind == kNormLayer) {  // mean first, then the squares about it: no cancellation where the mean is large
@@ -199,7 +227,8 @@ __device__ __forceinline__ void normalise(float (&v)[NC][VEC], const Place<VEC, 
             if (at.in(i, n))
 #pragma unroll
                 for (int k = 0; k < VEC; ++k)
-                    v[i][k] -= mean;
+                    if (at.has(i, k, n))
+                        v[i][k] -= mean;
     }
     float s = 0.0f;
 #pragma unroll
@@ -215,16 +244,23 @@ __device__ __forceinline__ void normalise(float (&v)[NC][VEC], const Place<VEC, 
             v[i][k] *= r;
 }
 
-template <int VEC, int NC, typename T>
-__device__ __forceinline__ void load_row_at(Raw<VEC> (&v)[NC], const T* p, const Place<VEC, NC>& at, int n)
+template <int VEC, int NC, bool ODD, typename T>
+__device__ __forceinline__ void load_row_at(Raw<VEC> (&v)[NC], const T* p, const Place<VEC, NC, ODD>& at, int n)
 {
     p += at.first;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        if (at.in(i, n))
+        if (at.in(i, n) && at.all(i, n)) {
             v[i].load(p + i * 32 * VEC);
-        else
+        } else {
             v[i].zero();
+            if constexpr (ODD) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k)
+                    if (at.has(i, k, n))
+                        v[i].load_one(p + i * 32 * VEC, k);
+            }
+        }
     }
 }
 
@@ -236,20 +272,32 @@ __device__ __forceinline__ void values(const Raw<VEC> (&r)[NC], bool f32, float 
         r[i].values(f32, v[i]);
 }
 
-template <int VEC, int NC, typename T>
-__device__ __forceinline__ void store_row_at(const float (&v)[NC][VEC], T* p, const Place<VEC, NC>& at, int n)
+__device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_one(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
+
+// `whole`: the row lies on the vectors' borders as the loaded rows do (always, unless ODD).
+template <int VEC, int NC, bool ODD, typename T>
+__device__ __forceinline__ void store_row_at(const float (&v)[NC][VEC], T* p, const Place<VEC, NC, ODD>& at, int n,
+                                             bool whole = true)
 {
     p += at.first;
 #pragma unroll
-    for (int i = 0; i < NC; ++i)
-        if (at.in(i, n))
+    for (int i = 0; i < NC; ++i) {
+        if (at.in(i, n) && at.all(i, n) && (!ODD || whole)) {
             store_row(p + i * 32 * VEC, v[i]);
+        } else if constexpr (ODD) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k)
+                if (at.has(i, k, n))
+                    store_one(p + i * 32 * VEC + k, v[i][k]);
+        }
+    }
 }
 
 // The row as 8-bit integers with their step.
-template <int VEC, int NC>
-__device__ __forceinline__ void quant_row_at(const float (&v)[NC][VEC], int8_t* q, float* scale, const Place<VEC, NC>& at,
-                                             int n, float* red)
+template <int VEC, int NC, bool ODD>
+__device__ __forceinline__ void quant_row_at(const float (&v)[NC][VEC], int8_t* q, float* scale,
+                                             const Place<VEC, NC, ODD>& at, int n, float* red, bool whole = true)
 {
     float top = 0.0f;
 #pragma unroll
@@ -274,10 +322,16 @@ __device__ __forceinline__ void quant_row_at(const float (&v)[NC][VEC], int8_t* 
                     const float u[4] = {v[i][4 * k], v[i][4 * k + 1], v[i][4 * k + 2], v[i][4 * k + 3]};
                     p[k] = step.pack4(u);
                 }
-                if constexpr (VEC == 8)
+                if (ODD && !(whole && at.all(i, n))) {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k)
+                        if (at.has(i, k, n))
+                            o[k] = int8_t(p[k / 4] >> (8 * (k & 3)));
+                } else if constexpr (VEC == 8) {
                     *reinterpret_cast<uint2*>(o) = make_uint2(p[0], p[1]);
-                else
+                } else {
                     *reinterpret_cast<uint32_t*>(o) = p[0];
+                }
             }
         }
 }
@@ -298,7 +352,7 @@ __device__ __forceinline__ float tanh_near(float x)
 
 // The vectors over a row's places, as far as one chunk of one thread goes: y's factor g(gate) * y_weight, and x's
 // h * factor + shift with factor = x_weight * (1 + scale).
-template <int VEC>
+template <int VEC, bool ODD>
 struct Vectors {
     float gate[VEC], factor[VEC], shift[VEC];
     __device__ __forceinline__ void branch(const GateNormArgs& a, long sample, int c)
@@ -307,7 +361,7 @@ struct Vectors {
         for (int k = 0; k < VEC; ++k)
             gate[k] = 1.0f;
         if (a.gate) {
-            load_vec(a.gate + sample * a.gate_stride + c, gate);
+            load_cols<VEC, ODD>(a.gate + sample * a.gate_stride, c, a.n, gate);
             if (a.tanh_gate)
 #pragma unroll
                 for (int k = 0; k < VEC; ++k)
@@ -315,7 +369,7 @@ struct Vectors {
         }
         if (a.y_weight) {
             float w[VEC];
-            load_vec(a.y_weight + c, w);
+            load_cols<VEC, ODD>(a.y_weight, c, a.n, w);
 #pragma unroll
             for (int k = 0; k < VEC; ++k)
                 gate[k] *= w[k];
@@ -329,49 +383,57 @@ struct Vectors {
             shift[k] = 0.0f;
         }
         if (a.x_weight)
-            load_vec(a.x_weight + c, factor);
+            load_cols<VEC, ODD>(a.x_weight, c, a.n, factor);
         if (a.scale) {
             float s[VEC];
-            load_vec(a.scale + sample * a.mod_stride + c, s);
+            load_cols<VEC, ODD>(a.scale + sample * a.mod_stride, c, a.n, s);
 #pragma unroll
             for (int k = 0; k < VEC; ++k)
                 factor[k] = fmaf(factor[k], s[k], factor[k]);
         }
         if (a.shift)
-            load_vec(a.shift + sample * a.mod_stride + c, shift);
+            load_cols<VEC, ODD>(a.shift + sample * a.mod_stride, c, a.n, shift);
     }
 };
 
-// A block a run of `run` rows of one sample, NC chunks of 32 * VEC values a warp and row. n is a multiple of VEC. KEEP: the
-// vectors stay in shared memory from row to row and each row is loaded while the one before is worked on (otherwise a run is one
-// row).
+// A launch's arguments: a sample's blocks; out_whole: out's rows lie on the vectors' borders as x's do.
+struct GateNormOf : GateNormArgs {
+    unsigned blocks;
+    bool out_whole;
+};
+
+// A block a run of `run` rows of one sample, NC chunks of 32 * VEC values a warp and row. The vectors stay in shared memory from
+// row to row and each row is loaded while the one before is worked on.
+// ODD: rows that do not all begin on a vector's border, but x, y and x_out alike. Rows four apart begin alike, so a run takes
+// every fourth row and all of it has one place in the vectors; the cut vectors at a row's ends go value by value.
 // T: threads at most; up to 256 leave 85 registers each for three blocks an SM, the widest rows take an SM's for one block.
-template <int VEC, int NC, bool KEEP, int T>
-__global__ void __launch_bounds__(T, KEEP && NC * VEC <= 12 ? (T == 256 ? 3 : 2) : 1) k_gate_norm(const GateNormArgs a, int run)
+template <int VEC, int NC, bool ODD, int T>
+__global__ void __launch_bounds__(T, NC * VEC <= 12 ? (T == 256 ? 3 : 2) : 1) k_gate_norm(const GateNormOf a, int run)
 {
     __shared__ float red[2][5][16];
     grid_dep_wait();
     grid_dep_launch();
-    const unsigned blocks = (unsigned(a.rows_per_sample) + run - 1) / run;  // of a sample
-    const long sample = blockIdx.x / blocks;
-    const long lo = sample * a.rows_per_sample + long(blockIdx.x % blocks) * run;
-    const long hi = min(min(a.rows, (sample + 1) * a.rows_per_sample), lo + run);
+    constexpr int kApart = ODD ? 4 : 1;
+    const unsigned part = blockIdx.x % a.blocks;
+    const long sample = blockIdx.x / a.blocks;
+    const long lo = sample * a.rows_per_sample + long(part / kApart) * run * kApart + part % kApart;
+    const long hi = min(min(a.rows, (sample + 1) * a.rows_per_sample), lo + long(run) * kApart);
     const int n = a.n;
     const float inv_n = 1.0f / float(n);
-    const Place<VEC, NC> at;
-    extern __shared__ __align__(16) float kept[];  // KEEP: [gate, factor, shift][n], each thread its own places
-    float* mine = kept + at.first;
-    if constexpr (KEEP)
+    const Place<VEC, NC, ODD> at(ODD ? int((reinterpret_cast<uintptr_t>(a.x) / 4 + lo * a.ldx) & 3) : 0);
+    extern __shared__ __align__(16) float kept[];  // [gate, factor, shift][ns], each thread its own places
+    const int ns = ODD ? (n + 6) & ~3 : n;
+    float* mine = kept + Place<VEC, NC>().first;
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
-            if (at.in(i, n)) {
-                Vectors<VEC> v;
-                v.branch(a, sample, at.first + i * 32 * VEC);
-                v.stream(a, sample, at.first + i * 32 * VEC);
-                store_row(mine + i * 32 * VEC, v.gate);
-                store_row(mine + n + i * 32 * VEC, v.factor);
-                store_row(mine + 2 * n + i * 32 * VEC, v.shift);
-            }
+    for (int i = 0; i < NC; ++i)
+        if (at.in(i, n)) {
+            Vectors<VEC, ODD> v;
+            v.branch(a, sample, at.at(i));
+            v.stream(a, sample, at.at(i));
+            store_row(mine + i * 32 * VEC, v.gate);
+            store_row(mine + ns + i * 32 * VEC, v.factor);
+            store_row(mine + 2 * ns + i * 32 * VEC, v.shift);
+        }
     Raw<VEC> rx[NC], ry[NC];
     const auto load = [&](long row) {
         load_row_at(rx, a.x + row * a.ldx, at, n);
@@ -383,24 +445,21 @@ __global__ void __launch_bounds__(T, KEEP && NC * VEC <= 12 ? (T == 256 ? 3 : 2)
     if (lo < hi)
         load(lo);
     int turn = 0;
-    for (long row = lo; row < hi; ++row, turn ^= 1) {
+    for (long row = lo; row < hi; row += kApart, turn ^= 1) {
         float x[NC][VEC], y[NC][VEC];
         values(rx, true, x);
         if (a.y)
             values(ry, a.y_f32, y);
-        if (KEEP && row + 1 < hi)
-            load(row + 1);
+        if (row + kApart < hi)
+            load(row + kApart);
         if (a.y) {
             if (a.y_norm != kNormNone)
                 normalise(y, at, a.y_norm, n, inv_n, a.eps, red[turn][0]);
 #pragma unroll
             for (int i = 0; i < NC; ++i)
                 if (at.in(i, n)) {
-                    Vectors<VEC> v;
-                    if constexpr (KEEP)
-                        load_shared(mine + i * 32 * VEC, v.gate);
-                    else
-                        v.branch(a, sample, at.first + i * 32 * VEC);
+                    Vectors<VEC, ODD> v;
+                    load_shared(mine + i * 32 * VEC, v.gate);
 #pragma unroll
                     for (int k = 0; k < VEC; ++k)
                         x[i][k] = fmaf(y[i][k], v.gate[k], x[i][k]);
@@ -414,23 +473,19 @@ __global__ void __launch_bounds__(T, KEEP && NC * VEC <= 12 ? (T == 256 ? 3 : 2)
 #pragma unroll
         for (int i = 0; i < NC; ++i)
             if (at.in(i, n)) {
-                Vectors<VEC> v;
-                if constexpr (KEEP) {
-                    load_shared(mine + n + i * 32 * VEC, v.factor);
-                    load_shared(mine + 2 * n + i * 32 * VEC, v.shift);
-                } else {
-                    v.stream(a, sample, at.first + i * 32 * VEC);
-                }
+                Vectors<VEC, ODD> v;
+                load_shared(mine + ns + i * 32 * VEC, v.factor);
+                load_shared(mine + 2 * ns + i * 32 * VEC, v.shift);
 #pragma unroll
                 for (int k = 0; k < VEC; ++k)
                     x[i][k] = fmaf(x[i][k], v.factor[k], v.shift[k]);
             }
         if (a.out_type == kOutBf16)
-            store_row_at(x, static_cast<__nv_bfloat16*>(a.out) + row * a.ldo, at, n);
+            store_row_at(x, static_cast<__nv_bfloat16*>(a.out) + row * a.ldo, at, n, a.out_whole);
         else if (a.out_type == kOutF32)
-            store_row_at(x, static_cast<float*>(a.out) + row * a.ldo, at, n);
+            store_row_at(x, static_cast<float*>(a.out) + row * a.ldo, at, n, a.out_whole);
         else
-            quant_row_at(x, static_cast<int8_t*>(a.out) + row * a.ldo, a.out_scale + row, at, n, red[turn][4]);
+            quant_row_at(x, static_cast<int8_t*>(a.out) + row * a.ldo, a.out_scale + row, at, n, red[turn][4], a.out_whole);
     }
 }
 
@@ -487,10 +542,10 @@ bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(
 struct Deal {
     int nc, warps;
 };
-Deal deal(int chunks, int most, bool few_warps)
+Deal deal(int chunks, int most, bool few_warps, int least = 1)
 {
     Deal best{0, 0};
-    for (int nc = 1; nc <= most; ++nc) {
+    for (int nc = least; nc <= most; ++nc) {
         const int warps = (chunks + nc - 1) / nc;
         const int more = best.nc ? warps * nc - best.warps * best.nc : -1;
         if (warps <= 16 && (more < 0 || (more == 0 && few_warps)))
@@ -499,39 +554,57 @@ Deal deal(int chunks, int most, bool few_warps)
     return best;
 }
 
-template <int VEC, int NC, bool KEEP, int T>
-cudaError_t launch_gate_norm_of(const GateNormArgs& a, int warps, cudaStream_t st)
+template <int VEC, int NC, bool ODD, int T>
+cudaError_t launch_gate_norm_of(GateNormOf& a, int warps, cudaStream_t st)
 {
+    constexpr int kApart = ODD ? 4 : 1;
     const long samples = (a.rows + a.rows_per_sample - 1) / a.rows_per_sample;
-    const size_t smem = KEEP ? size_t(3) * a.n * sizeof(float) : 0;
+    const size_t smem = size_t(3) * (ODD ? (a.n + 6) & ~3 : a.n) * sizeof(float);
     if (smem > 48 * 1024) {
         static std::atomic<uint64_t> devs{0};
-        const cudaError_t e = smem_limit_once(devs, k_gate_norm<VEC, NC, KEEP, T>, 3 * kGateNormMaxWidth * int(sizeof(float)));
+        const cudaError_t e =
+            smem_limit_once(devs, k_gate_norm<VEC, NC, ODD, T>, 3 * kGateNormMaxWidth * int(sizeof(float)));
         if (e != cudaSuccess)
             return e;
     }
     // Runs as long as still leave one wave of resident blocks (two waves: 65 against 63 us at 8704 x 3072, three 69).
+    const long apart = (a.rows_per_sample + kApart - 1) / kApart;
     int run = 1;
-    if (KEEP && a.rows > 2L * num_sms()) {
+    if (a.rows > 2L * num_sms()) {
         int resident = 1;
         const cudaError_t e =
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, k_gate_norm<VEC, NC, KEEP, T>, 32 * warps, smem);
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, k_gate_norm<VEC, NC, ODD, T>, 32 * warps, smem);
         if (e != cudaSuccess)
             return e;
         const long wave = long(num_sms()) * std::max(1, resident);
-        run = int(std::min(a.rows_per_sample, std::max(1L, (a.rows + wave - 1) / wave)));
+        run = int(std::min(apart, std::max(1L, (a.rows + wave - 1) / wave)));
     }
-    return launch_k(k_gate_norm<VEC, NC, KEEP, T>, dim3(unsigned(samples * ((a.rows_per_sample + run - 1) / run))), 32 * warps,
-                    smem, st, a, run);
+    a.blocks = unsigned((apart + run - 1) / run * kApart);
+    return launch_k(k_gate_norm<VEC, NC, ODD, T>, dim3(unsigned(samples * a.blocks)), 32 * warps, smem, st, a, run);
 }
 
-template <int VEC, int NC, bool KEEP>
-cudaError_t launch_gate_norm(const GateNormArgs& a, int warps, cudaStream_t st)
+template <int VEC, int NC, bool ODD = false>
+cudaError_t launch_gate_norm(GateNormOf& a, int warps, cudaStream_t st)
 {
-    if constexpr (KEEP && NC * VEC <= 12)
+    if constexpr (NC * VEC <= 12)
         if (warps <= 8)
-            return launch_gate_norm_of<VEC, NC, KEEP, 256>(a, warps, st);
-    return launch_gate_norm_of<VEC, NC, KEEP, 512>(a, warps, st);
+            return launch_gate_norm_of<VEC, NC, ODD, 256>(a, warps, st);
+    return launch_gate_norm_of<VEC, NC, ODD, 512>(a, warps, st);
+}
+
+template <bool ODD>
+cudaError_t launch_gate_norm_by_four(GateNormOf& a, int chunks, cudaStream_t st)
+{
+    const bool many = a.rows > 2L * num_sms();
+    // Rows with cut vectors: two chunks a warp at least where there are many (the warps with an end hold the others up at each
+    // reduction: 4099 x 1283 20.8 us on 6 warps, 24.3 on 11).
+    const Deal d = deal(chunks, chunks <= 48 ? 3 : 6, many, ODD && many ? 2 : 1);
+    return d.nc == 1   ? launch_gate_norm<4, 1, ODD>(a, d.warps, st)
+           : d.nc == 2 ? launch_gate_norm<4, 2, ODD>(a, d.warps, st)
+           : d.nc == 3 ? launch_gate_norm<4, 3, ODD>(a, d.warps, st)
+           : d.nc == 4 ? launch_gate_norm<4, 4, ODD>(a, d.warps, st)
+           : d.nc == 5 ? launch_gate_norm<4, 5, ODD>(a, d.warps, st)
+                       : launch_gate_norm<4, 6, ODD>(a, d.warps, st);
 }
 
 template <typename XT, int VEC, int NC>
@@ -568,38 +641,29 @@ cudaError_t gate_norm(const GateNormArgs& args, cudaStream_t st)
 {
     if (args.rows == 0)
         return cudaSuccess;
-    GateNormArgs a = args;
+    GateNormOf a{args, 0, true};
     a.rows_per_sample = std::min(a.rows_per_sample, a.rows);
-    // 16-byte accesses where every row and vector allows them, single values otherwise.
+    // Vectors of four where every row and vector allows them; rows that begin off a border, but alike, cut their end vectors
+    // (1916 x 2719 to int8 21 us, value by value 31; 4803 x 5111 90 against 100); rows that begin differently go by value.
     const size_t yb = a.y_f32 ? 16 : 8, ob = a.out_type == kOutBf16 ? 8 : a.out_type == kOutF32 ? 16 : 4;
     const bool vec = a.n % 4 == 0 && aligned(a.x, 16) && a.ldx % 4 == 0 &&
                      (!a.y || (aligned(a.y, yb) && a.ldy % 4 == 0 && aligned(a.x_out, 16) && a.ldxo % 4 == 0)) &&
                      aligned(a.y_weight, 16) && aligned(a.gate, 16) && a.gate_stride % 4 == 0 &&
                      aligned(a.x_weight, 16) && aligned(a.scale, 16) && aligned(a.shift, 16) &&
                      a.mod_stride % 4 == 0 && (a.out_type == kOutNone || (aligned(a.out, ob) && a.ldo % 4 == 0));
+    const auto as_x = [&](const void* p, size_t bytes, long ld) {
+        return ((reinterpret_cast<uintptr_t>(p) / bytes ^ reinterpret_cast<uintptr_t>(a.x) / 4) & 3) == 0 && (ld - a.ldx) % 4 == 0;
+    };
+    a.out_whole = a.out_type == kOutNone || as_x(a.out, ob / 4, a.ldo);
     cudaError_t e;
-    if (vec) {
-        const int chunks = (a.n + 127) / 128;
-        const Deal d = deal(chunks, chunks <= 48 ? 3 : 6, a.rows > 2L * num_sms());
-        e = d.nc == 1   ? launch_gate_norm<4, 1, true>(a, d.warps, st)
-            : d.nc == 2 ? launch_gate_norm<4, 2, true>(a, d.warps, st)
-            : d.nc == 3 ? launch_gate_norm<4, 3, true>(a, d.warps, st)
-            : d.nc == 4 ? launch_gate_norm<4, 4, true>(a, d.warps, st)
-            : d.nc == 5 ? launch_gate_norm<4, 5, true>(a, d.warps, st)
-                        : launch_gate_norm<4, 6, true>(a, d.warps, st);
-    } else {
-        // 4, 6 or 8 chunks a warp, whichever leaves the fewest places idle (4099 x 1283: 22 us on 7 warps of 6, 25 on 11 of 4).
-        const int chunks = (a.n + 31) / 32;
-        const auto places = [&](int nc) { return (chunks + nc - 1) / nc * nc; };
-        if (chunks > 128)
-            e = launch_gate_norm<1, 24, false>(a, (chunks + 23) / 24, st);
-        else if (chunks <= 64 && places(4) <= places(6) && places(4) <= places(8))
-            e = launch_gate_norm<1, 4, true>(a, (chunks + 3) / 4, st);
-        else if (chunks <= 96 && places(6) <= places(8))
-            e = launch_gate_norm<1, 6, true>(a, (chunks + 5) / 6, st);
-        else
-            e = launch_gate_norm<1, 8, true>(a, (chunks + 7) / 8, st);
-    }
+    if (vec)
+        e = launch_gate_norm_by_four<false>(a, (a.n + 127) / 128, st);
+    else if (a.n + 3 <= kGateNormMaxWidth && (!a.y || (as_x(a.y, yb / 4, a.ldy) && as_x(a.x_out, 4, a.ldxo))))
+        e = launch_gate_norm_by_four<true>(a, (a.n + 3 + 127) / 128, st);
+    else if (a.n <= 4096)
+        e = launch_gate_norm<1, 8>(a, (a.n + 255) / 256, st);
+    else
+        e = launch_gate_norm<1, 24>(a, (a.n + 767) / 768, st);
     if (e != cudaSuccess)
         return e;
     count_launch();

@@ -132,6 +132,44 @@ def test_runs_of_rows(cuda, rows, n, samples, out):
         _check(ops, c, per, y_norm, x_norm, tanh=y_norm == 1, mod=True, out_type=kind, in_place=y_norm == 1)
 
 
+@pytest.mark.parametrize("off_x,off_y,off_o", [(1, 1, 1), (1, 1, 2), (3, 3, 0), (2, 1, 1), (0, 2, 0)])
+@pytest.mark.parametrize("rows,n,ld", [(5, 129, 131), (700, 1283, 1283 + 8), (900, 640, 641), (420, 5111, 5119), (40, 12288, 12289)])
+@pytest.mark.parametrize("out", ["bf16", "f32", "i8"])
+def test_rows_at_any_place(cuda, off_x, off_y, off_o, rows, n, ld, out):
+    """x, y and out at their own places in wider rows, alike and not, against the same call on rows of their own; nothing
+    outside the rows is written. The sums' order may differ: 2 TERM of the standardised values, whose size is below 12 here,
+    through factors below 3, and a rounding of the output; a whole number may differ by one."""
+    import torch
+    import mkimage
+
+    ops = mkimage.ops
+    kind, dtype = dict(bf16=(ops.OUT_BF16, torch.bfloat16), f32=(ops.OUT_F32, torch.float32), i8=(ops.OUT_I8, torch.int8))[out]
+    per = -(-rows // 2)
+    c = _case(cuda, rows, n, n + off_x, False, 2)
+
+    def at(t, off):
+        buf = torch.full((rows * ld + 16,), 3, device=cuda, dtype=t)
+        return buf, buf[off:off + rows * ld].view(rows, ld)[:, :n]
+
+    (xb, x), (yb, y), (ob, o) = at(torch.float32, off_x), at(torch.bfloat16, off_y), at(dtype, off_o)
+    x.copy_(c["x"])
+    y.copy_(c["y"])
+    rx, step = c["x"].clone(), torch.empty(rows, device=cuda) if out == "i8" else None
+    args = dict(y_norm=1, y_weight=c["yw"], gate=c["gate"], x_norm=2, x_weight=c["xw"], scale=c["scale"], shift=c["shift"],
+                rows_per_sample=per, out_type=kind)
+    ref = ops.gate_add_norm(rx, c["y"], **args)
+    ops.gate_add_norm(x, y, out=o, out_scale=step, **args)
+    assert ((x - rx).abs() <= 2 * TERM * 12 * 3 + 4 * U * rx.abs()).all()
+    if out == "i8":
+        assert ((step - ref[1]).abs() <= 1e-4 * ref[1]).all() and int((o.int() - ref[0].int()).abs().max()) <= 1
+    else:
+        err = 1e-3 + (2.0 ** -7 * ref.float().abs() if out == "bf16" else 0)
+        assert ((o.float() - ref.float()).abs() <= err).all()
+    for buf, rows_of in ((xb, x), (ob, o)):
+        rows_of.fill_(3)
+        assert bool((buf == 3).all())
+
+
 def test_in_place_no_output_and_no_branch(cuda):
     import torch
     import mkimage
