@@ -719,6 +719,65 @@ cudaError_t launch_rows(const GemmI8Args& a, cudaStream_t st)
     return launch_k(k_i8_rows<MR, 1, 1>, dim3((a.N + 7) / 8), 256, 0, st, a);
 }
 
+// How k_i8_few would run: tokens a tile, parts of K, and about how long in steps of kBK of K (0.2 us each). Beside its steps
+// a tile takes 8, its epilogue 0.42 a token that a CTA finishes, and a cut of K 6.5 and 0.17 a token that is sent. Many parts
+// pay for long K (132 x 1056 x 6784: 16 tokens, whole 14.1 us, 64 tokens in four parts 8.8), small tiles for short K (77 x 1280
+// x 1280: 16 tokens in two parts 4.7, 64 in four 6.0).
+struct FewPlan {
+    int bn, splits;
+    float steps;
+};
+
+// Clusters of `size` (2, 4, 8) k_i8_few CTAs, one an SM, that the current device runs at once: they have to fit its GPCs (36
+// clusters of four are two waves: 192 x 288 x 9600 15.4 us, 18 of them 8.4). Kept for devices 0..63 once asked.
+int clusters_at_once(int size)
+{
+    static std::atomic<int> known[64][9];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess)
+        return 0;
+    const bool keep = dev >= 0 && dev < 64;
+    if (keep && known[dev][size].load(std::memory_order_relaxed))
+        return known[dev][size].load(std::memory_order_relaxed);
+    static std::atomic<uint64_t> devs{0};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(192);
+    cfg.dynamicSmemBytes = FewCfg<16>::kSmem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = size;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (smem_limit_once(devs, k_i8_few<16>, FewCfg<16>::kSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k_i8_few<16>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    if (keep)
+        known[dev][size].store(n, std::memory_order_relaxed);
+    return n;
+}
+
+FewPlan plan_few(long M, long N, int K)
+{
+    FewPlan best{0, 0, 0.0f};
+    const int num_k = (K + kBK - 1) / kBK;
+    for (int bn = 16; bn <= 64; bn *= 2) {
+        const long tiles = (M + bn - 1) / bn * ((N + 127) / 128);
+        // Parts that all run at once, two steps each or more.
+        for (int s = 1; s <= 8 && (s == 1 || (num_k >= 2 * s && tiles * s <= num_sms() && tiles <= clusters_at_once(s))); s *= 2) {
+            const float sent = s > 1 ? 6.5f + 0.17f * bn * (s - 1) / s : 0.0f;
+            const float steps = float((tiles + num_sms() - 1) / num_sms()) * ((num_k + s - 1) / s + 8.0f + 0.42f * bn / s + sent);
+            if (!best.bn || steps < best.steps)
+                best = FewPlan{bn, s, steps};
+        }
+    }
+    return best;
+}
+
 template <int BN>
 cudaError_t launch_few(I8Params& P, cudaStream_t st)
 {
@@ -726,11 +785,7 @@ cudaError_t launch_few(I8Params& P, cudaStream_t st)
     const cudaError_t e = smem_limit_once(devs, k_i8_few<BN>, FewCfg<BN>::kSmem);
     if (e != cudaSuccess)
         return e;
-    // K over as many CTAs as the SMs allow, two stages a part or more.
-    const int tiles = (P.a.M + BN - 1) / BN * ((P.a.N + 127) / 128), num_k = (P.a.K + kBK - 1) / kBK;
-    P.splits = 1;
-    while (P.splits < 8 && tiles * P.splits * 2 <= num_sms() && num_k >= 4 * P.splits)
-        P.splits *= 2;
+    const int tiles = (P.a.M + BN - 1) / BN * ((P.a.N + 127) / 128);
     return launch_k_cluster(k_i8_few<BN>, dim3(unsigned(tiles) * P.splits), P.splits, 192, FewCfg<BN>::kSmem, st, P);
 }
 
@@ -765,13 +820,6 @@ cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
     } else {
         I8Params P{};
         P.a = a;
-        // k_i8_few's tokens a tile: the fewest that leave no more than a tile for each SM (W comes out of L2 again for each
-        // tile, but K is cut less and an epilogue is short). Where that takes more than 32 of them, over 64 rows, the pair
-        // kernel is faster: 256 x 3072 x 3072 12.6 against 10.3 us; 200 x 1280 x 1280 5.4 against 6.8, 77 rows 4.7 against 6.4.
-        int few_bn = 16;
-        while (few_bn < 64 && (a.M + few_bn - 1L) / few_bn * ((a.N + 127L) / 128) > num_sms())
-            few_bn *= 2;
-        const bool few = a.M <= 64 || few_bn <= 32;
         // Pair tiles of 256, 192, 160 or 128 columns: a round of tiles takes about as long as its columns and 128 more (its rows
         // of x, the way in and out), so the width whose rounds take least, the widest among equals. In us, 256, 192, 160, 128
         // columns: 4097 x 1280 x 5120 31.1, 26.6, 25.5, 32.8; 700 x 8192 x 1024 13.0, 11.7, 14.5, 13.9; 512 x 9216 x 3072
@@ -784,16 +832,21 @@ cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
         for (const int width : {192, 160, 128})
             if (cost(width) < cost(bn))
                 bn = width;
+        // Against k_i8_few in its steps: a round of 128 columns takes one for each of K, and a launch 24 beside them (256 x 3072 x
+        // 3072 10.3 us here, 12.6 there; 200 x 1280 x 1280 6.8 and 5.3, 500 x 512 x 8192 18.0 and 9.4).
+        const FewPlan plan = plan_few(a.M, a.N, a.K);
+        const bool few = plan.steps <= float(cost(bn)) / 256.0f * ((a.K + kBK - 1) / kBK) + 24.0f;
+        P.splits = plan.splits;
         const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
-        if (!encode_2d(&P.tx, u8, a.x, a.K, a.M, a.ldx, kBK, few ? few_bn : 128) ||
+        if (!encode_2d(&P.tx, u8, a.x, a.K, a.M, a.ldx, kBK, few ? plan.bn : 128) ||
             !encode_2d(&P.tw, u8, a.w, a.K, a.N, a.ldw, kBK, few ? 128 : bn / 2)) {
             *err = "proj_i8: tensor map encoding failed";
             return cudaErrorInvalidValue;
         }
         if (few) {
-            e = few_bn == 16   ? launch_few<16>(P, st)
-                : few_bn == 32 ? launch_few<32>(P, st)
-                               : launch_few<64>(P, st);
+            e = plan.bn == 16   ? launch_few<16>(P, st)
+                : plan.bn == 32 ? launch_few<32>(P, st)
+                                : launch_few<64>(P, st);
         } else {
             e = bn == 256   ? launch_pair<256>(P, err, st)
                 : bn == 192 ? launch_pair<192>(P, err, st)

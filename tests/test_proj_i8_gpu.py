@@ -111,6 +111,24 @@ def test_largest_sums_are_exact(cuda, M):
     assert bool((out == float(128 * 128 * K)).all())
 
 
+# Few tiles over a long K: tiles of 16 to 64 tokens, K in one to eight parts.
+@pytest.mark.parametrize("M,N,K", [(132, 1056, 6784), (192, 288, 9600), (191, 290, 9408), (500, 512, 8192), (194, 1568, 11072),
+                                   (40, 2048, 8192), (300, 100, 12300), (60, 128, 12288), (30, 20000, 512), (13, 1664, 8192)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_parts_of_a_long_k(cuda, M, N, K, f32):
+    import torch
+    import mkimage
+
+    x, xs, w, ws, b = _case(cuda, M, N, K, M + N)
+    buf = torch.full((M + 2, N + 3), 5.0, dtype=torch.float32 if f32 else torch.bfloat16, device=cuda)
+    out = buf[1:M + 1, 1:N + 1]
+    mkimage.ops.proj_i8(x, xs, w, ws, bias=b, act=2, out=out)
+    assert mkimage.ops.check_kernels() == 0
+    _check(out, x, xs, w, ws, b, 2)
+    out.fill_(5)
+    assert bool((buf == 5).all())
+
+
 # Tiles of 160, 160, 192, 192, 128 and 256 columns on 148 SMs, whole and cut.
 @pytest.mark.parametrize("M,N", [(2000, 2560), (2000, 2467), (700, 8192), (705, 8101), (1030, 1500), (8000, 777)])
 @pytest.mark.parametrize("f32", [False, True])
