@@ -412,13 +412,15 @@ __global__ void __launch_bounds__(192, 1) k_i8_few(const __grid_constant__ I8Par
 constexpr int kEpiWarps = 8;
 constexpr int kPairThreads = 32 * (2 + kEpiWarps);
 
-template <int BN>
+template <int BN, bool F32>
 struct PairCfg {
     static constexpr int kABytes = 128 * kBK, kBBytes = BN / 2 * kBK, kStageBytes = kABytes + kBBytes;
-    static constexpr int kBox = 32 * 64;  // a warp's box: 32 rows of 64 bytes
-    static constexpr int kStages = BN == 256 ? 6 : BN > 128 ? 7 : 8;
+    // A warp's boxes of 32 rows of 64 bytes: one for bf16, two for fp32, whose 32 columns are two of them (3679 x 10240 x 1216
+    // with GELU 81 -> 74 us; the stage that they cost 256 columns: 8192 x 3072 x 3072 60.0 -> 61.5).
+    static constexpr int kBox = 32 * 64, kBoxes = F32 ? 2 : 1;
+    static constexpr int kStages = BN == 256 ? 6 - F32 : BN == 192 ? 7 - F32 : BN == 160 ? 7 : 8 - F32;
     static constexpr int kVec = 2 * 2 * BN * 4;  // w_scale and bias of two tiles
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + kEpiWarps * kBox + kVec + 256;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kEpiWarps * kBoxes * kBox + kVec + 256;
     static constexpr int kTmemCols = BN > 128 ? 512 : 256;  // two accumulators, a power of two
     static_assert(kStageBytes % 1024 == 0 && kSmem <= 227 * 1024);
 };
@@ -460,15 +462,15 @@ __device__ __forceinline__ void store_box(T* p, long ldy, const uint8_t* box, in
 // issues 256 x BN x 32 MMAs into one of two accumulators, warps 2-9 of both CTAs drain the other: a thread a row, 32 columns at
 // a time and every second 32 each, through a 2 KB box a warp that leaves as TMA stores. With four such warps and boxes of 4 KB
 // the epilogue was what the tensor pipe waited for (8192 x 12288 x 3072 with GELU 218 us, with eight 205).
-template <int BN>
+template <int BN, bool F32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i8_pair(const __grid_constant__ I8Params P)
 {
-    using C = PairCfg<BN>;
+    using C = PairCfg<BN, F32>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* boxes = smem + C::kStages * C::kStageBytes;
-    float* vec = reinterpret_cast<float*>(boxes + kEpiWarps * C::kBox);  // [2][w_scale, bias][BN]
-    uint64_t* full = reinterpret_cast<uint64_t*>(boxes + kEpiWarps * C::kBox + C::kVec);
+    float* vec = reinterpret_cast<float*>(boxes + kEpiWarps * C::kBoxes * C::kBox);  // [2][w_scale, bias][BN]
+    uint64_t* full = reinterpret_cast<uint64_t*>(boxes + kEpiWarps * C::kBoxes * C::kBox + C::kVec);
     uint64_t* empty = full + C::kStages;
     uint64_t* acc_full = empty + C::kStages;
     uint64_t* acc_empty = acc_full + 2;
@@ -575,8 +577,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i
     } else {
         const int q = warp & 3, et = int(threadIdx.x) - 64;
         const uint32_t acc_empty0 = map_to_cta(smem_u32(&acc_empty[0]), 0);
-        uint8_t* box = boxes + (warp - 2) * C::kBox;
-        uint32_t lt = 0;
+        uint8_t* const own = boxes + (warp - 2) * C::kBoxes * C::kBox;
+        uint32_t lt = 0, turn = 0;
         for (int tile = pair; tile < num_tiles; tile += npairs, ++lt) {
             int mb, nb;
             tile_of(tile, num_m, num_n, mb, nb);
@@ -613,13 +615,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i
                     v[j + 2] = fmaf(float(int(t[j + 2])) * sx, s.z, b.z);
                     v[j + 3] = fmaf(float(int(t[j + 3])) * sx, s.w, b.w);
                 }
-                act_out(v, a.act, a.out_f32);
+                act_out(v, a.act, F32);
                 // Through the box to columns from `col`: as a TMA store, or along rows that TMA cannot address (a thread storing
                 // its own row: 45 against 16 us at 2300 x 2100 x 2048 to bf16, 81 against 19 at 8000 x 777 x 1000) and the last
                 // columns (a cut box would write zeros as far as a piece of 16 bytes goes).
                 const auto send = [&](const uint4 (&w)[4], int col, auto* y) {
+                    uint8_t* box = own + turn++ % C::kBoxes * C::kBox;
                     if (lane == 0)
-                        bulk_wait_read<0>();  // the last store has read the box
+                        bulk_wait_read<C::kBoxes - 1>();  // the last store from this box has read it
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -627,6 +630,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i
                     if (!P.boxes || col + int(64 / sizeof(*y)) > a.N) {
                         __syncwarp();
                         store_box(y + row0 * a.ldy + col, a.ldy, box, a.M - row0, a.N - col, lane);
+                        if (lane == 0)
+                            bulk_commit();  // a group a box, empty here: the waits count them
                         return;
                     }
                     fence_proxy_async_smem();
@@ -637,7 +642,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i
                         bulk_commit();
                     }
                 };
-                if (a.out_f32) {
+                if constexpr (F32) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint4 w[4];
@@ -789,24 +794,30 @@ cudaError_t launch_few(I8Params& P, cudaStream_t st)
     return launch_k_cluster(k_i8_few<BN>, dim3(unsigned(tiles) * P.splits), P.splits, 192, FewCfg<BN>::kSmem, st, P);
 }
 
-template <int BN>
-cudaError_t launch_pair(I8Params& P, const char** err, cudaStream_t st)
+template <int BN, bool F32>
+cudaError_t launch_pair_of(I8Params& P, const char** err, cudaStream_t st)
 {
     const GemmI8Args& a = P.a;
-    const int size = a.out_f32 ? 4 : 2;
+    const int size = F32 ? 4 : 2;
     P.boxes = (reinterpret_cast<uintptr_t>(a.y) & 15) == 0 && (a.ldy * size) % 16 == 0;
-    if (P.boxes && !encode_2d(&P.ty, a.out_f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.N,
+    if (P.boxes && !encode_2d(&P.ty, F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.N,
                               a.M, a.ldy * size, 64 / size, 32, CU_TENSOR_MAP_SWIZZLE_64B)) {
         *err = "proj_i8: tensor map encoding failed";
         return cudaErrorInvalidValue;
     }
     const int tiles = int((a.M + 255L) / 256 * ((a.N + BN - 1L) / BN));
     static std::atomic<uint64_t> devs{0};
-    const cudaError_t e = smem_limit_once(devs, k_i8_pair<BN>, PairCfg<BN>::kSmem);
+    const cudaError_t e = smem_limit_once(devs, k_i8_pair<BN, F32>, PairCfg<BN, F32>::kSmem);
     if (e != cudaSuccess)
         return e;
     const int pairs = std::min(tiles, num_sms() / 2);
-    return launch_k(k_i8_pair<BN>, dim3(2 * pairs), kPairThreads, PairCfg<BN>::kSmem, st, P);
+    return launch_k(k_i8_pair<BN, F32>, dim3(2 * pairs), kPairThreads, PairCfg<BN, F32>::kSmem, st, P);
+}
+
+template <int BN>
+cudaError_t launch_pair(I8Params& P, const char** err, cudaStream_t st)
+{
+    return P.a.out_f32 ? launch_pair_of<BN, true>(P, err, st) : launch_pair_of<BN, false>(P, err, st);
 }
 
 }  // namespace
