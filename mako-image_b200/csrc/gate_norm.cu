@@ -396,9 +396,10 @@ struct Vectors {
     }
 };
 
-// A launch's arguments: a sample's blocks; out_whole: out's rows lie on the vectors' borders as x's do.
+// A launch's arguments: a sample's blocks, the rows that runs start at (ODD: the first four of a sample, or as many as it has);
+// out_whole: out's rows lie on the vectors' borders as x's do.
 struct GateNormOf : GateNormArgs {
-    unsigned blocks;
+    unsigned blocks, starts;
     bool out_whole;
 };
 
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(T, NC * VEC <= 12 ? (T == 256 ? 3 : 2) : 1) k_
     constexpr int kApart = ODD ? 4 : 1;
     const unsigned part = blockIdx.x % a.blocks;
     const long sample = blockIdx.x / a.blocks;
-    const long lo = sample * a.rows_per_sample + long(part / kApart) * run * kApart + part % kApart;
+    const long lo = sample * a.rows_per_sample + long(part / a.starts) * run * kApart + part % a.starts;
     const long hi = min(min(a.rows, (sample + 1) * a.rows_per_sample), lo + long(run) * kApart);
     const int n = a.n;
     const float inv_n = 1.0f / float(n);
@@ -579,7 +580,8 @@ cudaError_t launch_gate_norm_of(GateNormOf& a, int warps, cudaStream_t st)
         const long wave = long(num_sms()) * std::max(1, resident);
         run = int(std::min(apart, std::max(1L, (a.rows + wave - 1) / wave)));
     }
-    a.blocks = unsigned((apart + run - 1) / run * kApart);
+    a.starts = unsigned(std::min(a.rows_per_sample, long(kApart)));
+    a.blocks = unsigned((apart + run - 1) / run) * a.starts;
     return launch_k(k_gate_norm<VEC, NC, ODD, T>, dim3(unsigned(samples * a.blocks)), 32 * warps, smem, st, a, run);
 }
 
@@ -641,7 +643,7 @@ cudaError_t gate_norm(const GateNormArgs& args, cudaStream_t st)
 {
     if (args.rows == 0)
         return cudaSuccess;
-    GateNormOf a{args, 0, true};
+    GateNormOf a{args, 0, 1, true};
     a.rows_per_sample = std::min(a.rows_per_sample, a.rows);
     // Vectors of four where every row and vector allows them; rows that begin off a border, but alike, cut their end vectors
     // (1916 x 2719 to int8 21 us, value by value 31; 4803 x 5111 90 against 100); rows that begin differently go by value.

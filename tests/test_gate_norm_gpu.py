@@ -132,6 +132,17 @@ def test_runs_of_rows(cuda, rows, n, samples, out):
         _check(ops, c, per, y_norm, x_norm, tanh=y_norm == 1, mod=True, out_type=kind, in_place=y_norm == 1)
 
 
+@pytest.mark.parametrize("rows,n,per", [(7, 131, 1), (1001, 131, 2), (1001, 1283, 3), (1003, 131, 5), (2501, 333, 6), (999, 4099, 4)])
+def test_odd_rows_of_short_samples(cuda, rows, n, per):
+    """Samples of fewer rows than the four that runs of odd rows start at, and a few more."""
+    import mkimage
+
+    ops = mkimage.ops
+    c = _case(cuda, rows, n, rows + n, False, -(-rows // per))
+    _check(ops, c, per, 1, 2, True, True, ops.OUT_BF16)
+    _check(ops, c, per, 0, 1, False, True, ops.OUT_I8, in_place=True)
+
+
 @pytest.mark.parametrize("off_x,off_y,off_o", [(1, 1, 1), (1, 1, 2), (3, 3, 0), (2, 1, 1), (0, 2, 0)])
 @pytest.mark.parametrize("rows,n,ld", [(5, 129, 131), (700, 1283, 1283 + 8), (900, 640, 641), (420, 5111, 5119), (40, 12288, 12289)])
 @pytest.mark.parametrize("out", ["bf16", "f32", "i8"])
