@@ -217,8 +217,8 @@ enum { MKB_OUT_NONE = 0, MKB_OUT_BF16 = 1, MKB_OUT_F32 = 2, MKB_OUT_I8 = 3 };
  * is and only norms it). y: the branch's output, bf16 or fp32 (y_f32). y_weight and x_weight [n], gate, scale and shift
  * (those of sample row / rows_per_sample at gate + sample * gate_stride, scale + sample * mod_stride and shift + sample *
  * mod_stride) are fp32 and may each be NULL. out is written as out_type says, with out_scale [rows] for MKB_OUT_I8 (else
- * NULL). Statistics are fp32, a LayerNorm's squares are taken about its mean. n up to 12288, any alignment (16-byte aligned
- * rows and vectors with n a multiple of 4 take wide accesses). */
+ * NULL). Statistics are fp32, a LayerNorm's squares are taken about its mean. n up to 12288, any alignment (wide accesses where
+ * x, y and x_out begin alike: at one place of a group of four values, in every row). */
 mkb_status mkb_gate_add_norm(const float* x, long ldx, float* x_out, long ldxo, const void* y, long ldy, int y_f32,
                              int y_norm, const float* y_weight, const float* gate, long gate_stride, int tanh_gate,
                              int x_norm, const float* x_weight, const float* scale, const float* shift, long mod_stride,

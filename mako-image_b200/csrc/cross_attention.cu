@@ -170,8 +170,9 @@ struct Walk {
 
 // A row's step over CH chunks of 32 keys: its scores in tensor memory at ts to weights 2^(s sc - m), bf16, over the first
 // half of the same columns; the row's maximum m and sum l; O at `to` rescaled where the maximum grew. Of the last chunk only the
-// first `tail` keys are visible. With `masked` each score is cut at its key's bound, +inf or -inf (the minimum drops a NaN, and a visible NaN comes back as inf - inf). Straight code for each CH: the
-// chunks' loads, exponentials and stores interleave.
+// first `tail` keys are visible. With `masked` each score is cut at its key's bound, +inf or -inf (the minimum drops a NaN,
+// and a visible NaN comes back as inf - inf). Straight code for each CH: the chunks' loads, exponentials and stores
+// interleave.
 template <int D, int CH>
 __device__ __forceinline__ void softmax_step(uint32_t ts, uint32_t to, int tail, bool masked, const float* bound,
                                              float sc, bool first, float& m, float& l)
