@@ -132,6 +132,22 @@ def test_runs_of_rows(cuda, rows, n, samples, out):
         _check(ops, c, per, y_norm, x_norm, tanh=y_norm == 1, mod=True, out_type=kind, in_place=y_norm == 1)
 
 
+@pytest.mark.parametrize("n", [4000, 4040, 4043, 4044, 4056, 4093, 4096, 4097, 4100])
+@pytest.mark.parametrize("off", [0, 1])
+def test_widths_around_48_kb_of_vectors(cuda, n, off):
+    """Three vectors of 4096 values fill the shared memory that a launch has without asking, with aligned rows, odd ones and
+    ones that begin differently."""
+    import torch
+    import mkimage
+
+    ops = mkimage.ops
+    for rows in (3, 500):
+        c = _case(cuda, rows, n, n, False, 1)
+        y = torch.empty(rows * n + 8, dtype=torch.bfloat16, device=cuda)[off:off + rows * n].view(rows, n)
+        c["y"] = y.copy_(c["y"])
+        _check(ops, c, rows, 1, 1, True, True, ops.OUT_BF16)
+
+
 @pytest.mark.parametrize("rows,n,per", [(7, 131, 1), (1001, 131, 2), (1001, 1283, 3), (1003, 131, 5), (2501, 333, 6), (999, 4099, 4)])
 def test_odd_rows_of_short_samples(cuda, rows, n, per):
     """Samples of fewer rows than the four that runs of odd rows start at, and a few more."""
