@@ -599,7 +599,7 @@ cudaError_t launch_gate_norm_by_four(GateNormOf& a, int chunks, cudaStream_t st)
 {
     const bool many = a.rows > 2L * num_sms();
     // Rows with cut vectors: two chunks a warp at least where there are many (the warps with an end hold the others up at each
-    // reduction: 4099 x 1283 20.8 us on 6 warps, 24.3 on 11).
+    // reduction: 4099 x 1283 20.8 us on 4 warps, 24.3 on 11).
     const Deal d = deal(chunks, chunks <= 48 ? 3 : 6, many, ODD && many ? 2 : 1);
     return d.nc == 1   ? launch_gate_norm<4, 1, ODD>(a, d.warps, st)
            : d.nc == 2 ? launch_gate_norm<4, 2, ODD>(a, d.warps, st)
