@@ -26,66 +26,61 @@ constexpr int kBK = 128;  // bytes of K a stage: one 128-byte swizzle row
 
 // ------------------------------------------------------------------------------------------------ epilogue arithmetic
 
-// Activations. TANH_SFU: the GELU's tanh from the SFU (absolute error 2^-10.9, below the rounding of bf16 outputs);
-// otherwise (1 + tanh(u)) / 2 = 1 / (1 + e^-2u) to a few fp32 roundings.
-template <bool TANH_SFU>
+// v / (1 + 2^e).
+__device__ __forceinline__ float over_one_and_power(float v, float e)
+{
+    float p, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(e));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + p));
+    return v * r;
+}
+
+// Activations to a few fp32 roundings of their value (the erf form's are of v). The GELU's (1 + tanh(u)) / 2 is
+// 1 / (1 + e^-2u): 1 + tanh(u) cancels where v is negative, and with tanh.approx the result was off by a fifth of itself at -3.
+// The second SFU operation costs where tiles wait for their epilogue: 8192 x 12288 x 3072 to bf16 205 -> 207 us,
+// 3679 x 10240 x 1216 57 -> 63, 700 x 8192 x 1024 14.1 -> 15.1; nothing for few rows.
 __device__ __forceinline__ float act1(float v, int act)
 {
+    constexpr float kLog2e = 1.4426950408889634f;
     if (act == kActGeluTanh) {
-        const float u = 0.7978845608028654f * fmaf(0.044715f * v, v * v, v);
-        if constexpr (TANH_SFU) {
-            float t;
-            asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(u));
-            return 0.5f * v * (1.0f + t);
-        }
-        return __fdividef(v, 1.0f + __expf(-2.0f * u));
+        constexpr float c = -2.0f * 0.7978845608028654f * kLog2e;
+        return over_one_and_power(v, v * fmaf(c * 0.044715f, v * v, c));
     }
     if (act == kActSilu)
-        return __fdividef(v, 1.0f + __expf(-v));
+        return over_one_and_power(v, -kLog2e * v);
     if (act == kActQuickGelu)
-        return __fdividef(v, 1.0f + __expf(-1.702f * v));
+        return over_one_and_power(v, -1.702f * kLog2e * v);
     if (act == kActGeluErf)
         return 0.5f * v * (1.0f + erff(v * 0.7071067811865476f));
     return v;
 }
 
 // The switch outside the loop, so that the columns' chains interleave.
-template <bool TANH_SFU, int N>
-__device__ __forceinline__ void act_all(float (&v)[N], int act)
+template <int N>
+__device__ __forceinline__ void act_out(float (&v)[N], int act)
 {
     switch (act) {
     case kActGeluTanh:
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            v[j] = act1<TANH_SFU>(v[j], kActGeluTanh);
+            v[j] = act1(v[j], kActGeluTanh);
         break;
     case kActSilu:
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            v[j] = act1<TANH_SFU>(v[j], kActSilu);
+            v[j] = act1(v[j], kActSilu);
         break;
     case kActQuickGelu:
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            v[j] = act1<TANH_SFU>(v[j], kActQuickGelu);
+            v[j] = act1(v[j], kActQuickGelu);
         break;
     case kActGeluErf:
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            v[j] = act1<TANH_SFU>(v[j], kActGeluErf);
+            v[j] = act1(v[j], kActGeluErf);
         break;
     }
-}
-
-template <int N>
-__device__ __forceinline__ void act_out(float (&v)[N], int act, bool f32)
-{
-    if (act == kActNone)
-        return;
-    if (f32)
-        act_all<false>(v, act);
-    else
-        act_all<true>(v, act);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -173,7 +168,7 @@ __global__ void __launch_bounds__(256) k_i8_rows(const GemmI8Args a)
     if (m >= a.M || m >= MR || n >= a.N)
         return;
     float v[1] = {fmaf(float(s) * a.x_scale[m], a.w_scale[n], a.bias ? a.bias[n] : 0.0f)};
-    act_out(v, a.act, a.out_f32);
+    act_out(v, a.act);
     if (a.out_f32)
         static_cast<float*>(a.y)[m * a.ldy + n] = v[0];
     else
@@ -380,7 +375,7 @@ __global__ void __launch_bounds__(192, 1) k_i8_few(const __grid_constant__ I8Par
 #pragma unroll
             for (int j = 0; j < W; ++j)
                 v[j] = fmaf(float(int(s[j])) * sx[part * mine + c + j], sw, bias);
-            act_out(v, a.act, a.out_f32);
+            act_out(v, a.act);
             if (n < a.N)
 #pragma unroll
                 for (int j = 0; j < W; ++j)
@@ -615,7 +610,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i
                     v[j + 2] = fmaf(float(int(t[j + 2])) * sx, s.z, b.z);
                     v[j + 3] = fmaf(float(int(t[j + 3])) * sx, s.w, b.w);
                 }
-                act_out(v, a.act, F32);
+                act_out(v, a.act);
                 // Through the box to columns from `col`: as a TMA store, or along rows that TMA cannot address (a thread storing
                 // its own row: 45 against 16 us at 2300 x 2100 x 2048 to bf16, 81 against 19 at 8000 x 777 x 1000) and the last
                 // columns (a cut box would write zeros as far as a piece of 16 bytes goes).

@@ -1,0 +1,39 @@
+"""Ends of the quantised block's ranges: the negative tail of the projections' GELU. u = 2^-24, half a step of fp32."""
+
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+# One row and few rows, tiles of CTA pairs with one and several rounds.
+@pytest.mark.parametrize("M,N", [(1, 3000), (2, 3001), (7, 3000), (300, 12000), (2000, 6001)])
+@pytest.mark.parametrize("f32", [False, True])
+def test_gelu_tanh_keeps_its_negative_tail(cuda, M, N, f32):
+    """gelu(v) = v / (1 + e^-2u) with u = 0.798 (v + 0.0447 v^3), relative to the value however small it is.
+
+    x is zero, so v is the bias. u is off by 5 u of itself (its terms have one sign: two constants, three roundings), which moves
+    e^-2u by 10 |u| u; the exponential adds (2 + 1.18 * 2 |u|) ulp = (4 + 4.8 |u|) u, the sum 1 u, the division 2 ulp = 4 u:
+    (9 + 15 |u|) u in all. bf16 adds 2^-8 of the value. A quotient by more than 2^126 may be 0: 16 / 2^126."""
+    import torch
+    import mkimage
+
+    K = 640
+    v = torch.linspace(-13, 4, N, device=cuda)
+    x = torch.zeros(M, K, dtype=torch.int8, device=cuda)
+    w = torch.ones(N, K, dtype=torch.int8, device=cuda)
+    out = mkimage.ops.proj_i8(x, torch.ones(M, device=cuda), w, torch.ones(N, device=cuda), bias=v, act=mkimage.ops.ACT_GELU_TANH,
+                              out_f32=f32)
+    assert mkimage.ops.check_kernels() == 0
+    v = v.double()
+    u = math.sqrt(2 / math.pi) * (v + 0.044715 * v ** 3)
+    ref = v * torch.sigmoid(2 * u)
+    tol = (9 + 15 * u.abs()) * U * ref.abs() + 2.0 ** -122
+    if not f32:
+        tol = tol * (1 + 2.0 ** -8) + 2.0 ** -8 * ref.abs()
+    err = (out.double() - ref).abs()
+    good = bool((err <= tol).all())
+    assert good, float((err / ref.abs()).max())
