@@ -20,7 +20,7 @@ __device__ __forceinline__ float max_abs(float m, float x)
 
 struct RowStep {
     static constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, ties to even
-    float step, inv, half;
+    float step, inv;
     __device__ __forceinline__ explicit RowStep(float amax)
     {
         step = amax <= 3.4028235e38f ? __fdiv_rn(amax, 127.0f) : __uint_as_float(0x7fffffffu);
@@ -28,12 +28,12 @@ struct RowStep {
             step = 0.0f;
         // A row of zeros, or one with an infinity or a NaN in it (step NaN), has only zeros.
         inv = step > 0.0f ? 1.0f / step : 0.0f;
-        half = 0.5f * step;
     }
     // x / step to the nearest whole number, ties to even, as the low byte of each result's bits. x * inv is off by a few
     // roundings, so its nearest whole number may be one off next to a border of two; the remainder x - q step decides. It is
     // a multiple of the smaller of the two numbers' last places and no larger than about step / 2, so the fused
-    // multiply-add gives it without rounding.
+    // multiply-add gives it without rounding. Twice the remainder is set against the step: below 2^-125 half a step may be no
+    // fp32 number.
     template <int N>
     __device__ __forceinline__ void whole(const float (&x)[N], float (&t)[N]) const
     {
@@ -41,12 +41,12 @@ struct RowStep {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             t[i] = fmaf(x[i], inv, kRound);
-            far = fmaxf(far, fabsf(fmaf(kRound - t[i], step, x[i])) - half);
+            far = fmaxf(far, fmaf(2.0f, fabsf(fmaf(kRound - t[i], step, x[i])), -step));
         }
         if (far >= 0.0f) {  // on or beyond a border: rare
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float r = fmaf(kRound - t[i], step, x[i]), over = fabsf(r) - half;
+                const float r = fmaf(kRound - t[i], step, x[i]), over = fmaf(2.0f, fabsf(r), -step);
                 if (over > 0.0f || (over == 0.0f && (__float_as_int(t[i]) & 1)))
                     t[i] += copysignf(1.0f, r);
             }

@@ -1,4 +1,5 @@
-"""Ends of the quantised block's ranges: the negative tail of the projections' GELU. u = 2^-24, half a step of fp32."""
+"""Ends of the quantised block's ranges: the negative tail of the projections' GELU, steps at the small end
+of fp32. u = 2^-24, half a step of fp32."""
 
 import math
 
@@ -37,3 +38,28 @@ def test_gelu_tanh_keeps_its_negative_tail(cuda, M, N, f32):
     err = (out.double() - ref).abs()
     good = bool((err <= tol).all())
     assert good, float((err / ref.abs()).max())
+
+
+def test_quantize_rows_at_the_smallest_steps(cuda):
+    """Steps in [2^-126, 2^-125), where half a step may be no fp32 number: quotients on and next to every border."""
+    import torch
+    import mkimage
+
+    g = torch.Generator().manual_seed(5)
+    low = 127 * 2.0 ** -126
+    tops = torch.cat([torch.tensor([low], dtype=torch.float64), low * (1 + torch.rand(200, generator=g, dtype=torch.float64)),
+                      torch.tensor([2 * low, 2.3 * low], dtype=torch.float64)]).float()
+    step = (tops / torch.tensor(127.0)).double()
+    k = torch.arange(-127, 127, dtype=torch.float64) + 0.5
+    at = (k[None] * step[:, None]).float()
+    inf = torch.full_like(at, math.inf)
+    x = torch.cat([tops[:, None], at, torch.nextafter(at, inf), torch.nextafter(at, -inf)], 1)
+    x = torch.minimum(torch.maximum(x, -tops[:, None]), tops[:, None])
+    want = (x.double() / step[:, None]).round()
+    assert int((step * 2.0 ** 149).long().remainder(2).sum()) > 50  # odd significands are among them
+    for pad in (0, 1):  # single values, vectors of four
+        n = x.shape[1] + pad
+        q, got = mkimage.ops.quantize_rows(torch.cat([x, x[:, 1:2]], 1)[:, :n].to(cuda))
+        wrong = int((q.double().cpu() != torch.cat([want, want[:, 1:2]], 1)[:, :n]).sum())
+        same = torch.equal(got.double().cpu(), step)
+        assert wrong == 0 and same
