@@ -1,5 +1,5 @@
-"""Ends of the quantised block's ranges: the negative tail of the projections' GELU, steps at the small end
-of fp32. u = 2^-24, half a step of fp32."""
+"""Ends of the quantised block's ranges: the negative tail of the projections' GELU, steps at the small end of fp32, a gate's
+tanh on both sides of its two forms. u = 2^-24, half a step of fp32."""
 
 import math
 
@@ -63,3 +63,30 @@ def test_quantize_rows_at_the_smallest_steps(cuda):
         wrong = int((q.double().cpu() != torch.cat([want, want[:, 1:2]], 1)[:, :n]).sum())
         same = torch.equal(got.double().cpu(), step)
         assert wrong == 0 and same
+
+
+@pytest.mark.parametrize("n", [12288, 5001])
+def test_gate_tanh_on_both_sides_of_its_forms(cuda, n):
+    """x = 0 and y = 1, so the residual that comes out is tanh(gate) alone.
+
+    Below 0.4 a series x + x^3 p(x^2): what it leaves out is under 2^-27 of x there, x^3 p is under 0.06 of x with roundings of
+    4 u of itself, the last sum is one more: 1.5 u. From 0.4 on 1 - t, t = 2 / (e^2a + 1): the exponential is off by
+    (2 + 1.18 * 2 a) ulp = (4 + 4.8 a) u of itself, the sum by 1 u, the division by 2 ulp = 4 u, the difference by 1 u of the
+    result, one more u for the product with y and the sum with x."""
+    import torch
+    import mkimage
+
+    a = torch.cat([torch.linspace(0, 0.42, n // 2), torch.linspace(0.35, 0.45, n // 4), torch.linspace(0.4, 12, n - n // 2 - n // 4)])
+    for sign in (1, -1):
+        gate = (sign * a).to(cuda)
+        out = torch.empty(1, n, device=cuda)
+        mkimage.ops.gate_add_norm(torch.zeros(1, n, device=cuda), torch.ones(1, n, device=cuda), gate=gate, tanh_gate=True,
+                                  x_out=out, out_type=mkimage.ops.OUT_NONE)
+        g = gate.double()
+        ref, t = torch.tanh(g), 2 / (torch.exp(2 * g.abs()) + 1)
+        tol = torch.where(g.abs() < 0.4 + 1e-6, 1.5 * U * ref.abs(), torch.zeros_like(g))
+        big = ((9 + 4.8 * g.abs()) * t + 2 * ref.abs()) * U
+        tol = torch.where(g.abs() >= 0.4 - 1e-6, torch.maximum(tol, big), tol)
+        err = (out[0].double() - ref).abs()
+        good = bool((err <= tol).all())
+        assert good, (float((err - tol).max()), float(g[(err - tol).argmax()]))
