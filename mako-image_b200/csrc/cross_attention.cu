@@ -781,8 +781,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_cross(const __grid_constant__ C
 
 constexpr int kFewRows = 4;    // query rows that share a key head
 constexpr int kFewWarps = 8;
-// K and V rows a lane takes a round, each, and the rounds in flight: 64 KB a CTA, three CTAs an SM (96 KB: 27 against 22 us at
-// 2 x 24 heads of 128 over 4096 keys). Several query rows leave registers for two rows a round (two rows: 23 against 29 us).
+// K and V rows a lane takes a round, each, and the rounds in flight: 64 KB a CTA, so that three of one or two rows fit an SM
+// (96 KB: 27 against 22 us at 2 x 24 heads of 128 over 4096 keys). Several query rows leave registers for two rows a round (two rows: 23 against 29 us).
 template <int R>
 struct FewCfg {
     static constexpr int kDepth = R == 1 ? 4 : 2, kRounds = 8 / kDepth;
@@ -1150,18 +1150,41 @@ cudaError_t launch(const CrossParams& P, cudaStream_t st)
                          : launch<D, kHideNone>(P, st);
 }
 
+// k_cross_few CTAs that an SM of the current device holds: three, but two of four rows' (128 registers a thread, and at D = 128
+// the warps' parts take 16 KB beside the rounds). Kept for devices 0..63 once asked.
+template <int D, int R>
+int few_at_once()
+{
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess)
+        return 1;
+    const bool keep = dev >= 0 && dev < 64;
+    if (keep && known[dev].load(std::memory_order_relaxed))
+        return known[dev].load(std::memory_order_relaxed);
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_cross_few<D, R>, 32 * kFewWarps, kFewSmem) != cudaSuccess) {
+        cudaGetLastError();
+        return 1;
+    }
+    n = std::max(1, n);
+    if (keep)
+        known[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 template <int D, int R>
 cudaError_t launch_few(const CrossArgs& a, cudaStream_t st)
 {
-    // The keys over as many CTAs as the SMs hold at once, three each, 128 keys a CTA or more (four an SM leave a second wave:
-    // 128 key heads of 4096 keys 61 against 51 us; the size that divides the CTAs most evenly over the SMs instead, 6 for 8 at
-    // 48 key heads, was slower: 23.6 against 22.4 us).
-    const int pairs = a.B * a.Hkv;
-    const int splits = std::max(1, std::min({kMaxSplits, kFewWarps, 3 * num_sms() / pairs, a.Lk / 128}));
     static std::atomic<uint64_t> devs{0};
     const cudaError_t e = smem_limit_once(devs, k_cross_few<D, R>, kFewSmem);
     if (e != cudaSuccess)
         return e;
+    // The keys over as many CTAs as the SMs hold at once, 128 keys a CTA or more (more than that leave a second wave: 128 key
+    // heads of 4096 keys 61 against 51 us, 148 of 512 keys with four rows each 24.7 against 16.4; the size that divides the CTAs most evenly over the SMs instead, 6 for 8 at 48 key
+    // heads, was slower: 23.6 against 22.4 us).
+    const int pairs = a.B * a.Hkv;
+    const int splits = std::max(1, std::min({kMaxSplits, kFewWarps, few_at_once<D, R>() * num_sms() / pairs, a.Lk / 128}));
     return launch_k_cluster(k_cross_few<D, R>, dim3(pairs * splits), splits, 32 * kFewWarps, kFewSmem, st, a, splits);
 }
 

@@ -1,5 +1,5 @@
 """Ends of the quantised block's ranges: the negative tail of the projections' GELU, steps at the small end of fp32, a gate's
-tanh on both sides of its two forms. u = 2^-24, half a step of fp32."""
+tanh on both sides of its two forms, a few query rows of as many key heads as fill the GPU. u = 2^-24, half a step of fp32."""
 
 import math
 
@@ -90,3 +90,28 @@ def test_gate_tanh_on_both_sides_of_its_forms(cuda, n):
         err = (out[0].double() - ref).abs()
         good = bool((err <= tol).all())
         assert good, (float((err - tol).max()), float(g[(err - tol).argmax()]))
+
+
+@pytest.mark.parametrize("B,H,Hkv,Lq,Lk,d", [(4, 148, 37, 1, 512, 128), (4, 148, 37, 1, 512, 64), (4, 30, 30, 4, 400, 128),
+                                             (4, 111, 37, 1, 300, 128), (4, 74, 37, 1, 512, 128), (5, 60, 60, 1, 700, 64)])
+def test_few_rows_of_many_key_heads(cuda, B, H, Hkv, Lq, Lk, d):
+    """Key heads for one, two and three CTAs an SM. Weights and sums are fp32 here, so 2^-11 of sum p|v| / sum p covers the
+    scores' and the exponentials' errors, and the bf16 output is 2^-8 of the value; a sample without keys is zeros."""
+    import torch
+    import mkimage
+
+    g = torch.Generator().manual_seed(H + Lk)
+    q, k, v = (torch.randn(B, h, n, d, generator=g).to(torch.bfloat16).to(cuda) for h, n in ((H, Lq), (Hkv, Lk), (Hkv, Lk)))
+    lens = torch.tensor([Lk, 0, Lk // 3, 1, Lk - 1][:B], dtype=torch.int32, device=cuda)
+    got = mkimage.ops.cross_attention(q, k, v, key_len=lens).reshape(B, Lq, H, d).double()
+    assert mkimage.ops.check_kernels() == 0
+    for b in range(B):
+        n = int(lens[b])
+        if n == 0:
+            assert int((got[b] != 0).sum()) == 0
+            continue
+        kk, vv = (t[b, :, :n].double().repeat_interleave(H // Hkv, 0) for t in (k, v))
+        p = torch.softmax(q[b].double() @ kk.transpose(1, 2) / math.sqrt(d), -1)
+        ref, mag = (p @ vv).transpose(0, 1), (p @ vv.abs()).transpose(0, 1)
+        good = bool(((got[b] - ref).abs() <= 2.0 ** -11 * mag + 2.0 ** -8 * ref.abs()).all())
+        assert good, b
