@@ -631,6 +631,13 @@ mkb_status mkb_check_kernels(uint32_t* bits);
 mkb_status mkb_selftest_stalled_gemm(const void* x, long ldx, const void* w, long ldw, float* y, long ldy, int M,
                                      int N, int K, void* stream);
 
+/* The same for mkb_proj_i8 to fp32 on CTA pairs, whose loads complete on the barriers of a pair's first CTA: CTA 0 never
+ * loads its half of the first stage. Both CTAs of its pair give up after 2 s, the first waits for what either has loaded
+ * (another 2 s on the withheld half) and both return; the other pairs finish. mkb_check_kernels then returns MKB_ERR_KERNEL
+ * with bits among 0 to 3 (the roles that gave up) and bit 4. For tests of error detection; nothing else calls it. */
+mkb_status mkb_selftest_stalled_proj_i8(const int8_t* x, long ldx, const float* x_scale, const int8_t* w, long ldw,
+                                        const float* w_scale, float* y, long ldy, int M, int N, int K, void* stream);
+
 /* Failure-path self-test of the head exchange's wait for its peers (mkb_dit_sp_head_exchange mode 2; no counterpart
  * in the reference): launches the wait that holds a rank's output projection until every flag in `flags` (n device
  * words, the rank's own at index `self` skipped) has reached *value (a device word). A flag that stays below runs

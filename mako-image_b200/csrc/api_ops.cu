@@ -107,6 +107,31 @@ mkb_status run_gemm(Epi epi, const void* x, long ldx, const void* w, long ldw, G
 
 int pick_bn(int M, int N) { return gemm_pick_tile(M, N, true).bn; }
 
+mkb_status proj_i8(const int8_t* x, long ldx, const float* x_scale, const int8_t* w, long ldw, const float* w_scale,
+                   const float* bias, void* y, long ldy, int M, int N, int K, int act, int out_f32, int test_stall, void* stream)
+{
+    if (act < MKB_ACT_NONE || act > MKB_ACT_GELU_ERF)
+        return fail(MKB_ERR_INVALID, "proj_i8: unknown activation");
+    if (M < 0 || N <= 0 || K <= 0 || K > kI8MaxK)
+        return fail(MKB_ERR_INVALID, "proj_i8: need M >= 0, N > 0 and 0 < K <= 131071 (exact 32-bit sums)");
+    if (M > (1 << 30) || N > (1 << 30) || double((M + 127L) / 128) * double((N + 127L) / 128) > double(1 << 30))
+        return fail(MKB_ERR_INVALID, "proj_i8: need M, N <= 2^30 and no more than 2^30 output tiles of 128 x 128");
+    if (ldx < K || ldw < K || ldy < N || (ldx & 15) || (ldw & 15))
+        return fail(MKB_ERR_INVALID, "proj_i8: need ldx, ldw >= K and multiples of 16, ldy >= N");
+    if (M == 0)
+        return MKB_OK;
+    if (!x || !x_scale || !w || !w_scale || !y)
+        return fail(MKB_ERR_INVALID, "proj_i8: null argument");
+    if ((reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(w) & 15) ||
+        (reinterpret_cast<uintptr_t>(y) & (out_f32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(x_scale) & 3) ||
+        (reinterpret_cast<uintptr_t>(w_scale) & 3) || (reinterpret_cast<uintptr_t>(bias) & 3))
+        return fail(MKB_ERR_INVALID, "proj_i8: x and w need 16-byte alignment, the others their element's");
+    GemmI8Args a{x, ldx, x_scale, w, ldw, w_scale, bias, y, ldy, M, N, K, act, out_f32, device_status_word(), test_stall};
+    const char* err = nullptr;
+    const cudaError_t e = gemm_i8(a, &err, static_cast<cudaStream_t>(stream));
+    return err ? fail(MKB_ERR_INVALID, err) : cuda_status(e, "proj_i8 launch");
+}
+
 }  // namespace
 
 }  // namespace mkb
@@ -436,26 +461,7 @@ mkb_status mkb_quantize_rows(const void* x, long ldx, int x_f32, int8_t* q, long
 mkb_status mkb_proj_i8(const int8_t* x, long ldx, const float* x_scale, const int8_t* w, long ldw, const float* w_scale,
                        const float* bias, void* y, long ldy, int M, int N, int K, int act, int out_f32, void* stream)
 {
-    if (act < MKB_ACT_NONE || act > MKB_ACT_GELU_ERF)
-        return fail(MKB_ERR_INVALID, "proj_i8: unknown activation");
-    if (M < 0 || N <= 0 || K <= 0 || K > kI8MaxK)
-        return fail(MKB_ERR_INVALID, "proj_i8: need M >= 0, N > 0 and 0 < K <= 131071 (exact 32-bit sums)");
-    if (M > (1 << 30) || N > (1 << 30) || double((M + 127L) / 128) * double((N + 127L) / 128) > double(1 << 30))
-        return fail(MKB_ERR_INVALID, "proj_i8: need M, N <= 2^30 and no more than 2^30 output tiles of 128 x 128");
-    if (ldx < K || ldw < K || ldy < N || (ldx & 15) || (ldw & 15))
-        return fail(MKB_ERR_INVALID, "proj_i8: need ldx, ldw >= K and multiples of 16, ldy >= N");
-    if (M == 0)
-        return MKB_OK;
-    if (!x || !x_scale || !w || !w_scale || !y)
-        return fail(MKB_ERR_INVALID, "proj_i8: null argument");
-    if ((reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(w) & 15) ||
-        (reinterpret_cast<uintptr_t>(y) & (out_f32 ? 3 : 1)) || (reinterpret_cast<uintptr_t>(x_scale) & 3) ||
-        (reinterpret_cast<uintptr_t>(w_scale) & 3) || (reinterpret_cast<uintptr_t>(bias) & 3))
-        return fail(MKB_ERR_INVALID, "proj_i8: x and w need 16-byte alignment, the others their element's");
-    GemmI8Args a{x, ldx, x_scale, w, ldw, w_scale, bias, y, ldy, M, N, K, act, out_f32, device_status_word()};
-    const char* err = nullptr;
-    const cudaError_t e = gemm_i8(a, &err, static_cast<cudaStream_t>(stream));
-    return err ? fail(MKB_ERR_INVALID, err) : cuda_status(e, "proj_i8 launch");
+    return proj_i8(x, ldx, x_scale, w, ldw, w_scale, bias, y, ldy, M, N, K, act, out_f32, 0, stream);
 }
 
 mkb_status mkb_gate_add_norm(const float* x, long ldx, float* x_out, long ldxo, const void* y, long ldy, int y_f32,
@@ -584,6 +590,12 @@ mkb_status mkb_selftest_stalled_gemm(const void* x, long ldx, const void* w, lon
         return fail(MKB_ERR_INVALID, err ? err : "selftest: unsupported arguments");
     op.p.test_stall = 1;  // the 1-CTA kernel: CTA 0 withholds its first stage's load
     return cuda_status(gemm_launch(op, static_cast<cudaStream_t>(stream)), "selftest launch");
+}
+
+mkb_status mkb_selftest_stalled_proj_i8(const int8_t* x, long ldx, const float* x_scale, const int8_t* w, long ldw,
+                                        const float* w_scale, float* y, long ldy, int M, int N, int K, void* stream)
+{
+    return proj_i8(x, ldx, x_scale, w, ldw, w_scale, nullptr, y, ldy, M, N, K, MKB_ACT_NONE, 1, 1, stream);
 }
 
 mkb_status mkb_check_kernels(uint32_t* bits)

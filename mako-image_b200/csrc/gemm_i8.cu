@@ -472,6 +472,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i
     uint64_t* drain = acc_empty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile uint32_t* gave_up = tmem_slot + 2;  // either CTA's roles
+    volatile uint32_t* loaded = tmem_slot + 3;   // the leader's: stages that each CTA had loaded when it gave up
     const GemmI8Args& a = P.a;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = cluster_ctarank();
@@ -491,6 +493,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
+        *gave_up = 0;
+        loaded[0] = loaded[1] = ~0u;
         fence_barrier_init();
     }
     if (warp == 0 && lane == 0) {
@@ -508,10 +512,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i
     tc_fence_after();
     grid_dep_launch();
     const uint32_t tmem = *tmem_slot;
+    uint32_t it = 0;  // warp 0: stages loaded; warp 1: stages multiplied
 
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t it = 0;
             bool ok = true;
             for (int tile = pair; tile < num_tiles && ok; tile += npairs) {
                 int mb, nb;
@@ -525,6 +529,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i
                     uint8_t* sa = smem + s * C::kStageBytes;
                     if (leader)
                         mbar_arrive_expect_tx(&full[s], 2 * C::kStageBytes);  // both CTAs' loads land on it
+                    if (a.test_stall && it == 0 && blockIdx.x == 0)
+                        continue;  // half of the stage's bytes never arrive: full[0] cannot complete (failure-path test)
                     tma_load_2d_pair(sa, &P.tx, &full[s], kb * kBK, mb * 256 + int(rank) * 128);
                     tma_load_2d_pair(sa + C::kABytes, &P.tw, &full[s], kb * kBK, nb * BN + int(rank) * (BN / 2));
                 }
@@ -534,7 +540,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i
         // The leader's whole warp walks and waits, so that descriptors stay in uniform registers; one lane issues.
         if (leader) {
             constexpr uint32_t idesc = idesc_i8_s32(256, BN);
-            uint32_t it = 0, lt = 0;
+            uint32_t lt = 0;
             bool ok = true;
             for (int tile = pair; tile < num_tiles && ok; tile += npairs, ++lt) {
                 const uint32_t acc = lt & 1, acc_ph = (lt >> 1) & 1;
@@ -588,6 +594,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i
             }
             const float sx = row < a.M ? __ldg(a.x_scale + row) : 0.0f;
             const bool got = mbar_wait(&acc_full[acc], acc_ph, a.status, kErrWaitAccFull, abort_flag);
+            __syncwarp();  // a wait that ran out may have left the lanes apart
             // Also publishes the vectors; the warps leave together or not at all.
             if (named_barrier_or<1, 32 * kEpiWarps>(!got))
                 break;
@@ -669,7 +676,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i
     }
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag) {
+        st_cluster(map_to_cta(smem_u32(const_cast<uint32_t*>(loaded) + rank), 0), it);
+        for (uint32_t c = 0; c < 2; ++c)
+            st_cluster(map_to_cta(smem_u32(const_cast<uint32_t*>(gave_up)), c), 1);
+    }
+    __syncwarp();
     cluster_sync_all();  // the leader's MMAs read this CTA's shared memory until here
+    if (*gave_up) {
+        // Let the loads already issued land before either CTA can exit. They complete on the leader's barriers, which it alone
+        // can wait on; a stage that only the other CTA has loaded expects that CTA's bytes, one that only this CTA has (the
+        // other gave up first) does not complete, and its wait runs out: the rest have had as long.
+        if (threadIdx.x == 0 && leader) {
+            const uint32_t whole = uint32_t((num_tiles - pair + npairs - 1) / npairs) * num_k;  // where a CTA did not give up
+            const uint32_t mine = min(loaded[0], whole), all = max(mine, min(loaded[1], whole));
+            for (uint32_t j = all > C::kStages ? all - C::kStages : 0; j < all; ++j) {
+                if (j >= mine)
+                    mbar_arrive_expect_tx(&full[j % C::kStages], C::kStageBytes);
+                if (!mbar_wait(&full[j % C::kStages], (j / C::kStages) & 1, a.status, kErrWaitDrain, nullptr))
+                    break;
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();
+    }
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc_pair(tmem, C::kTmemCols);
@@ -820,7 +850,7 @@ cudaError_t launch_pair(I8Params& P, const char** err, cudaStream_t st)
 cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
 {
     cudaError_t e;
-    if (a.M <= kRowsMax) {
+    if (a.M <= kRowsMax && !a.test_stall) {
         e = a.M == 1   ? launch_rows<1>(a, st)
                        : launch_rows<2>(a, st);
     } else {
@@ -841,7 +871,7 @@ cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st)
         // Against k_i8_few in its steps: a round of 128 columns takes one for each of K, and a launch 24 beside them (256 x 3072 x
         // 3072 10.3 us here, 12.6 there; 200 x 1280 x 1280 6.8 and 5.3, 500 x 512 x 8192 18.0 and 9.4).
         const FewPlan plan = plan_few(a.M, a.N, a.K);
-        const bool few = plan.steps <= float(cost(bn)) / 256.0f * ((a.K + kBK - 1) / kBK) + 24.0f;
+        const bool few = !a.test_stall && plan.steps <= float(cost(bn)) / 256.0f * ((a.K + kBK - 1) / kBK) + 24.0f;
         P.splits = plan.splits;
         const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
         if (!encode_2d(&P.tx, u8, a.x, a.K, a.M, a.ldx, kBK, few ? plan.bn : 128) ||

@@ -23,6 +23,8 @@ struct GemmI8Args {
     int act;  // Act of gemm.cuh
     int out_f32;
     uint32_t* status;
+    // Failure-path testing only (mkb_selftest_stalled_proj_i8): the pair kernel's CTA 0 withholds its first stage's load.
+    int test_stall = 0;
 };
 cudaError_t gemm_i8(const GemmI8Args& a, const char** err, cudaStream_t st);
 

@@ -1,5 +1,6 @@
 """Ends of the quantised block's ranges: the negative tail of the projections' GELU, steps at the small end of fp32, a gate's
-tanh on both sides of its two forms, a few query rows of as many key heads as fill the GPU. u = 2^-24, half a step of fp32."""
+tanh on both sides of its two forms, a few query rows of as many key heads as fill the GPU, a pair of CTAs whose
+load never comes. u = 2^-24, half a step of fp32."""
 
 import math
 
@@ -115,3 +116,33 @@ def test_few_rows_of_many_key_heads(cuda, B, H, Hkv, Lq, Lk, d):
         ref, mag = (p @ vv).transpose(0, 1), (p @ vv.abs()).transpose(0, 1)
         good = bool(((got[b] - ref).abs() <= 2.0 ** -11 * mag + 2.0 ** -8 * ref.abs()).all())
         assert good, b
+
+
+def test_a_stalled_pair_gives_up_and_the_context_survives(cuda):
+    """A pair whose first CTA never loads its half of the first stage: the roles' 2 s waits run out, so does the wait for the
+    loads in flight, and the kernel returns; the other pairs' rows are right, and so is the next call."""
+    import ctypes
+    import time
+
+    import torch
+    import mkimage
+
+    M, N, K = 1024, 512, 2048
+    g = torch.Generator().manual_seed(8)
+    x, w = (torch.randint(-128, 128, (r, K), generator=g, dtype=torch.int8).to(cuda) for r in (M, N))
+    xs, ws = torch.ones(M, device=cuda), torch.ones(N, device=cuda)
+    y = torch.zeros(M, N, device=cuda)
+    ref = (x.double() @ w.double().T).float()
+    assert mkimage.ops.check_kernels() == 0
+    t0 = time.time()
+    p = [t.data_ptr() for t in (x, xs, w, ws, y)]
+    mkimage.check(mkimage.lib.mkb_selftest_stalled_proj_i8(p[0], K, p[1], p[2], K, p[3], p[4], N, M, N, K, None))
+    bits = ctypes.c_uint32()
+    code = mkimage.lib.mkb_check_kernels(ctypes.byref(bits))  # synchronises: the kernel has returned by now
+    elapsed = time.time() - t0
+    assert code == 4 and bits.value & 15 and bits.value & 16, (code, hex(bits.value))
+    assert 3 < elapsed < 30, elapsed
+    right = (y == ref).all(1)
+    assert int(right.sum()) >= M // 2  # the first pair's tile, 256 rows, is not among them
+    assert mkimage.ops.check_kernels() == 0
+    assert torch.equal(mkimage.ops.proj_i8(x, xs, w, ws, out_f32=True), ref) and mkimage.ops.check_kernels() == 0
