@@ -214,7 +214,7 @@ enum { MKB_OUT_NONE = 0, MKB_OUT_BF16 = 1, MKB_OUT_F32 = 2, MKB_OUT_I8 = 3 };
  *   x_out = x + g(gate) * N_y(y) * y_weight         (g: identity, or tanh with tanh_gate)
  *   out   = N_x(x_out) * x_weight * (1 + scale) + shift
  * x, x_out: the fp32 residual stream [rows][n] (x_out may be x; NULL or x where y is NULL, which leaves the residual as it
- * is and only norms it). y: the branch's output, bf16 or fp32 (y_f32). y_weight and x_weight [n], gate, scale and shift
+ * is and only norms it). out may take x's or y's place, row for row in the same type, but not x_out's beside it. y: the branch's output, bf16 or fp32 (y_f32). y_weight and x_weight [n], gate, scale and shift
  * (those of sample row / rows_per_sample at gate + sample * gate_stride, scale + sample * mod_stride and shift + sample *
  * mod_stride) are fp32 and may each be NULL. out is written as out_type says, with out_scale [rows] for MKB_OUT_I8 (else
  * NULL). Statistics are fp32, a LayerNorm's squares are taken about its mean. n up to 12288, any alignment (wide accesses where

@@ -109,3 +109,13 @@ def test_python_checks_refuse():
     for call in bad:
         with pytest.raises(mkimage.MkbError):
             call()
+
+
+@pytest.mark.parametrize("change", [
+    dict(out=P, xo=P, out_type=2), dict(out=2 * P, xo=2 * P, out_type=1), dict(out=P, xo=2 * P, out_type=1, y=4 * P),
+    dict(out=P, xo=2 * P, out_type=2, ldo=72, y=4 * P), dict(out=4 * P, xo=2 * P, out_type=2, y=4 * P),
+    dict(out=4 * P, xo=2 * P, out_type=3, osc=P, y=4 * P), dict(out=4 * P, xo=2 * P, out_type=1, ldo=72, y=4 * P),
+    dict(out=P, y=None, y_norm=0, xo=None, out_type=1)])
+def test_gate_add_norm_refuses_an_output_over_its_operands(change):
+    """An output over x_out, or over x or y in another type or at another distance of rows."""
+    _refused(mkimage.lib.mkb_gate_add_norm, _with(NORM, **change), "memory of its own")

@@ -1,6 +1,6 @@
 """Ends of the quantised block's ranges: the negative tail of the projections' GELU, steps at the small end of fp32, a gate's
 tanh on both sides of its two forms, a few query rows of as many key heads as fill the GPU, a pair of CTAs whose
-load never comes. u = 2^-24, half a step of fp32."""
+load never comes, outputs in their operands' places. u = 2^-24, half a step of fp32."""
 
 import math
 
@@ -116,6 +116,29 @@ def test_few_rows_of_many_key_heads(cuda, B, H, Hkv, Lq, Lk, d):
         ref, mag = (p @ vv).transpose(0, 1), (p @ vv.abs()).transpose(0, 1)
         good = bool(((got[b] - ref).abs() <= 2.0 ** -11 * mag + 2.0 ** -8 * ref.abs()).all())
         assert good, b
+
+
+@pytest.mark.parametrize("rows,n", [(5, 640), (700, 1283), (900, 2048)])
+def test_an_output_in_the_place_of_its_operand(cuda, rows, n):
+    """y's rows become the norm (bf16), x's rows too where there is no branch or where x_out is elsewhere (fp32): the same bits
+    as with memory of its own."""
+    import torch
+    import mkimage
+
+    ops = mkimage.ops
+    g = torch.Generator().manual_seed(n)
+    x, y = torch.randn(rows, n, generator=g).to(cuda), torch.randn(rows, n, generator=g).to(torch.bfloat16).to(cuda)
+    args = dict(y_norm=1, x_norm=2, rows_per_sample=rows // 2)
+    xo = torch.empty_like(x)
+    want = ops.gate_add_norm(x, y, x_out=xo, **args)
+    x1, y1 = x.clone(), y.clone()
+    assert torch.equal(ops.gate_add_norm(x1, y1, out=y1, **args), want) and torch.equal(x1, xo)
+    want = ops.gate_add_norm(x, y, x_out=xo, out_type=ops.OUT_F32, **args)
+    x1, x2 = x.clone(), torch.empty_like(x)
+    assert torch.equal(ops.gate_add_norm(x1, y, x_out=x2, out=x1, out_type=ops.OUT_F32, **args), want) and torch.equal(x2, xo)
+    want = ops.gate_add_norm(x, x_norm=1, out_type=ops.OUT_F32)
+    x1 = x.clone()
+    assert torch.equal(ops.gate_add_norm(x1, x_norm=1, out=x1, out_type=ops.OUT_F32), want)
 
 
 def test_a_stalled_pair_gives_up_and_the_context_survives(cuda):
