@@ -192,14 +192,15 @@ mkb_status mkb_attention_kv_arriving(const void* q, int Lq, int Lq_rows, const v
 
 /* Rows to 8-bit integers: scale[r] = max |x[r]| / 127 (fp32) and q[r][i] = x[r][i] / scale[r] rounded to the nearest whole
  * number, ties to even (decided exactly). x is bf16 (x_f32 = 0) or fp32, rows ldx apart; q rows ldq apart. A row of zeros,
- * or with no magnitude above 127 * 2^-126, has scale 0 and zeros; a row holding an infinity or a NaN has scale NaN and
+ * or of magnitudes below 127 * 2^-126, has scale 0 and zeros; a row holding an infinity or a NaN has scale NaN and
  * zeros, so that a projection of it is NaN. Any n up to 2^24. */
 mkb_status mkb_quantize_rows(const void* x, long ldx, int x_f32, int8_t* q, long ldq, float* scale, long rows, int n,
                              void* stream);
 
 /* y[m][n] = act(x_scale[m] * w_scale[n] * sum_k x[m][k] w[n][k] + bias[n]): mkb_proj on 8-bit integers, with the scale of
  * each token (mkb_quantize_rows of the activations) and of each output channel (mkb_quantize_rows of the weight's rows).
- * The sums are exact 32-bit integers (K <= 131071; M and N up to 2^30, and no more 128 x 128 tiles than that). x and w are
+ * The sums are exact 32-bit integers (K <= 131071; M and N up to 2^30, and no more 128 x 128 tiles than that), the rest is fp32,
+ * rounded once for bf16: the activations to a few fp32 roundings of their value (the erf GELU's: of its argument). x and w are
  * 16-byte aligned with ldx and ldw multiples of 16 (K itself may be any: what lies between K and the row's end is not read
  * as data); y is bf16 (out_f32 = 0) or fp32, any ldy >= N. */
 mkb_status mkb_proj_i8(const int8_t* x, long ldx, const float* x_scale, const int8_t* w, long ldw, const float* w_scale,
@@ -232,7 +233,9 @@ mkb_status mkb_gate_add_norm(const float* x, long ldx, float* x_out, long ldxo, 
  * key head h / (H / Hkv). bf16, head_dim 64 or 128; element (b, h, row, i) of q is at
  * q + b * q_sample + h * q_head + row * q_row + i, k, v and out likewise (strides in elements, multiples of 8, 0 where a
  * sample or head is shared; pointers 16-byte aligned): head-major and token-major rows alike. scale <= 0: 1 /
- * sqrt(head_dim). Lk may be 0 (zeros). */
+ * sqrt(head_dim). Lk may be 0 (zeros). Scores, maxima, sums and outputs are held in fp32. The weights are rounded to bf16 before
+ * they meet v, as in mkb_attention, except where (H / Hkv) Lq is 1 or 2, or up to 4 with Lk <= 512: those calls keep them in
+ * fp32, and so may differ from the same rows of a larger call in the last bits. */
 mkb_status mkb_cross_attention(const void* q, long q_row, long q_head, long q_sample, const void* k, long k_row,
                                long k_head, long k_sample, const void* v, long v_row, long v_head, long v_sample, void* out,
                                long out_row, long out_head, long out_sample, int B, int H, int Hkv, int Lq, int Lk,

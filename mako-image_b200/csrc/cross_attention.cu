@@ -16,6 +16,9 @@
 // the key steps each and put the parts together through distributed shared memory: no workspace, no second launch. An item of a
 // single query tile gives it to both softmax groups there, who take the steps in turn as two parts.
 // Only ceil(visible / 16) * 16 keys of the last tile are multiplied and exponentiated (77 keys cost 80, not 128).
+// Scores, maxima, sums and O are fp32. The weights alone are rounded, to bf16, as the second product takes P in V's type: each is
+// off by up to 2^-8 of itself, which leaves results a relative error of 2.0 to 2.1e-3 where their own rounding to bf16 makes
+// 1.7e-3. The sum l adds them before that rounding. k_cross_few keeps fp32 weights (1.7e-3).
 // TMEM columns: S_A [0, 128), S_B [128, 256), O_A [256, 384), O_B [384, 512); P takes the first half of its S.
 #include "cross_attention.cuh"
 #include "common.cuh"
@@ -168,8 +171,8 @@ struct Walk {
     __device__ __forceinline__ int width() const { return min(kTile, (it.n - j * kTile + 15) & ~15); }
 };
 
-// A row's step over CH chunks of 32 keys: its scores in tensor memory at ts to weights 2^(s sc - m), bf16, over the first
-// half of the same columns; the row's maximum m and sum l; O at `to` rescaled where the maximum grew. Of the last chunk only the
+// A row's step over CH chunks of 32 keys: its scores in tensor memory at ts to weights 2^(s sc - m), bf16 (see above), over the
+// first half of the same columns; the row's maximum m and sum l; O at `to` rescaled where the maximum grew. Of the last chunk only the
 // first `tail` keys are visible. With `masked` each score is cut at its key's bound, +inf or -inf (the minimum drops a NaN,
 // and a visible NaN comes back as inf - inf). Straight code for each CH: the chunks' loads, exponentials and stores
 // interleave.

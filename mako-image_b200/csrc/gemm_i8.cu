@@ -411,7 +411,7 @@ template <int BN, bool F32>
 struct PairCfg {
     static constexpr int kABytes = 128 * kBK, kBBytes = BN / 2 * kBK, kStageBytes = kABytes + kBBytes;
     // A warp's boxes of 32 rows of 64 bytes: one for bf16, two for fp32, whose 32 columns are two of them (3679 x 10240 x 1216
-    // with GELU 81 -> 74 us; the stage that they cost 256 columns: 8192 x 3072 x 3072 60.0 -> 61.5).
+    // with GELU, as it was then, 81 -> 74 us, 68 now; the stage that they cost 256 columns: 8192 x 3072 x 3072 60.0 -> 61.5).
     static constexpr int kBox = 32 * 64, kBoxes = F32 ? 2 : 1;
     static constexpr int kStages = BN == 256 ? 6 - F32 : BN == 192 ? 7 - F32 : BN == 160 ? 7 : 8 - F32;
     static constexpr int kVec = 2 * 2 * BN * 4;  // w_scale and bias of two tiles
@@ -456,7 +456,7 @@ __device__ __forceinline__ void store_box(T* p, long ldy, const uint8_t* box, in
 // Persistent CTA pairs. Warp 0 of each CTA loads its 128 rows of x and its half of the W tile by TMA, the leader's warp 1
 // issues 256 x BN x 32 MMAs into one of two accumulators, warps 2-9 of both CTAs drain the other: a thread a row, 32 columns at
 // a time and every second 32 each, through a 2 KB box a warp that leaves as TMA stores. With four such warps and boxes of 4 KB
-// the epilogue was what the tensor pipe waited for (8192 x 12288 x 3072 with GELU 218 us, with eight 205).
+// the epilogue was what the tensor pipe waited for (8192 x 12288 x 3072 with a GELU by tanh.approx 218 us, with eight 205).
 template <int BN, bool F32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1) k_i8_pair(const __grid_constant__ I8Params P)
 {
