@@ -215,7 +215,8 @@ enum { MKB_OUT_NONE = 0, MKB_OUT_BF16 = 1, MKB_OUT_F32 = 2, MKB_OUT_I8 = 3 };
  *   x_out = x + g(gate) * N_y(y) * y_weight         (g: identity, or tanh with tanh_gate)
  *   out   = N_x(x_out) * x_weight * (1 + scale) + shift
  * x, x_out: the fp32 residual stream [rows][n] (x_out may be x; NULL or x where y is NULL, which leaves the residual as it
- * is and only norms it). out may take x's or y's place, row for row in the same type, but not x_out's beside it. y: the branch's output, bf16 or fp32 (y_f32). y_weight and x_weight [n], gate, scale and shift
+ * is and only norms it). x_out and out may take x's or y's place, row for row in the same type, but not each
+ * other's. y: the branch's output, bf16 or fp32 (y_f32). y_weight and x_weight [n], gate, scale and shift
  * (those of sample row / rows_per_sample at gate + sample * gate_stride, scale + sample * mod_stride and shift + sample *
  * mod_stride) are fp32 and may each be NULL. out is written as out_type says, with out_scale [rows] for MKB_OUT_I8 (else
  * NULL). Statistics are fp32, a LayerNorm's squares are taken about its mean. n up to 12288, any alignment (wide accesses where
@@ -233,7 +234,7 @@ mkb_status mkb_gate_add_norm(const float* x, long ldx, float* x_out, long ldxo, 
  * key head h / (H / Hkv). bf16, head_dim 64 or 128; element (b, h, row, i) of q is at
  * q + b * q_sample + h * q_head + row * q_row + i, k, v and out likewise (strides in elements, multiples of 8, 0 where a
  * sample or head is shared; pointers 16-byte aligned): head-major and token-major rows alike. scale <= 0: 1 /
- * sqrt(head_dim). Lk may be 0 (zeros). Scores, maxima, sums and outputs are held in fp32. The weights are rounded to bf16 before
+ * sqrt(head_dim). Lk may be 0 (zeros). Scores, maxima, sums and running outputs are held in fp32. The weights are rounded to bf16 before
  * they meet v, as in mkb_attention, except where (H / Hkv) Lq is 1 or 2, or up to 4 with Lk <= 512: those calls keep them in
  * fp32, and so may differ from the same rows of a larger call in the last bits. */
 mkb_status mkb_cross_attention(const void* q, long q_row, long q_head, long q_sample, const void* k, long k_row,

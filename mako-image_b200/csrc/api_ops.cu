@@ -503,6 +503,8 @@ mkb_status mkb_gate_add_norm(const float* x, long ldx, float* x_out, long ldxo, 
     const bool as_y = out_type == (y_f32 ? MKB_OUT_F32 : MKB_OUT_BF16) && ldo == ldy;
     if (out_type != MKB_OUT_NONE && ((y && out == x_out) || (out == x && !as_x) || (y && out == y && !as_y)))
         return fail(MKB_ERR_INVALID, "gate_add_norm: out is memory of its own, or x's or y's rows in their type and places, not x_out's");
+    if (y && x_out == y && !(y_f32 && ldxo == ldy))
+        return fail(MKB_ERR_INVALID, "gate_add_norm: x_out is memory of its own, or x's or y's fp32 rows in their places");
     GateNormArgs a{x,        ldx,      x_out, ldxo,  y,     ldy,        y_f32,           y_norm, x_norm,
                    tanh_gate, y_weight, gate,  gate_stride, x_weight, scale, shift,       mod_stride, rows_per_sample,
                    eps,      out,      ldo,   out_type, out_scale, rows, n};

@@ -119,3 +119,9 @@ def test_python_checks_refuse():
 def test_gate_add_norm_refuses_an_output_over_its_operands(change):
     """An output over x_out, or over x or y in another type or at another distance of rows."""
     _refused(mkimage.lib.mkb_gate_add_norm, _with(NORM, **change), "memory of its own")
+
+
+@pytest.mark.parametrize("change", [dict(xo=4 * P, y=4 * P), dict(xo=4 * P, y=4 * P, y_f32=1, ldy=72)])
+def test_gate_add_norm_refuses_a_residual_over_the_branch(change):
+    """x_out over a bf16 y, or over an fp32 one at another distance of rows."""
+    _refused(mkimage.lib.mkb_gate_add_norm, _with(NORM, **change), "memory of its own")

@@ -136,6 +136,10 @@ def test_an_output_in_the_place_of_its_operand(cuda, rows, n):
     want = ops.gate_add_norm(x, y, x_out=xo, out_type=ops.OUT_F32, **args)
     x1, x2 = x.clone(), torch.empty_like(x)
     assert torch.equal(ops.gate_add_norm(x1, y, x_out=x2, out=x1, out_type=ops.OUT_F32, **args), want) and torch.equal(x2, xo)
+    yf = y.float()
+    want = ops.gate_add_norm(x, yf, x_out=xo, **args)
+    y1 = yf.clone()
+    assert torch.equal(ops.gate_add_norm(x, y1, x_out=y1, **args), want) and torch.equal(y1, xo)
     want = ops.gate_add_norm(x, x_norm=1, out_type=ops.OUT_F32)
     x1 = x.clone()
     assert torch.equal(ops.gate_add_norm(x1, x_norm=1, out=x1, out_type=ops.OUT_F32), want)
